@@ -197,6 +197,65 @@ int qb_paged_decode_attn_grouped(const void* q, const void* k_cache, const void*
                                  int* err, qb_stream_t stream);
 size_t qb_paged_decode_grouped_workspace_bytes(int batch, int hq, int D, int n_slots);
 
+/* ---------------------------------------------------------------- 8-bit paged KV cache
+ * No counterpart in the reference (its cache is bf16, qwen3_naive.py:1059-1066).  The cache holds
+ * e4m3 codes k_cache / v_cache [num_blocks, hkv, page_size, D] and one fp32 scale per block of 64
+ * tokens and head, k_scale / v_scale [num_blocks, hkv, page_size / 64]; value = code * scale.  Slots,
+ * page ids and block tables are those of the bf16 cache; bt_width is the number of entries of a
+ * block_tables row (a key beyond them sets QB_DEVERR_PAGE, as does a page outside the pool; such keys
+ * are left out).  D = 128, page_size = 256; codes 16-byte aligned.
+ *
+ * The store: QK-norm + RoPE of the projection as in qb_qk_norm_rope_fwd (in fp32 throughout), rotated q
+ * rounded to bf16 into q_out [T, hq, D], rotated k and v rounded to codes at slot_mapping (-1 skips;
+ * a slot outside the pool sets QB_DEVERR_SLOT and is skipped; of two tokens with one slot the later is
+ * kept).  A block's scale is the smallest power of two, at least 2^-126, under which every finite value
+ * appended since its first row lies within 448.  A call that writes the first row of a block begins it
+ * anew; otherwise a larger value raises the scale and the rows already there are rounded again.  What is
+ * not finite is stored as NaN.  The tokens of a call may be in any order. */
+int qb_qk_norm_rope_store_fp8(const void* qkv, int64_t T, int64_t ld_in, int hq, int hkv, int D,
+                              const int64_t* positions, const float* cos_sin, int64_t max_pos,
+                              const void* q_norm_w, const void* k_norm_w, float eps, void* q_out,
+                              void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                              const int32_t* slot_mapping, int64_t num_blocks, int page_size, int* err,
+                              qb_stream_t stream);
+/* Single-token decode attention over that cache; arguments as qb_paged_decode_attn.  q rows q_stride
+ * elements apart (a multiple of 8), heads of a row together; out [batch, hq, D] contiguous.  hq is a
+ * multiple of hkv, hq / hkv <= 16.  split_tokens: a multiple of 64, at most 8192; split_tokens *
+ * max_splits >= every length (keys beyond are left out and set QB_DEVERR_SHAPE).  workspace:
+ * qb_paged_decode_fp8_workspace_bytes(batch, hq, max_splits), any contents; calls that share one must
+ * not overlap. */
+int qb_paged_decode_attn_fp8(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
+                             const float* k_scale, const float* v_scale, int64_t num_blocks,
+                             int page_size, const int32_t* block_tables, int64_t bt_stride, int bt_width,
+                             const int32_t* seqlens, int seqlen_add, int batch, int hq, int hkv, int D,
+                             float scale, int split_tokens, int max_splits, float* workspace, void* out,
+                             int* err, qb_stream_t stream);
+/* The grouped form; arguments as qb_paged_decode_attn_grouped, with the shared and the own keys split
+ * apart: shared_tokens * shared_splits >= every shared_len, own_tokens * own_splits >= every
+ * seqlens[b] + seqlen_add - kv_start[b].  Sequences in no group are left out of `out`; kv_start is a
+ * multiple of 64.  workspace: qb_paged_decode_fp8_workspace_bytes(batch, hq, shared_splits +
+ * own_splits). */
+int qb_paged_decode_attn_grouped_fp8(const void* q, int64_t q_stride, const void* k_cache,
+                                     const void* v_cache, const float* k_scale, const float* v_scale,
+                                     int64_t num_blocks, int page_size, const int32_t* block_tables,
+                                     int64_t bt_stride, int bt_width, const int32_t* seqlens,
+                                     int seqlen_add, int batch, int hq, int hkv, int D, float scale,
+                                     const int32_t* group_members, const int32_t* shared_len,
+                                     int n_groups, const int32_t* kv_start, int shared_tokens,
+                                     int shared_splits, int own_tokens, int own_splits,
+                                     float* workspace, void* out, int* err, qb_stream_t stream);
+size_t qb_paged_decode_fp8_workspace_bytes(int batch, int hq, int n_slots);
+/* Causal attention of the query rows cu_seqlens_q over the first cu_seqlens_k keys of each sequence in
+ * that cache; arguments as the paged form of qb_attn_varlen_fwd.  q and out rows q_stride / o_stride
+ * elements apart (multiples of 8).  hq / hkv <= 16.  Rows in no sequence are left as they were. */
+int qb_attn_paged_prefill_fp8(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
+                              const float* k_scale, const float* v_scale, int64_t num_blocks,
+                              int page_size, const int32_t* block_tables, int64_t bt_stride, int bt_width,
+                              const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,
+                              const int32_t* tile_info, int n_tiles, int tiles_per_seq, int hq, int hkv,
+                              int D, float scale, void* out, int64_t o_stride, int64_t total_q, int* err,
+                              qb_stream_t stream);
+
 /* ---------------------------------------------------------------- lm_head log-prob / sampling
  * Token log-probability from bf16 logits rows; replaces the fp32
  * log_softmax + gather of forward_logprob (qwen3_grpo_train.py:48-52).

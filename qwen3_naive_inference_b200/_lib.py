@@ -64,6 +64,13 @@ SIGNATURES: dict[str, tuple] = {
     "qb_gemm_qk_norm_rope": (I, [P, L, P, L, L, I, I, L, P, P, L, P, P, F, P, L, P, L, P, P, P, P, L, P, P, I, P,
                                  P]),
     "qb_gemm_plan": (I, [L, L, L, I, I, P, P, P]),
+    "qb_qk_norm_rope_store_fp8": (I, [P, L, L, I, I, I, P, P, L, P, P, F, P, P, P, P, P, P, L, I, P, P]),
+    # (q, q_stride, k, v, k_scale, v_scale, num_blocks, page_size, block_tables, bt_stride, bt_width, ...
+    "qb_paged_decode_attn_fp8": (I, [P, L, P, P, P, P, L, I, P, L, I, P, I, I, I, I, I, F, I, I, P, P, P, P]),
+    "qb_paged_decode_attn_grouped_fp8": (I, [P, L, P, P, P, P, L, I, P, L, I, P, I, I, I, I, I, F, P, P, I, P, I, I,
+                                             I, I, P, P, P, P]),
+    "qb_paged_decode_fp8_workspace_bytes": (c_size_t, [I, I, I]),
+    "qb_attn_paged_prefill_fp8": (I, [P, L, P, P, P, P, L, I, P, L, I, P, P, I, P, I, I, I, I, I, F, P, L, L, P, P]),
     "qb_f32_to_bf16": (I, [P, P, L, P]),
     "qb_accumulate_bf16": (I, [P, P, L, P]),
 }

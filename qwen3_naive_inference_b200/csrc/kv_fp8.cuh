@@ -1,0 +1,38 @@
+// The 8-bit paged KV cache: layout constants and conversions shared by the kernels that fill and
+// read it.
+//
+// k_cache / v_cache [num_blocks, hkv, 256, 128] hold e4m3 codes, k_scale / v_scale
+// [num_blocks, hkv, 4] one fp32 scale per block of 64 tokens and head: value = code * scale.  The
+// 64 tokens of a block and head are 8 KB in a row, so one bulk copy brings a tile.
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace {
+
+constexpr int KV8_D = 128;      // head width
+constexpr int KV8_PAGE = 256;   // tokens of a page
+constexpr int KV8_BLOCK = 64;   // tokens that share a scale
+constexpr int KV8_SUBS = KV8_PAGE / KV8_BLOCK;
+constexpr int KV8_TILE = KV8_BLOCK * KV8_D;  // bytes of one block's codes of one head
+
+// Two e4m3 codes (the low 16 bits) as two halves: exact, every code is a half value (NaN stays NaN).
+QB_DEVICE uint32_t e4m3x2_to_half2(uint32_t codes) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo;\n\tcvt.u16.u32 lo, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(codes));
+  return r;
+}
+QB_DEVICE float2 e4m3x2_to_float2(uint32_t codes) {
+  const uint32_t h = e4m3x2_to_half2(codes);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+// Four values as e4m3 codes, round to nearest even; beyond +-448 saturates, NaN stays NaN.
+QB_DEVICE uint32_t float4_to_e4m3x4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+
+}  // namespace

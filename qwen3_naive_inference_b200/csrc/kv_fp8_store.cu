@@ -1,0 +1,343 @@
+// QK-norm + RoPE of a projected token row with the append of its keys and values to the 8-bit paged
+// cache (kv_fp8.cuh); the 8-bit form of the store in qk_norm_rope_fwd8_kernel.
+//
+//   y = x * rsqrt(mean(x^2) + eps) * w,   (lo, hi) -> (lo c - hi s, hi c + lo s)      (fp32)
+//
+// Keys and values go from fp32 to e4m3 in one rounding (no bf16 in between); q is rounded to bf16.
+// A block of 64 tokens and head has one scale: the smallest power of two under which everything
+// appended since the block's first row stays within 448.  A power of two moves a code between scales
+// without a rounding (but for codes that become subnormal, 2^-15 below the block's largest value),
+// so a block may be filled a token at a time: where a later token raises the scale, the rows already
+// there are rounded again under the new one.  A call that writes row 0 of a block begins it anew (a
+// recycled page's old scale is dropped).
+//
+// Work split: one CTA per window of eight tokens and kv head for K and V, further CTAs for q.  All
+// tokens of the call that fall into one block are handled by the CTA whose window holds the first of
+// them, so a block's scale has one writer; the CTA finds the others by scanning the slots (tokens
+// whose left neighbour is in the same block never scan).  A slot given twice takes the later token.
+#include <float.h>
+
+#include "kv_fp8.cuh"
+
+namespace {
+
+constexpr int ST_THREADS = 256, ST_WARPS = ST_THREADS / 32, ST_HALVES = ST_THREADS / 16;
+constexpr int ST_WIN = ST_WARPS;               // tokens of a window: a warp each in a decode step
+constexpr int ST_ROWS = KV8_BLOCK / ST_HALVES;  // rows of a block per half-warp
+constexpr int ST_QH = 4;                       // q heads per half-warp item (one rotation-table row for all)
+
+struct __align__(16) Row8 {  // eight bf16 of a head row
+  uint32_t w[4];
+};
+
+struct StoreParams {
+  const bf16* qkv;
+  int64_t T, ld;
+  int hq, hkv;
+  const int64_t* positions;
+  const float* cos_sin;
+  int64_t max_pos;
+  const bf16* qw;
+  const bf16* kw;
+  float eps;
+  bf16* q_out;
+  uint8_t* codes[2];  // K, V
+  float* scales[2];
+  const int32_t* slots;
+  int64_t num_slots;
+  int n_kv_ctas;
+  int* err;
+};
+
+QB_DEVICE Row8 ld_row(const bf16* p) { return *reinterpret_cast<const Row8*>(p); }
+QB_DEVICE void unpack_row(const Row8& r, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack_bf16x2(r.w[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+QB_DEVICE float half_sum(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+QB_DEVICE float half_max(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+QB_DEVICE int64_t checked_pos(const StoreParams& p, int64_t t, bool tell) {
+  const int64_t pos = p.positions[t];
+  if (pos >= 0 && pos < p.max_pos) return pos;
+  if (tell) qb_set_err(p.err, QB_DEVERR_SHAPE);
+  return 0;
+}
+// cos and sin of the eight rotation-table columns of lane l (columns j and j + 64 turn together)
+QB_DEVICE void ld_rotation(const StoreParams& p, int64_t pos, int l, float (&c)[8], float (&s)[8]) {
+  const float* row = p.cos_sin + pos * KV8_D + (l & 7) * 8;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float4 a = reinterpret_cast<const float4*>(row)[i];
+    const float4 b = reinterpret_cast<const float4*>(row + KV8_D / 2)[i];
+    c[4 * i] = a.x; c[4 * i + 1] = a.y; c[4 * i + 2] = a.z; c[4 * i + 3] = a.w;
+    s[4 * i] = b.x; s[4 * i + 1] = b.y; s[4 * i + 2] = b.z; s[4 * i + 3] = b.w;
+  }
+}
+// QK-norm and rotation of a head row spread over a half-warp (lane l: elements 8l..8l+7).  Every
+// lane of the warp takes part in the shuffles.
+QB_DEVICE void norm_rope(float (&v)[8], const float (&w)[8], const float (&c)[8], const float (&s)[8], float eps,
+                         int l) {
+  const float rstd = qk_rstd(half_sum(qk_sumsq8(v)), eps);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = v[i] * rstd * w[i];
+    const float partner = __shfl_xor_sync(0xffffffffu, x, 8);
+    v[i] = l < 8 ? qk_rope_lo(x, partner, c[i], s[i]) : qk_rope_hi(x, partner, c[i], s[i]);
+  }
+}
+// Largest finite magnitude of a lane's values (what is not finite is stored as NaN, whatever the scale).
+QB_DEVICE float finite_max(const float (&v)[8]) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = fabsf(v[i]);
+    m = fmaxf(m, a <= FLT_MAX ? a : 0.f);
+  }
+  return m;
+}
+// Smallest power of two (at least 2^-126) under which `top` is within 448 = 1.75 * 2^8.
+QB_DEVICE float scale_for(float top) {
+  const uint32_t b = __float_as_uint(top);
+  const int e = (int)(b >> 23) - ((b & 0x7fffffu) <= 0x600000u ? 8 : 7);
+  return __uint_as_float((uint32_t)max(e, 1) << 23);
+}
+QB_DEVICE float scaled(float x, float inv) { return fabsf(x) <= FLT_MAX ? x * inv : __int_as_float(0x7fffffff); }
+QB_DEVICE void st_codes(uint8_t* dst, const float (&v)[8], float inv) {
+  uint2 u;
+  u.x = float4_to_e4m3x4(scaled(v[0], inv), scaled(v[1], inv), scaled(v[2], inv), scaled(v[3], inv));
+  u.y = float4_to_e4m3x4(scaled(v[4], inv), scaled(v[5], inv), scaled(v[6], inv), scaled(v[7], inv));
+  *reinterpret_cast<uint2*>(dst) = u;
+}
+// Rounds the block's rows that this call does not write again under a scale larger by 1 / ratio.
+// `n` threads take part, this one as number `i`.
+QB_DEVICE void round_again(uint8_t* block, const int* row_src, float ratio, int i, int n) {
+  for (int c = i; c < KV8_TILE / 16; c += n) {
+    if (row_src[c >> 3] >= 0) continue;
+    uint4* at = reinterpret_cast<uint4*>(block) + c;
+    uint4 u = *at;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 a = e4m3x2_to_float2(w[k] & 0xffffu), b = e4m3x2_to_float2(w[k] >> 16);
+      w[k] = float4_to_e4m3x4(a.x * ratio, a.y * ratio, b.x * ratio, b.y * ratio);
+    }
+    *at = u;
+  }
+}
+// The block's scale after values up to `top` joined it: the old one unless the block begins anew or
+// `top` needs a larger one.
+QB_DEVICE float joined_scale(float old, float top, bool anew) {
+  const float need = scale_for(top);
+  return anew ? need : fmaxf(old, need);
+}
+
+QB_DEVICE void store_q(const StoreParams& p, int64_t cta) {
+  const int l = threadIdx.x & 15;
+  const int per_token = (p.hq + ST_QH - 1) / ST_QH;
+  const int64_t item = cta * ST_HALVES + (threadIdx.x >> 4);
+  const bool live = item < p.T * per_token;
+  const int64_t t = live ? item / per_token : 0;
+  const int h0 = live ? (int)(item % per_token) * ST_QH : 0;
+  Row8 raw[ST_QH];
+#pragma unroll
+  for (int k = 0; k < ST_QH; ++k)
+    raw[k] = h0 + k < p.hq ? ld_row(p.qkv + t * p.ld + (h0 + k) * KV8_D + l * 8) : Row8{};
+  float c[8], s[8], w[8];
+  ld_rotation(p, checked_pos(p, t, live && l == 0), l, c, s);
+  unpack_row(ld_row(p.qw + l * 8), w);
+#pragma unroll
+  for (int k = 0; k < ST_QH; ++k) {
+    float v[8];
+    unpack_row(raw[k], v);
+    norm_rope(v, w, c, s, p.eps, l);
+    if (live && h0 + k < p.hq) {
+      Row8 o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o.w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+      *reinterpret_cast<Row8*>(p.q_out + (t * p.hq + h0 + k) * KV8_D + l * 8) = o;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(ST_THREADS)
+kv_fp8_store_kernel(StoreParams p) {
+  qb_pdl_trigger();
+  qb_pdl_wait();
+  __shared__ int row_src[ST_WIN][KV8_BLOCK];  // per run head of the window: the token of each row, or -1
+  __shared__ int first[ST_WIN], blocks[ST_WIN], rows[ST_WIN];
+  __shared__ unsigned top[2];
+  if ((int64_t)blockIdx.x >= p.n_kv_ctas) {
+    store_q(p, (int64_t)blockIdx.x - p.n_kv_ctas);
+    return;
+  }
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, l = tid & 15;
+  const int head = blockIdx.x % p.hkv;
+  const int64_t t0 = (int64_t)(blockIdx.x / p.hkv) * ST_WIN;
+
+  // run heads of the window: tokens whose left neighbour is in another block
+  bool heads_here = false;
+  if (tid < ST_WIN) {
+    const int64_t t = t0 + tid;
+    int blk = -1;
+    if (t < p.T) {
+      const int64_t slot = p.slots[t];
+      if (slot >= 0 && slot < p.num_slots) {
+        blk = (int)(slot / KV8_BLOCK);
+        if (t > 0 && p.slots[t - 1] >= 0 && p.slots[t - 1] / KV8_BLOCK == blk) blk = -1;
+      } else if (slot != -1 && head == 0) {
+        qb_set_err(p.err, QB_DEVERR_SLOT);
+      }
+    }
+    blocks[tid] = blk;
+    first[tid] = INT32_MAX;
+    rows[tid] = 0;
+    heads_here = blk >= 0;
+  }
+  for (int i = tid; i < ST_WIN * KV8_BLOCK; i += ST_THREADS) (&row_src[0][0])[i] = -1;
+  if (!__syncthreads_or(heads_here)) return;
+  // every token of the call in one of those blocks
+  for (int64_t t = tid; t < p.T; t += ST_THREADS) {
+    const int slot = p.slots[t];
+    const int blk = slot >= 0 ? slot / KV8_BLOCK : -2;
+#pragma unroll
+    for (int i = 0; i < ST_WIN; ++i)
+      if (blk == blocks[i]) {
+        atomicMin(&first[i], (int)t);
+        if (atomicMax(&row_src[i][slot % KV8_BLOCK], (int)t) < 0) atomicAdd(&rows[i], 1);
+      }
+  }
+  __syncthreads();
+  bool many = false;
+  if (tid < ST_WIN) {
+    if (blocks[tid] >= 0 && first[tid] != (int)(t0 + tid)) blocks[tid] = -1;  // another run head came first
+    many = blocks[tid] >= 0 && rows[tid] > 1;
+  }
+  many = __syncthreads_or(many);
+
+  float kw[8];
+  unpack_row(ld_row(p.kw + l * 8), kw);
+  const int kcol = (p.hq + head) * KV8_D + l * 8, vcol = kcol + p.hkv * KV8_D;
+  if (!many) {
+    // one token per block (a decode step): a warp each, its first half K, its second half V
+    const int blk = blocks[warp];
+    if (blk < 0) return;  // uniform across the warp; no barrier follows
+    const int which = lane >> 4;
+    const int row = p.slots[t0 + warp] % KV8_BLOCK;
+    const int64_t t = row_src[warp][row];  // the later one where a slot is given twice
+    const int64_t at = (int64_t)(blk / KV8_SUBS) * p.hkv + head;  // (page, head)
+    float* scale = p.scales[which] + at * KV8_SUBS + blk % KV8_SUBS;
+    uint8_t* block = p.codes[which] + (at * KV8_SUBS + blk % KV8_SUBS) * KV8_TILE;
+    const float old = *scale;
+    float v[8], y[8], c[8], s[8];
+    unpack_row(ld_row(p.qkv + t * p.ld + (which ? vcol : kcol)), v);
+    ld_rotation(p, checked_pos(p, t, lane == 0 && head == 0), l, c, s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = v[i];
+    norm_rope(y, kw, c, s, p.eps, l);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = which ? v[i] : y[i];
+    const bool anew = row == 0;
+    const float now = joined_scale(old, half_max(finite_max(v)), anew);
+    st_codes(block + row * KV8_D + l * 8, v, 1.f / now);
+    if (l == 0) *scale = now;
+    if (!anew && now > old) round_again(block, row_src[warp], old / now, l, 16);
+    return;
+  }
+  // blocks that take several tokens (prompt chunks), one after another: 16 half-warps on 64 rows
+  for (int i = 0; i < ST_WIN; ++i) {
+    const int blk = blocks[i];
+    if (blk < 0) continue;  // uniform across the CTA
+    __syncthreads();        // `top` of the block before has been read
+    if (tid < 2) top[tid] = 0;
+    __syncthreads();
+    const int64_t at = ((int64_t)(blk / KV8_SUBS) * p.hkv + head) * KV8_SUBS + blk % KV8_SUBS;
+    const float old_k = p.scales[0][at], old_v = p.scales[1][at];
+    float k[ST_ROWS][8];
+    Row8 v[ST_ROWS];
+    float top_k = 0.f, top_v = 0.f;
+#pragma unroll
+    for (int r = 0; r < ST_ROWS; ++r) {
+      const int64_t t = row_src[i][(tid >> 4) + r * ST_HALVES];
+      const bool live = t >= 0;
+      unpack_row(live ? ld_row(p.qkv + t * p.ld + kcol) : Row8{}, k[r]);
+      v[r] = live ? ld_row(p.qkv + t * p.ld + vcol) : Row8{};
+    }
+#pragma unroll
+    for (int r = 0; r < ST_ROWS; ++r) {
+      const int64_t t = row_src[i][(tid >> 4) + r * ST_HALVES];
+      float c[8], s[8];
+      ld_rotation(p, t >= 0 ? checked_pos(p, t, l == 0 && head == 0) : 0, l, c, s);
+      norm_rope(k[r], kw, c, s, p.eps, l);
+      float x[8];
+      unpack_row(v[r], x);
+      top_k = fmaxf(top_k, t >= 0 ? finite_max(k[r]) : 0.f);
+      top_v = fmaxf(top_v, finite_max(x));
+    }
+    top_k = warp_max(top_k);
+    top_v = warp_max(top_v);
+    if (lane == 0) {  // magnitudes are not negative: their bits order as they do
+      atomicMax(&top[0], __float_as_uint(top_k));
+      atomicMax(&top[1], __float_as_uint(top_v));
+    }
+    __syncthreads();
+    const bool anew = row_src[i][0] >= 0;
+    const float now_k = joined_scale(old_k, __uint_as_float(top[0]), anew);
+    const float now_v = joined_scale(old_v, __uint_as_float(top[1]), anew);
+    uint8_t* kb = p.codes[0] + at * KV8_TILE;
+    uint8_t* vb = p.codes[1] + at * KV8_TILE;
+#pragma unroll
+    for (int r = 0; r < ST_ROWS; ++r) {
+      const int row = (tid >> 4) + r * ST_HALVES;
+      if (row_src[i][row] < 0) continue;
+      float x[8];
+      unpack_row(v[r], x);
+      st_codes(kb + row * KV8_D + l * 8, k[r], 1.f / now_k);
+      st_codes(vb + row * KV8_D + l * 8, x, 1.f / now_v);
+    }
+    if (!anew && now_k > old_k) round_again(kb, row_src[i], old_k / now_k, tid, ST_THREADS);
+    if (!anew && now_v > old_v) round_again(vb, row_src[i], old_v / now_v, tid, ST_THREADS);
+    if (tid == 0) {
+      p.scales[0][at] = now_k;
+      p.scales[1][at] = now_v;
+    }
+  }
+}
+
+}  // namespace
+
+extern "C" int qb_qk_norm_rope_store_fp8(const void* qkv, int64_t T, int64_t ld_in, int hq, int hkv, int D,
+                                         const int64_t* positions, const float* cos_sin, int64_t max_pos,
+                                         const void* q_norm_w, const void* k_norm_w, float eps, void* q_out,
+                                         void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                                         const int32_t* slot_mapping, int64_t num_blocks, int page_size, int* err,
+                                         qb_stream_t stream) {
+  QB_CHECK_ARG(T >= 0 && hq > 0 && hkv > 0 && num_blocks >= 0 && max_pos > 0);
+  if (D != KV8_D || page_size != KV8_PAGE) return QB_ERR_UNSUPPORTED;
+  if (T == 0) return QB_OK;
+  QB_CHECK_ARG(qkv && positions && cos_sin && q_norm_w && k_norm_w && q_out && slot_mapping);
+  QB_CHECK_ARG(k_cache && v_cache && k_scale && v_scale);
+  QB_CHECK_ARG(ld_in >= (int64_t)(hq + 2 * hkv) * KV8_D && ld_in % 8 == 0);
+  const auto al16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+  QB_CHECK_ARG(al16(qkv) && al16(cos_sin) && al16(q_norm_w) && al16(k_norm_w) && al16(q_out) && al16(k_cache) &&
+               al16(v_cache));
+  QB_CHECK_ARG(num_blocks <= (int64_t)INT32_MAX / KV8_PAGE);  // slots are int32
+  const int64_t kv = (T + ST_WIN - 1) / ST_WIN * hkv;
+  const int64_t q = (T * ((hq + ST_QH - 1) / ST_QH) + ST_HALVES - 1) / ST_HALVES;
+  QB_CHECK_ARG(T < INT32_MAX && kv + q <= INT32_MAX);
+  StoreParams p{(const bf16*)qkv, T, ld_in, hq, hkv, positions, cos_sin, max_pos, (const bf16*)q_norm_w,
+                (const bf16*)k_norm_w, eps, (bf16*)q_out, {(uint8_t*)k_cache, (uint8_t*)v_cache},
+                {k_scale, v_scale}, slot_mapping, num_blocks * KV8_PAGE, (int)kv, err};
+  return qb_launch(kv_fp8_store_kernel, dim3((unsigned)(kv + q)), dim3(ST_THREADS), 0, (cudaStream_t)stream, 1, p);
+}

@@ -26,7 +26,9 @@ __all__ = [
     "gemm_qk_norm_rope", "qkv_attention", "attention_packed", "attention_paged_prefill",
     "paged_decode_attention", "silu_mul", "add", "linear", "swiglu_linear", "logprob", "sample", "grpo_advantage",
     "grpo_loss", "mask_sum", "build_tiles", "decode_split_plan", "lm_head_logprob",
-    "grpo_logit_loss",
+    "grpo_logit_loss", "kv_cache_fp8", "qk_norm_rope_store_fp8", "paged_decode_attention_fp8",
+    "paged_decode_attention_grouped_fp8", "attention_paged_prefill_fp8", "decode_split_plan_fp8",
+    "grouped_decode_plan_fp8",
 ]
 
 BF16 = torch.bfloat16
@@ -519,6 +521,209 @@ def paged_decode_attention_grouped(q, k_cache, v_cache, block_tables, seqlens, s
                                              _p(group_members), _p(shared_len), group_members.shape[0],
                                              _p(kv_start), split_tokens, s_sh, s_own, _p(workspace), _p(out),
                                              _p(err_flag()), stream_ptr()), "qb_paged_decode_attn_grouped")
+    return out
+
+
+# ---------------------------------------------------------------- 8-bit paged KV cache
+FP8 = torch.float8_e4m3fn
+KV_FP8_PAGE, KV_FP8_BLOCK = 256, 64  # tokens of a page, tokens that share a scale
+
+
+def kv_cache_fp8(num_blocks: int, hkv: int, device=None):
+    """A zeroed 8-bit paged cache: (k_cache, v_cache, k_scale, v_scale), e4m3 codes [num_blocks, hkv,
+    256, 128] and one fp32 scale per 64 tokens and head [num_blocks, hkv, 4]; value = code * scale."""
+    codes = [torch.zeros(num_blocks, hkv, KV_FP8_PAGE, 128, dtype=torch.uint8, device=device).view(FP8)
+             for _ in range(2)]
+    scales = [torch.zeros(num_blocks, hkv, KV_FP8_PAGE // KV_FP8_BLOCK, dtype=torch.float32, device=device)
+              for _ in range(2)]
+    return (*codes, *scales)
+
+
+def _check_kv_fp8(what, k_cache, v_cache, k_scale, v_scale, *others):
+    """(num_blocks, hkv) of an 8-bit cache; refuses tensors the kernels cannot take."""
+    if not k_cache.is_cuda:
+        raise NativeError("qwen3_naive_inference_b200 ops need CUDA tensors (no CPU fallback)")
+    dev = k_cache.get_device()
+    if dev != torch.cuda.current_device():
+        raise NativeError(f"{what}: the tensors must be on the current CUDA device")
+    shape = k_cache.shape
+    if k_cache.dtype != FP8 or v_cache.dtype != FP8 or len(shape) != 4 or shape[2:] != (KV_FP8_PAGE, 128) \
+            or v_cache.shape != shape:
+        raise NativeError(f"{what} needs float8_e4m3fn caches [num_blocks, kv_heads, {KV_FP8_PAGE}, 128]")
+    sshape = (shape[0], shape[1], KV_FP8_PAGE // KV_FP8_BLOCK)
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or k_scale.shape != sshape \
+            or v_scale.shape != sshape:
+        raise NativeError(f"{what} needs fp32 scales [num_blocks, kv_heads, {KV_FP8_PAGE // KV_FP8_BLOCK}]")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
+            and v_scale.is_contiguous()):
+        raise NativeError(f"{what} needs contiguous caches and scales")
+    for t in (v_cache, k_scale, v_scale, *others):
+        if t is not None and t.get_device() != dev:
+            raise NativeError(f"{what}: every tensor must be on the caches' device")
+    return shape[0], shape[1]
+
+
+def _fp8_rows(what, q, hkv):
+    """q [n, hq, 128] bf16 with the heads of a row together and rows on 16-byte boundaries."""
+    if q.dtype != BF16 or q.dim() != 3 or q.shape[2] != 128:
+        raise NativeError(f"{what} needs bf16 queries [n, heads, 128]")
+    hq = q.shape[1]
+    if hq % hkv or hq > 16 * hkv:
+        raise NativeError(f"{what}: {hq} query heads over {hkv} kv heads (a multiple, at most 16 times)")
+    if q.stride(2) != 1 or q.stride(1) != 128 or q.stride(0) % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+    return q
+
+
+def _fp8_ints(what, *ts):
+    for t in ts:
+        if t.dtype != torch.int32 or t.stride(-1) != 1:
+            raise NativeError(f"{what} needs int32 index tensors with unit stride")
+
+
+def _fp8_out(what, out, q, strided=False):
+    if out is None:
+        return torch.empty(q.shape, dtype=BF16, device=q.device)
+    if out.dtype != BF16 or out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != 128 \
+            or out.stride(0) % 8 or out.data_ptr() % 16 or out.get_device() != q.get_device():
+        raise NativeError(f"{what}: out must be bf16 like q, rows on 16-byte boundaries")
+    if not strided and not out.is_contiguous():
+        raise NativeError(f"{what}: out must be contiguous")
+    return out
+
+
+def qk_norm_rope_store_fp8(qkv, positions, cos_sin, q_norm_w, k_norm_w, eps, hq, hkv, k_cache, v_cache, k_scale,
+                           v_scale, slot_mapping):
+    """The 8-bit form of :func:`qk_norm_rope_store`: returns rotated q [T, hq, 128]; rotated k and v go
+    to the rows ``slot_mapping`` (int32, -1 skips) of the 8-bit cache, and the scales of the blocks they
+    enter are raised where they have to be (the rows already there are then rounded again).  A call that
+    writes the first row of a block begins it anew."""
+    num_blocks, hkv_c = _check_kv_fp8("qk_norm_rope_store_fp8", k_cache, v_cache, k_scale, v_scale, qkv, positions,
+                                      cos_sin, q_norm_w, k_norm_w, slot_mapping)
+    T, ld = qkv.shape
+    if hkv_c != hkv or ld != (hq + 2 * hkv) * 128 or qkv.dtype != BF16:
+        raise NativeError(f"qk_norm_rope_store_fp8 needs a bf16 projection [T, ({hq} + 2 * {hkv}) * 128] and a cache "
+                          f"of {hkv} heads")
+    if positions.dtype != torch.long or positions.shape != (T,) or slot_mapping.shape != (T,):
+        raise NativeError("qk_norm_rope_store_fp8 needs int64 positions [T] and int32 slots [T]")
+    _fp8_ints("qk_norm_rope_store_fp8", slot_mapping)
+    if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[1] != 128 or not cos_sin.is_contiguous() \
+            or q_norm_w.dtype != BF16 or k_norm_w.dtype != BF16 or q_norm_w.numel() != 128 or k_norm_w.numel() != 128:
+        raise NativeError("qk_norm_rope_store_fp8 needs an fp32 rotation table [max_pos, 128] and bf16 norm weights")
+    if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
+        qkv = qkv.contiguous()
+    positions, q_norm_w, k_norm_w = positions.contiguous(), q_norm_w.contiguous(), k_norm_w.contiguous()
+    q = torch.empty(T, hq, 128, dtype=BF16, device=qkv.device)
+    check(lib().qb_qk_norm_rope_store_fp8(_p(qkv), T, qkv.stride(0), hq, hkv, 128, _p(positions), _p(cos_sin),
+                                          cos_sin.shape[0], _p(q_norm_w), _p(k_norm_w), eps, _p(q), _p(k_cache),
+                                          _p(v_cache), _p(k_scale), _p(v_scale), _p(slot_mapping), num_blocks,
+                                          KV_FP8_PAGE, _p(err_flag()), stream_ptr()), "qb_qk_norm_rope_store_fp8")
+    return q
+
+
+def decode_split_plan_fp8(batch: int, hkv: int, max_ctx: int, sm_count: int = 148) -> tuple[int, int]:
+    """(split_tokens, max_splits) of :func:`paged_decode_attention_fp8` for sequences of up to ``max_ctx`` keys."""
+    want = max(1, math.ceil(4 * sm_count / max(1, batch * hkv)))
+    split = min(8192, max(64, math.ceil(math.ceil(max(1, max_ctx) / want) / 64) * 64))
+    return split, max(1, math.ceil(max_ctx / split))
+
+
+def grouped_decode_plan_fp8(batch, n_groups, hq, hkv, max_shared, max_own, sm_count=148):
+    """(shared_tokens, shared_splits, own_tokens, own_splits) of :func:`paged_decode_attention_grouped_fp8`."""
+    own, own_splits = decode_split_plan_fp8(batch, hkv, max(1, max_own), sm_count)
+    shared, shared_splits = decode_split_plan_fp8(n_groups, hkv, max(1, max_shared), sm_count)
+    return shared, shared_splits, own, own_splits
+
+
+def workspace_fp8(batch, hq, n_slots, device):
+    """Split-K partials of the 8-bit decode attentions; None where there is one split."""
+    nbytes = lib().qb_paged_decode_fp8_workspace_bytes(batch, hq, n_slots)
+    return torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
+
+
+def _fp8_workspace(what, workspace, batch, hq, n_slots, device):
+    if workspace is None:
+        return workspace_fp8(batch, hq, n_slots, device)
+    if workspace.numel() * workspace.element_size() < lib().qb_paged_decode_fp8_workspace_bytes(batch, hq, n_slots) \
+            or workspace.data_ptr() % 16 or not workspace.is_cuda:
+        raise NativeError(f"{what}: the workspace is too small for {n_slots} splits")
+    return workspace
+
+
+def paged_decode_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_tables, seqlens, scale, seqlen_add=1,
+                               split_tokens=None, max_splits=None, workspace=None, max_ctx=None, out=None):
+    """:func:`paged_decode_attention` over the 8-bit cache; any hq / hkv up to 16.  ``max_ctx`` bounds the
+    longest sequence (keys beyond it are left out and reported); default: what block_tables can name."""
+    what = "paged_decode_attention_fp8"
+    num_blocks, hkv = _check_kv_fp8(what, k_cache, v_cache, k_scale, v_scale, q, block_tables, seqlens, workspace)
+    q = _fp8_rows(what, q, hkv)
+    B, hq, _ = q.shape
+    _fp8_ints(what, block_tables, seqlens)
+    if block_tables.dim() != 2 or block_tables.shape[0] != B or seqlens.shape != (B,):
+        raise NativeError(f"{what} needs block_tables [batch, width] and seqlens [batch]")
+    if split_tokens is None:
+        split_tokens, max_splits = decode_split_plan_fp8(
+            B, hkv, block_tables.shape[1] * KV_FP8_PAGE if max_ctx is None else max_ctx)
+    out = _fp8_out(what, out, q)
+    ws = _fp8_workspace(what, workspace, B, hq, max_splits, q.device)
+    check(lib().qb_paged_decode_attn_fp8(_p(q), q.stride(0), _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale),
+                                         num_blocks, KV_FP8_PAGE, _p(block_tables), block_tables.stride(0),
+                                         block_tables.shape[1], _p(seqlens), seqlen_add, B, hq, hkv, 128, scale,
+                                         split_tokens, max_splits, _p(ws), _p(out), _p(err_flag()), stream_ptr()), "qb_paged_decode_attn_fp8",
+          kernels=2 if max_splits > 1 else 1)
+    return out
+
+
+def paged_decode_attention_grouped_fp8(q, k_cache, v_cache, k_scale, v_scale, block_tables, seqlens, scale,
+                                       group_members, shared_len, kv_start, plan, workspace=None, seqlen_add=1,
+                                       out=None):
+    """:func:`paged_decode_attention_grouped` over the 8-bit cache; ``plan`` from
+    :func:`grouped_decode_plan_fp8`.  Sequences in no group are left out of ``out``."""
+    what = "paged_decode_attention_grouped_fp8"
+    num_blocks, hkv = _check_kv_fp8(what, k_cache, v_cache, k_scale, v_scale, q, block_tables, seqlens, group_members,
+                                    shared_len, kv_start, workspace)
+    q = _fp8_rows(what, q, hkv)
+    B, hq, _ = q.shape
+    _fp8_ints(what, block_tables, seqlens, group_members, shared_len, kv_start)
+    n_groups = shared_len.shape[0]
+    if block_tables.dim() != 2 or block_tables.shape[0] != B or seqlens.shape != (B,) or kv_start.shape != (B,) \
+            or group_members.shape != (n_groups, 8) or not group_members.is_contiguous():
+        raise NativeError(f"{what} needs block_tables [batch, width], seqlens and kv_start [batch], group_members "
+                          "[groups, 8] and shared_len [groups]")
+    shared_tokens, shared_splits, own_tokens, own_splits = plan
+    out = _fp8_out(what, out, q)
+    ws = _fp8_workspace(what, workspace, B, hq, shared_splits + own_splits, q.device)
+    check(lib().qb_paged_decode_attn_grouped_fp8(
+        _p(q), q.stride(0), _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale), num_blocks, KV_FP8_PAGE,
+        _p(block_tables), block_tables.stride(0), block_tables.shape[1], _p(seqlens), seqlen_add, B, hq, hkv, 128, scale,
+        _p(group_members), _p(shared_len), n_groups, _p(kv_start), shared_tokens, shared_splits, own_tokens, own_splits,
+        _p(ws), _p(out), _p(err_flag()), stream_ptr()), "qb_paged_decode_attn_grouped_fp8", kernels=2)
+    return out
+
+
+def attention_paged_prefill_fp8(q, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
+                                block_tables, scale, tiles=None, out=None):
+    """:func:`attention_paged_prefill` over the 8-bit cache; any hq / hkv up to 16.  Query row i of a
+    sequence with Lq rows and Lk keys attends keys 0 .. Lk - Lq + i; rows in no sequence are left out."""
+    what = "attention_paged_prefill_fp8"
+    num_blocks, hkv = _check_kv_fp8(what, k_cache, v_cache, k_scale, v_scale, q, cu_seqlens_q, cu_seqlens_k,
+                                    block_tables, tiles)
+    q = _fp8_rows(what, q, hkv)
+    Tq, hq, _ = q.shape
+    _fp8_ints(what, cu_seqlens_q, cu_seqlens_k, block_tables)
+    batch = cu_seqlens_q.shape[0] - 1
+    if block_tables.dim() != 2 or block_tables.shape[0] < batch or cu_seqlens_k.shape != cu_seqlens_q.shape:
+        raise NativeError(f"{what} needs block_tables [batch, width] and cu_seqlens of batch + 1 entries")
+    if tiles is not None:
+        _fp8_ints(what, tiles)
+    out = _fp8_out(what, out, q, strided=True)
+    tps = (int(max_seqlen_q) + 63) // 64
+    n_tiles = 0 if tiles is None else tiles.numel() // 2
+    check(lib().qb_attn_paged_prefill_fp8(_p(q), q.stride(0), _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale),
+                                          num_blocks, KV_FP8_PAGE, _p(block_tables), block_tables.stride(0),
+                                          block_tables.shape[1], _p(cu_seqlens_q), _p(cu_seqlens_k), batch, _p(tiles),
+                                          n_tiles, tps, hq, hkv, 128, scale, _p(out), out.stride(0), Tq,
+                                          _p(err_flag()), stream_ptr()), "qb_attn_paged_prefill_fp8")
     return out
 
 
