@@ -1,0 +1,619 @@
+// Single-token attention over the 8-bit paged KV cache (kv_fp8.cuh), plain and grouped.
+//
+//   o = sum_j p_j vs_j V_j,   p = softmax_j(scale * ks_j * q . K_j)
+//
+// K_j, V_j the e4m3 codes of key j, ks_j, vs_j the scales of its block of 64 tokens and head.  Every
+// key's 256 bytes of codes are read once and meet hq / hkv query rows (a group's members times that),
+// so the bound is HBM: 2 * (128 + 1/16) bytes a key and kv head.
+//
+// A CTA takes one kv head of one sequence (or of a group's shared prefix) and a range of its keys.  A
+// producer warp brings 64-key tiles (8 KB of K, 8 KB of V: one block's codes lie in a row) by TMA into a
+// ring of stages; four warps take 16 keys of every tile each and never wait for one another: each keeps
+// its own running reference, sum and output, joined once at the end.
+//   S^T = K Q^T    mma m16n8k16: the 16 keys are the M rows, up to eight query rows the N columns.  Codes
+//                  become halves exactly (cvt); q is scaled by a power of two per row, so that its bf16
+//                  value is a half's too.  ks and the softmax scale meet the fp32 sums.
+//   P           =  2^(x - ref), halves.  ref follows the largest score so far minus 7 and moves only when
+//                  a score passes it by 15: P stays below 2^15 and loses nothing above 2^-31 of the largest.
+//   O^T += vs V^T P^T   the 128 head elements are the M rows (8 tiles), the warp's 16 keys the K dimension,
+//                  so a tile's product is one mma per 16 elements: vs, one number a tile, joins with the
+//                  fp32 accumulator, whatever the scales of other tiles are.
+// The order of head elements and keys inside a product is free, so every operand comes straight from
+// 16-byte shared-memory reads (conflict-free under the TMA swizzle) without a transpose but for the
+// byte pairs of V (prmt) and P (movmatrix).
+// Keys past the range count neither in P (their scores are -inf) nor through V (their codes are zeroed,
+// NaN codes of a recycled page included).  Pages outside the pool are reported and their tile skipped.
+#include "attn_fp8.cuh"
+
+namespace {
+
+constexpr int DC_WARPS = 4, DC_THREADS = DC_WARPS * 32 + 32;  // consumers, producer
+constexpr int DC_STAGES = 4;
+constexpr int DC_STAGE_BYTES = 2 * KV8_TILE;       // K then V
+constexpr int DC_MAX_TILES = 128;                  // of one CTA's range (8192 keys)
+constexpr int DC_WS_ROW = KV8_D + 4;               // workspace row: O / l, then ref + log2 l
+constexpr int DC_O_ROW = KV8_D + 4;                // shared-memory row of a warp's output (padded)
+constexpr int DC_META = DC_MAX_TILES * 12 + (2 * DC_STAGES + 1) * 8 + 8 + 2 * DC_WARPS * 16 * 4;
+constexpr int DC_SMEM = DC_STAGES * DC_STAGE_BYTES + DC_META + 1024 /*align*/;
+static_assert(DC_WARPS * 16 * DC_O_ROW * 4 <= DC_STAGES * DC_STAGE_BYTES, "the join reuses the stages");
+constexpr float DC_HEAD = 7.f, DC_SLACK = 15.f;    // ref = max - 7; moves when a score is above ref + 15
+
+struct DecodeP {
+  const bf16* q;
+  int64_t q_stride;
+  const float* ks;
+  const float* vs;
+  int64_t num_blocks;
+  const int32_t* bt;
+  int64_t bt_stride;
+  int bt_width;
+  const int32_t* seqlens;
+  int seqlen_add;
+  int batch, hq, hkv;
+  float scale_log2;
+  int own_tokens, own_splits, n_slots;
+  float* ws;
+  bf16* out;
+  int* err;
+  // grouped
+  const int32_t* members;     // [n_groups, 8], -1 padded
+  const int32_t* shared_len;
+  const int32_t* kv_start;
+  int n_groups, shared_tokens, shared_splits;
+  int chunk, n_chunks;        // members per shared CTA, shared CTAs per group
+  unsigned n_shared;          // shared CTAs; the own CTAs follow
+};
+
+// What a CTA works on: `rows` query rows over keys [begin, end) of table row `table`.
+struct Work {
+  int rows, table, begin, end, slot;
+};
+
+QB_DEVICE void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+QB_DEVICE uint32_t movmatrix_trans(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(a));
+  return d;
+}
+QB_DEVICE uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+QB_DEVICE uint4 lds128(uint32_t addr) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr));
+  return r;
+}
+QB_DEVICE float dc_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Row r of a CTA's work: its sequence and head, or -1.
+template <bool SHARED>
+QB_DEVICE int row_sequence(const DecodeP& p, const int32_t* members, int b, int r) {
+  if (!SHARED) return b;
+  const int m = members[r / (p.hq / p.hkv)];
+  return m >= 0 && m < p.batch ? m : -1;
+}
+
+// One CTA: the work `w` of kv head `kvh`; NT tiles of eight query rows.  `members`: the chunk's member
+// list (shared work), `b`: the sequence (own work).
+template <int NT, bool SHARED>
+QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtensorMap& tv, uint8_t* smem, uint32_t base,
+                           const Work& w, int kvh, const int32_t* members, int b) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int n = (w.end - w.begin + KV8_BLOCK - 1) / KV8_BLOCK;
+  const int group = p.hq / p.hkv;
+  uint8_t* meta = smem + DC_STAGES * DC_STAGE_BYTES;
+  const uint32_t bar = base + DC_STAGES * DC_STAGE_BYTES;  // full[S], empty[S], meta
+  auto full = [&](int s) { return bar + 8 * s; };
+  auto empty = [&](int s) { return bar + 8 * (DC_STAGES + s); };
+  const uint32_t ready = bar + 8 * (2 * DC_STAGES);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(meta + 8 * (2 * DC_STAGES + 1));
+  int* page_of = reinterpret_cast<int*>(meta + 8 * (2 * DC_STAGES + 2));
+  float* ks_of = reinterpret_cast<float*>(page_of + DC_MAX_TILES);
+  float* vs_of = ks_of + DC_MAX_TILES;
+  float* join = vs_of + DC_MAX_TILES;  // [warp][16] ref, [warp][16] l
+
+  if (warp == DC_WARPS) {
+    // ------------------------------------------------------------ producer
+    float ks[DC_MAX_TILES / 32], vs[DC_MAX_TILES / 32];
+#pragma unroll
+    for (int j = 0; j < DC_MAX_TILES / 32; ++j) {
+      const int i = lane + 32 * j;
+      ks[j] = vs[j] = 0.f;
+      if (i >= n) continue;
+      const int blk = w.begin / KV8_BLOCK + i, col = blk / KV8_SUBS;
+      int page = col < p.bt_width ? p.bt[(int64_t)w.table * p.bt_stride + col] : -1;
+      if (page < 0 || page >= p.num_blocks) {
+        qb_set_err(p.err, QB_DEVERR_PAGE);
+        page = -1;
+      } else {
+        const int64_t at = ((int64_t)page * p.hkv + kvh) * KV8_SUBS + blk % KV8_SUBS;
+        ks[j] = p.ks[at];
+        vs[j] = p.vs[at];
+      }
+      page_of[i] = page;
+    }
+    __syncwarp();
+    auto issue = [&](int i) {
+      const int s = i % DC_STAGES, page = page_of[i];
+      if (page < 0) {
+        mbar_arrive(full(s));
+        return;
+      }
+      const int row = ((page * p.hkv + kvh) * KV8_SUBS + (w.begin / KV8_BLOCK + i) % KV8_SUBS) * KV8_BLOCK;
+      const uint32_t at = base + s * DC_STAGE_BYTES;
+      mbar_expect_tx(full(s), DC_STAGE_BYTES);
+      tma_load_2d(at, &tk, 0, row, full(s));
+      tma_load_2d(at + KV8_TILE, &tv, 0, row, full(s));
+    };
+    int issued = 0;
+    if (lane == 0)
+      for (; issued < min(n, DC_STAGES); ++issued) issue(issued);
+#pragma unroll
+    for (int j = 0; j < DC_MAX_TILES / 32; ++j)
+      if (lane + 32 * j < n) {
+        ks_of[lane + 32 * j] = ks[j];
+        vs_of[lane + 32 * j] = vs[j];
+      }
+    __syncwarp();
+    if (lane == 0) {
+      mbar_arrive(ready);
+      for (; issued < n; ++issued) {
+        if (!mbar_wait(empty(issued % DC_STAGES), (uint32_t)(issued / DC_STAGES - 1) & 1u, abort_flag, p.err)) break;
+        issue(issued);
+      }
+      // never leave with a copy in flight into this CTA's shared memory
+      for (int i = max(0, issued - DC_STAGES); i < issued; ++i)
+        mbar_drain(full(i % DC_STAGES), (uint32_t)(i / DC_STAGES) & 1u);
+    }
+    __syncwarp();
+    __syncthreads();
+    __syncthreads();
+    return;
+  }
+  // -------------------------------------------------------------- consumers
+  // Q as B fragments: column g of tile nt is row nt * 8 + g; lane t holds elements 32t .. 32t+31, the two
+  // halves of product kk (chunk kk / 4, word kk % 4 of the codes' 16-byte chunks) at 32t + 4kk.
+  uint32_t qf[NT][8][2];
+  float fac[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = nt * 8 + g;
+    const int s = r < w.rows ? row_sequence<SHARED>(p, members, b, r) : -1;
+    uint4 raw[4];
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (s >= 0)
+        raw[i] = reinterpret_cast<const uint4*>(p.q + (int64_t)s * p.q_stride + (kvh * group + r % group) * KV8_D +
+                                                32 * t)[i];
+      const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = unpack_bf16x2(u[k]);
+        top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+      }
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // the row's largest value goes to [2^9, 2^10): a bf16 value is a half down to 2^-23 of it
+    const int e = max((int)(__float_as_uint(top) >> 23), 10);
+    const float mul = __uint_as_float((uint32_t)(263 - e) << 23);
+    const float back = __uint_as_float((uint32_t)(e - 9) << 23) * p.scale_log2;
+    fac[nt][0] = __shfl_sync(0xffffffffu, back, 8 * t);      // rows 2t and 2t + 1 of the tile
+    fac[nt][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = unpack_bf16x2(u[k]);
+        qf[nt][2 * i + k / 2][k & 1] = pack_half2(f.x * mul, f.y * mul);
+      }
+    }
+  }
+  float o[NT][8][4], ref[NT][2], l[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    ref[nt][0] = ref[nt][1] = -INFINITY;
+    l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+  }
+  bool ok = __all_sync(0xffffffffu, mbar_wait(ready, 0, abort_flag, p.err));
+  for (int i = 0; ok && i < n; ++i) {
+    const int s = i % DC_STAGES;
+    if (!__all_sync(0xffffffffu, mbar_wait(full(s), (uint32_t)(i / DC_STAGES) & 1u, abort_flag, p.err))) {
+      ok = false;
+      break;
+    }
+    const int live = page_of[i] < 0 ? 0 : w.end - w.begin - i * KV8_BLOCK;  // keys of the tile that count
+    if (live > 16 * warp) {
+      const uint32_t kt = base + s * DC_STAGE_BYTES, vt = kt + KV8_TILE;
+      float x[NT][4];
+      {  // scores of keys 16 warp + g and + 8
+        float part[NT][2][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) part[nt][c][0] = part[nt][c][1] = part[nt][c][2] = part[nt][c][3] = 0.f;
+        const uint32_t row = kt + (16 * warp + g) * KV8_D;
+        uint4 k0[2], k1[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t off = (uint32_t)((2 * t + c) ^ g) << 4;
+          k0[c] = lds128(row + off);
+          k1[c] = lds128(row + 8 * KV8_D + off);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t u0[4] = {k0[c].x, k0[c].y, k0[c].z, k0[c].w}, u1[4] = {k1[c].x, k1[c].y, k1[c].z, k1[c].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t a[4] = {e4m3x2_to_half2(u0[k] & 0xffffu), e4m3x2_to_half2(u1[k] & 0xffffu),
+                                   e4m3x2_to_half2(u0[k] >> 16), e4m3x2_to_half2(u1[k] >> 16)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16_16816(part[nt][c], a, qf[nt][4 * c + k][0], qf[nt][4 * c + k][1]);
+          }
+        }
+        const float ks = ks_of[i];
+        const bool in0 = 16 * warp + g < live, in1 = 16 * warp + g + 8 < live;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          x[nt][0] = in0 ? (part[nt][0][0] + part[nt][1][0]) * (fac[nt][0] * ks) : -INFINITY;
+          x[nt][1] = in0 ? (part[nt][0][1] + part[nt][1][1]) * (fac[nt][1] * ks) : -INFINITY;
+          x[nt][2] = in1 ? (part[nt][0][2] + part[nt][1][2]) * (fac[nt][0] * ks) : -INFINITY;
+          x[nt][3] = in1 ? (part[nt][0][3] + part[nt][1][3]) * (fac[nt][1] * ks) : -INFINITY;
+        }
+      }
+      bool far = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        far |= fmaxf(x[nt][0], x[nt][2]) > ref[nt][0] + DC_SLACK || fmaxf(x[nt][1], x[nt][3]) > ref[nt][1] + DC_SLACK;
+      if (__any_sync(0xffffffffu, far)) {  // the first tile, then rarely: move the reference, scale what is there
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float m = fmaxf(x[nt][c], x[nt][c + 2]);
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+            if (m > ref[nt][c] + DC_SLACK) {
+              const float now = m - DC_HEAD, alpha = dc_exp2(ref[nt][c] - now);
+              ref[nt][c] = now;
+              l[nt][c] *= alpha;
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                o[nt][k][c] *= alpha;
+                o[nt][k][c + 2] *= alpha;
+              }
+            }
+          }
+      }
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float r0 = ref[nt][0] == -INFINITY ? 0.f : ref[nt][0], r1 = ref[nt][1] == -INFINITY ? 0.f : ref[nt][1];
+        const float p0 = dc_exp2(x[nt][0] - r0), p1 = dc_exp2(x[nt][1] - r1);
+        const float p2 = dc_exp2(x[nt][2] - r0), p3 = dc_exp2(x[nt][3] - r1);
+        l[nt][0] += p0 + p2;
+        l[nt][1] += p1 + p3;
+        pb[nt][0] = movmatrix_trans(pack_half2(p0, p1));
+        pb[nt][1] = movmatrix_trans(pack_half2(p2, p3));
+      }
+      // V^T: lane (g, t) holds elements 16g .. 16g+15 of keys 2t, 2t+1, 2t+8, 2t+9
+      uint4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int row = 16 * warp + 2 * t + (k & 1) + 8 * (k >> 1);
+        v[k] = lds128(vt + row * KV8_D + ((uint32_t)(g ^ ((2 * t + (k & 1)) & 7)) << 4));
+        if (live < KV8_BLOCK && row >= live) v[k] = make_uint4(0, 0, 0, 0);
+      }
+      const float vs = vs_of[i];
+      const uint32_t vw[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
+                                 {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t lo = __byte_perm(vw[0][k], vw[1][k], half ? 0x7362 : 0x5140);
+          const uint32_t hi = __byte_perm(vw[2][k], vw[3][k], half ? 0x7362 : 0x5140);
+          const uint32_t a[4] = {e4m3x2_to_half2(lo & 0xffffu), e4m3x2_to_half2(lo >> 16),
+                                 e4m3x2_to_half2(hi & 0xffffu), e4m3x2_to_half2(hi >> 16)};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_f16_16816(d, a, pb[nt][0], pb[nt][1]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[nt][2 * k + half][c] = fmaf(vs, d[c], o[nt][2 * k + half][c]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty(s));
+  }
+  // -------------------------------------------------------------- join the four warps
+  __syncthreads();  // the producer has drained its copies: the stages are free
+  float* so = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int r = nt * 8 + 2 * t + c;
+      float sum = l[nt][c];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+      if (r >= w.rows) continue;
+      if (g == 0) {
+        join[warp * 16 + r] = ref[nt][c];
+        join[(DC_WARPS + warp) * 16 + r] = sum;
+      }
+      float4* dst = reinterpret_cast<float4*>(so + (warp * 16 + r) * DC_O_ROW + 16 * g);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        dst[k] = make_float4(o[nt][2 * k][c], o[nt][2 * k][c + 2], o[nt][2 * k + 1][c], o[nt][2 * k + 1][c + 2]);
+    }
+  __syncthreads();
+  if (*abort_flag) return;
+  for (int i = tid; i < w.rows * 32; i += DC_WARPS * 32) {
+    const int r = i >> 5, d = (i & 31) * 4;
+    const int seq = row_sequence<SHARED>(p, members, b, r);
+    float m = -INFINITY, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < DC_WARPS; ++k) m = fmaxf(m, join[k * 16 + r]);
+#pragma unroll
+    for (int k = 0; k < DC_WARPS; ++k) {
+      const float rk = join[k * 16 + r];
+      const float f = rk == -INFINITY ? 0.f : exp2f(rk - m);
+      const float4 x = *reinterpret_cast<const float4*>(so + (k * 16 + r) * DC_O_ROW + d);
+      sum += f * join[(DC_WARPS + k) * 16 + r];
+      acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+    }
+    if (seq < 0) continue;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t row = (int64_t)seq * p.hq + kvh * group + r % group;
+    if (p.n_slots == 1) {
+      uint2 u;
+      u.x = pack_bf16x2(acc.x * inv, acc.y * inv);
+      u.y = pack_bf16x2(acc.z * inv, acc.w * inv);
+      *reinterpret_cast<uint2*>(p.out + row * KV8_D + d) = u;
+    } else {
+      float* ws = p.ws + (row * p.n_slots + w.slot) * DC_WS_ROW;
+      *reinterpret_cast<float4*>(ws + d) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      if (d == 0) ws[KV8_D] = sum == 0.f ? -INFINITY : m + log2f(sum);
+    }
+  }
+}
+
+// A sequence's own keys: [first, len), and the splits of them that hold any.  first is a block's start
+// (-1: it is not).
+QB_DEVICE int own_first(const DecodeP& p, int b) {
+  const int first = p.kv_start ? p.kv_start[b] : 0;
+  return first >= 0 && first % KV8_BLOCK == 0 ? first : -1;
+}
+QB_DEVICE int own_live(const DecodeP& p, int b) {
+  const int first = own_first(p, b), keys = p.seqlens[b] + p.seqlen_add - first;
+  return first < 0 || keys <= 0 ? 0 : min(p.own_splits, (keys + p.own_tokens - 1) / p.own_tokens);
+}
+
+// NTS, NTO: row tiles of a shared and of an own CTA (NTS = 0: no groups).
+template <int NTS, int NTO>
+__global__ void __launch_bounds__(DC_THREADS, 3)
+decode_fp8_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, DecodeP p) {
+  extern __shared__ uint8_t smem_raw[];
+  qb_pdl_trigger();
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  if (threadIdx.x == 0) {
+    const uint32_t bar = base + DC_STAGES * DC_STAGE_BYTES;
+    for (int s = 0; s < DC_STAGES; ++s) {
+      mbar_init(bar + 8 * s, 1);
+      mbar_init(bar + 8 * (DC_STAGES + s), DC_WARPS);
+    }
+    mbar_init(bar + 16 * DC_STAGES, 1);
+    *reinterpret_cast<volatile int*>(smem + DC_STAGES * DC_STAGE_BYTES + 8 * (2 * DC_STAGES + 1)) = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tk)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tv)) : "memory");
+  }
+  __syncthreads();
+  qb_pdl_wait();
+  unsigned i = blockIdx.x;
+  const int group = p.hq / p.hkv;
+  if (NTS > 0 && i < p.n_shared) {
+    const int split = i % p.shared_splits;
+    i /= p.shared_splits;
+    const int kvh = i % p.hkv;
+    i /= p.hkv;
+    const int c = i % p.n_chunks, grp = i / p.n_chunks;
+    const int32_t* members = p.members + grp * 8 + c * p.chunk;
+    const int donor = p.members[grp * 8], keys = p.shared_len[grp];
+    Work w;
+    w.rows = min(p.chunk, 8 - c * p.chunk) * group;
+    w.table = donor;
+    w.begin = split * p.shared_tokens;
+    w.end = min(keys, w.begin + p.shared_tokens);
+    w.slot = split;
+    bool any = false;
+    for (int m = 0; m < 8 - c * p.chunk && m < p.chunk; ++m) any |= members[m] >= 0 && members[m] < p.batch;
+    if (split == p.shared_splits - 1 && w.end < keys && threadIdx.x == 0) qb_set_err(p.err, QB_DEVERR_SHAPE);
+    if (!any || w.begin >= w.end || donor < 0 || donor >= p.batch) return;
+    decode_work<NTS == 0 ? 1 : NTS, true>(p, tk, tv, smem, base, w, kvh, members, 0);
+    return;
+  }
+  i -= p.n_shared;
+  const int split = i % p.own_splits;
+  i /= p.own_splits;
+  const int kvh = i % p.hkv;
+  int b = i / p.hkv;
+  if (NTS > 0) b = p.members[b];
+  if (b < 0 || b >= p.batch) {
+    if (b >= p.batch && threadIdx.x == 0) qb_set_err(p.err, QB_DEVERR_SHAPE);
+    return;
+  }
+  const int len = p.seqlens[b] + p.seqlen_add, first = own_first(p, b);
+  const int64_t begin = (int64_t)first + (int64_t)split * p.own_tokens;
+  if ((first < 0 || (split == p.own_splits - 1 && begin + p.own_tokens < len)) && threadIdx.x == 0)
+    qb_set_err(p.err, QB_DEVERR_SHAPE);
+  if (first < 0) return;
+  Work w;
+  w.rows = group;
+  w.table = b;
+  w.begin = (int)min(begin, (int64_t)max(len, 0));
+  w.end = (int)min((int64_t)max(len, 0), begin + p.own_tokens);
+  w.slot = (NTS > 0 ? p.shared_splits : 0) + split;
+  if (w.begin >= w.end) {
+    if (p.n_slots == 1)  // no keys at all
+      for (int k = threadIdx.x; k < group * KV8_D / 4; k += DC_THREADS)
+        reinterpret_cast<uint2*>(p.out + ((int64_t)b * p.hq + kvh * group) * KV8_D)[k] = make_uint2(0, 0);
+    return;
+  }
+  decode_work<NTO, false>(p, tk, tv, smem, base, w, kvh, nullptr, b);
+}
+
+// Joins the splits of a (sequence, head): a warp each, weights 2^(lse - largest lse).  Only the splits
+// that hold keys were written and are read.
+__global__ void __launch_bounds__(128)
+decode_fp8_join_kernel(DecodeP p) {
+  qb_pdl_trigger();
+  qb_pdl_wait();
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const int h = (int)(item % p.hq);
+  const int64_t entry = item / p.hq;
+  if (entry >= (p.members ? p.n_groups * 8 : p.batch)) return;
+  int b = (int)entry, n_shared = 0;
+  if (p.members) {
+    b = p.members[entry];
+    const int donor = p.members[entry / 8 * 8], keys = p.shared_len[entry / 8];
+    if (b < 0 || b >= p.batch) return;
+    if (donor >= 0 && donor < p.batch && keys > 0)
+      n_shared = min(p.shared_splits, (keys + p.shared_tokens - 1) / p.shared_tokens);
+  }
+  const int own0 = p.members ? p.shared_splits : 0, n = n_shared + own_live(p, b);
+  const float* ws = p.ws + ((int64_t)b * p.hq + h) * p.n_slots * DC_WS_ROW;
+  auto slot = [&](int s) { return ws + (int64_t)(s < n_shared ? s : own0 + s - n_shared) * DC_WS_ROW; };
+  float m = -INFINITY;
+  for (int s = lane; s < n; s += 32) m = fmaxf(m, slot(s)[KV8_D]);
+  m = warp_max(m);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < n; ++s) {
+    const float* at = slot(s);
+    const float lse = at[KV8_D], f = lse == -INFINITY ? 0.f : exp2f(lse - m);
+    const float4 x = *reinterpret_cast<const float4*>(at + lane * 4);
+    sum += f;
+    acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint2 u;
+  u.x = pack_bf16x2(acc.x * inv, acc.y * inv);
+  u.y = pack_bf16x2(acc.z * inv, acc.w * inv);
+  *reinterpret_cast<uint2*>(p.out + ((int64_t)b * p.hq + h) * KV8_D + lane * 4) = u;
+}
+
+template <int NTS, int NTO>
+int launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeP& p, int64_t entries, cudaStream_t st) {
+  static bool attr = false;
+  if (!attr) {
+    if (cudaFuncSetAttribute(decode_fp8_kernel<NTS, NTO>, cudaFuncAttributeMaxDynamicSharedMemorySize, DC_SMEM) !=
+        cudaSuccess)
+      return qb_launch_status();
+    attr = true;
+  }
+  const int64_t ctas = p.n_shared + entries * p.hkv * p.own_splits;
+  if (ctas > INT32_MAX || entries * p.hq > INT32_MAX) return QB_ERR_INVALID;
+  const int rc = qb_launch_ex(decode_fp8_kernel<NTS, NTO>, dim3((unsigned)ctas), dim3(DC_THREADS), DC_SMEM, st, 1, true, tk,
+                              tv, p);
+  if (rc != QB_OK || p.n_slots == 1) return rc;
+  return qb_launch_ex(decode_fp8_join_kernel, dim3((unsigned)((entries * p.hq + 3) / 4)), dim3(128), 0, st, 1, true, p);
+}
+
+bool split_ok(int tokens, int splits) {
+  return tokens > 0 && tokens % KV8_BLOCK == 0 && tokens <= DC_MAX_TILES * KV8_BLOCK && splits >= 1 &&
+         (int64_t)tokens * splits <= INT32_MAX / 2;
+}
+
+}  // namespace
+
+extern "C" int qb_paged_decode_attn_fp8(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
+                                        const float* k_scale, const float* v_scale, int64_t num_blocks, int page_size,
+                                        const int32_t* block_tables, int64_t bt_stride, int bt_width,
+                                        const int32_t* seqlens, int seqlen_add, int batch, int hq, int hkv, int D,
+                                        float scale, int split_tokens, int max_splits, float* workspace, void* out,
+                                        int* err, qb_stream_t stream) {
+  if (D != KV8_D || page_size != KV8_PAGE) return QB_ERR_UNSUPPORTED;
+  QB_CHECK_ARG(batch >= 0 && split_ok(split_tokens, max_splits));
+  if (batch == 0) return QB_OK;
+  const int ok = kv8_check_cache(q, q_stride, k_cache, v_cache, k_scale, v_scale, num_blocks, block_tables, bt_stride,
+                                 bt_width, hq, hkv, out);
+  if (ok != QB_OK) return ok;
+  QB_CHECK_ARG(seqlens && (max_splits == 1 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0)));
+  CUtensorMap tk, tv;
+  if (!kv8_tmap(&tk, k_cache, num_blocks, hkv) || !kv8_tmap(&tv, v_cache, num_blocks, hkv)) return QB_ERR_INVALID;
+  DecodeP p{};
+  p.q = (const bf16*)q; p.q_stride = q_stride; p.ks = k_scale; p.vs = v_scale; p.num_blocks = num_blocks;
+  p.bt = block_tables; p.bt_stride = bt_stride; p.bt_width = bt_width; p.seqlens = seqlens; p.seqlen_add = seqlen_add;
+  p.batch = batch; p.hq = hq; p.hkv = hkv; p.scale_log2 = scale * KV8_LOG2E;
+  p.own_tokens = split_tokens; p.own_splits = max_splits; p.n_slots = max_splits;
+  p.ws = workspace; p.out = (bf16*)out; p.err = err;
+  const cudaStream_t st = (cudaStream_t)stream;
+  return hq / hkv <= 8 ? launch_decode<0, 1>(tk, tv, p, batch, st) : launch_decode<0, 2>(tk, tv, p, batch, st);
+}
+
+extern "C" int qb_paged_decode_attn_grouped_fp8(
+    const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, const float* k_scale,
+    const float* v_scale, int64_t num_blocks, int page_size, const int32_t* block_tables, int64_t bt_stride,
+    int bt_width, const int32_t* seqlens, int seqlen_add, int batch, int hq, int hkv, int D, float scale,
+    const int32_t* group_members, const int32_t* shared_len, int n_groups, const int32_t* kv_start, int shared_tokens,
+    int shared_splits, int own_tokens, int own_splits, float* workspace, void* out, int* err, qb_stream_t stream) {
+  if (D != KV8_D || page_size != KV8_PAGE) return QB_ERR_UNSUPPORTED;
+  QB_CHECK_ARG(batch >= 0 && n_groups >= 0 && n_groups <= INT32_MAX / 8 && split_ok(shared_tokens, shared_splits) &&
+               split_ok(own_tokens, own_splits) && shared_splits <= INT32_MAX - own_splits);
+  if (batch == 0 || n_groups == 0) return QB_OK;
+  const int ok = kv8_check_cache(q, q_stride, k_cache, v_cache, k_scale, v_scale, num_blocks, block_tables, bt_stride,
+                                 bt_width, hq, hkv, out);
+  if (ok != QB_OK) return ok;
+  QB_CHECK_ARG(seqlens && group_members && shared_len && kv_start && workspace &&
+               (reinterpret_cast<uintptr_t>(workspace) & 15) == 0);
+  CUtensorMap tk, tv;
+  if (!kv8_tmap(&tk, k_cache, num_blocks, hkv) || !kv8_tmap(&tv, v_cache, num_blocks, hkv)) return QB_ERR_INVALID;
+  DecodeP p{};
+  p.q = (const bf16*)q; p.q_stride = q_stride; p.ks = k_scale; p.vs = v_scale; p.num_blocks = num_blocks;
+  p.bt = block_tables; p.bt_stride = bt_stride; p.bt_width = bt_width; p.seqlens = seqlens; p.seqlen_add = seqlen_add;
+  p.batch = batch; p.hq = hq; p.hkv = hkv; p.scale_log2 = scale * KV8_LOG2E;
+  p.own_tokens = own_tokens; p.own_splits = own_splits; p.n_slots = shared_splits + own_splits;
+  p.ws = workspace; p.out = (bf16*)out; p.err = err;
+  p.members = group_members; p.shared_len = shared_len; p.kv_start = kv_start; p.n_groups = n_groups;
+  p.shared_tokens = shared_tokens; p.shared_splits = shared_splits;
+  const int group = hq / hkv, row_tiles = group == 1 ? 1 : 2;
+  p.chunk = min(8, row_tiles * 8 / group);
+  p.n_chunks = (8 + p.chunk - 1) / p.chunk;
+  const int64_t shared = (int64_t)n_groups * p.n_chunks * hkv * shared_splits;
+  QB_CHECK_ARG(shared <= INT32_MAX);
+  p.n_shared = (unsigned)shared;
+  const cudaStream_t st = (cudaStream_t)stream;
+  const int64_t entries = (int64_t)n_groups * 8;
+  if (group == 1) return launch_decode<1, 1>(tk, tv, p, entries, st);
+  if (group <= 8) return launch_decode<2, 1>(tk, tv, p, entries, st);
+  return launch_decode<2, 2>(tk, tv, p, entries, st);
+}
+
+extern "C" size_t qb_paged_decode_fp8_workspace_bytes(int batch, int hq, int n_slots) {
+  return n_slots <= 1 ? 0 : (size_t)batch * hq * n_slots * DC_WS_ROW * 4;
+}
