@@ -247,14 +247,20 @@ int qb_paged_decode_attn_grouped_fp8(const void* q, int64_t q_stride, const void
 size_t qb_paged_decode_fp8_workspace_bytes(int batch, int hq, int n_slots);
 /* Causal attention of the query rows cu_seqlens_q over the first cu_seqlens_k keys of each sequence in
  * that cache; arguments as the paged form of qb_attn_varlen_fwd.  q and out rows q_stride / o_stride
- * elements apart (multiples of 8).  hq / hkv <= 16.  Rows in no sequence are left as they were. */
+ * elements apart (multiples of 8).  hq / hkv <= 16.  Rows in no sequence are left as they were.
+ * tile_info has to hold every 64-row tile of a sequence.  With n_splits > 1 the keys are split over
+ * CTAs, split_keys (a multiple of 128) each, and joined by a second kernel; split_keys * n_splits >=
+ * every Lk (keys beyond are left out and set QB_DEVERR_SHAPE); workspace:
+ * qb_attn_paged_prefill_fp8_workspace_bytes(total_q, hq, n_splits), any contents. */
 int qb_attn_paged_prefill_fp8(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
                               const float* k_scale, const float* v_scale, int64_t num_blocks,
                               int page_size, const int32_t* block_tables, int64_t bt_stride, int bt_width,
                               const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,
                               const int32_t* tile_info, int n_tiles, int tiles_per_seq, int hq, int hkv,
-                              int D, float scale, void* out, int64_t o_stride, int64_t total_q, int* err,
+                              int D, float scale, int split_keys, int n_splits, float* workspace,
+                              void* out, int64_t o_stride, int64_t total_q, int* err,
                               qb_stream_t stream);
+size_t qb_attn_paged_prefill_fp8_workspace_bytes(int64_t total_q, int hq, int n_splits);
 
 /* ---------------------------------------------------------------- lm_head log-prob / sampling
  * Token log-probability from bf16 logits rows; replaces the fp32

@@ -1,13 +1,58 @@
-// Attention over the 8-bit paged KV cache (kv_fp8.cuh): decode, grouped decode, prefill.
+// Causal attention of query chunks over the 8-bit paged KV cache (kv_fp8.cuh) on tcgen05 + TMEM.
 //
-//   o = sum_j p_j vs_j V_j,   p = softmax_j(scale * ks_j * q . K_j)
+//   o_i = sum_j p_ij vs_j V_j,   p_i = softmax_j(scale * ks_j * q_i . K_j),   j <= Lk - Lq + i
 //
-// K_j, V_j the e4m3 codes of key j, ks_j, vs_j the scales of its block and head.
+// K_j, V_j the e4m3 codes of key j, ks_j, vs_j the scales of its block of 64 tokens and head.  Bound by
+// the tensor pipe (4 * 128 flops per query, head and key) and, as near, by the exponentials.
+//
+// A CTA takes up to 256 query rows of one sequence and kv head -- row R is query position R / group, head
+// R % group, so the group's heads share every key -- as two tiles of 128 rows, A and B, and walks the
+// keys in tiles of 128:
+//   warps 0-3, 4-7  softmax of tile A, of tile B: a thread per row
+//   warps 8-11      convert: codes come from global memory a tile ahead, become halves (exactly) and go
+//                   to shared memory in the swizzled layout of the MMA operands
+//   warp 12         one thread issues the MMAs:  S_x = Q_x K^T (both operands in shared memory),
+//                   O_x += P_x V (P_x from TMEM, over the columns of S_x)
+// While one tile's softmax runs, the tensor pipe works on the other's products.  TMEM: S_A, S_B, O_A, O_B
+// of 128 columns each.
+// Q enters as halves scaled by a power of two per row (its largest value in [2^9, 2^10): bf16 values stay
+// exact down to 2^-23 of it); ks and the softmax scale meet the fp32 scores.  P = 2^(x - ref) is rounded
+// to halves: ref is set 4 below the largest score and moved when a score passes it by 12.  vs joins P
+// relative to a reference of its own, which follows the blocks' scales (moved when one is over 8 times it),
+// so O counts in units of that reference; a block whose scale is 2^-10 of it or less is weighed after the
+// sum l has taken its probabilities.
+// Keys behind a row's last one take a score of -inf; their V must not count either, so codes past the
+// sequence are zeroed and, in tiles that some row sees in part, NaN codes of V are zeroed too and their
+// keys noted: a row that does attend such a key becomes NaN.
+// Few rows over many keys: the keys are split over CTAs, which write normalised partial outputs and the
+// rows' log-sums for a second kernel to join.
+// Every wait is bounded (~2 s): on timeout QB_DEVERR_TIMEOUT is raised, all roles leave, TMEM is freed.
 #include "attn_fp8.cuh"
+#include "tcgen05.cuh"
 
 namespace {
 
-struct RowParams {
+constexpr int PF_KEYS = 128;                       // keys of a tile: two blocks
+constexpr int PF_ROWS = 128;                       // rows of a query tile
+constexpr int PF_THREADS = 13 * 32;
+constexpr int PF_HALF = 128 * 64 * 2;              // [128 x 64] halves: 16 KB
+constexpr int PF_TILE = 2 * PF_HALF;               // [128 x 128]: element halves 0-63, 64-127
+constexpr int PF_STAGES = 2;
+constexpr int PF_Q = 0, PF_K = 2 * PF_TILE, PF_V = PF_K + PF_STAGES * PF_TILE;
+constexpr int PF_META = PF_V + PF_STAGES * PF_TILE;
+constexpr int PF_SLOTS = 4;                        // tiles whose scales are held
+constexpr int PF_BARS = 17;
+// barriers; TMEM slot, abort flag; row factors; per slot two ks, two vs, four words of NaN keys
+constexpr int PF_SMEM = PF_META + PF_BARS * 8 + 8 + 2 * PF_ROWS * 4 + PF_SLOTS * 32 + 1024 /*align*/;
+constexpr uint32_t PF_COL_S = 0, PF_COL_O = 256;   // + 128 * tile
+constexpr float PF_HEAD = 4.f, PF_SLACK = 12.f, PF_VSLACK = 8.f, PF_VLOW = 1.f / 1024;
+constexpr int PF_WS_ROW = KV8_D + 4;
+
+// kind::f16, D fp32, A and B f16, M = N = 128; S: both K-major, O: B (V) MN-major.
+constexpr uint32_t PF_IDESC_S = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+constexpr uint32_t PF_IDESC_O = PF_IDESC_S | (1u << 16);
+
+struct PrefillP {
   const bf16* q;
   int64_t q_stride;
   const uint8_t* k;
@@ -18,113 +63,568 @@ struct RowParams {
   const int32_t* bt;
   int64_t bt_stride;
   int bt_width;
-  const int32_t* seqlens;
-  int seqlen_add;
-  int batch, hq, hkv;  // batch: table rows
-  float scale_log2;
-  int n_groups;
-  const int32_t* members;
-  const int32_t* shared_len;
-  const int32_t* kv_start;
   const int32_t* cu_q;
   const int32_t* cu_k;
+  int batch;
+  const int32_t* tiles;  // nullable [n, 2]: (sequence, first row of a 64-row tile)
+  int tiles_per_seq;     // without tiles: of `unit` rows
+  int hq, hkv, pos_per_cta, unit;  // unit = max(64, pos_per_cta): rows a grid tile stands for
+  float scale_log2;
+  int split_keys, n_splits;
+  float* ws;
   bf16* out;
-  int64_t out_stride;
+  int64_t o_stride;
+  int64_t total_q;
   int* err;
 };
 
-struct RowState {
-  float q[4], o[4], m, l;
+QB_DEVICE uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+QB_DEVICE void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+QB_DEVICE void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// 16-byte chunk c (of 16) of row r of a [128 x 128] half tile in the swizzled operand layout
+QB_DEVICE uint32_t operand_chunk(int r, int c) {
+  return (uint32_t)((c >> 3) * PF_HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+struct PrefillSmem {
+  uint32_t base;
+  uint8_t* ptr;
+  QB_DEVICE uint32_t q(int x) const { return base + PF_Q + x * PF_TILE; }
+  QB_DEVICE uint32_t k(int s) const { return base + PF_K + s * PF_TILE; }
+  QB_DEVICE uint32_t v(int s) const { return base + PF_V + s * PF_TILE; }
+  QB_DEVICE uint32_t bar(int i) const { return base + PF_META + 8 * i; }
+  QB_DEVICE uint32_t q_full(int x) const { return bar(x); }
+  QB_DEVICE uint32_t k_full(int s) const { return bar(2 + s); }
+  QB_DEVICE uint32_t k_empty(int s) const { return bar(4 + s); }
+  QB_DEVICE uint32_t v_full(int s) const { return bar(6 + s); }
+  QB_DEVICE uint32_t v_empty(int s) const { return bar(8 + s); }
+  QB_DEVICE uint32_t s_full(int x) const { return bar(10 + x); }
+  QB_DEVICE uint32_t p_ready(int x) const { return bar(12 + x); }
+  QB_DEVICE uint32_t pv_done(int x) const { return bar(14 + x); }
+  QB_DEVICE uint32_t all_done() const { return bar(16); }
+  QB_DEVICE uint32_t* tmem_slot() const { return reinterpret_cast<uint32_t*>(ptr + PF_META + 8 * PF_BARS); }
+  QB_DEVICE volatile int* abort_flag() const { return reinterpret_cast<volatile int*>(tmem_slot() + 1); }
+  QB_DEVICE float* row_fac() const { return reinterpret_cast<float*>(tmem_slot() + 2); }
+  // slot of tile j: ks of its two blocks (negative: no such page), vs of both, bits of its NaN keys
+  QB_DEVICE float* scales(int j) const { return row_fac() + 2 * PF_ROWS + (j % PF_SLOTS) * 8; }
+  QB_DEVICE uint32_t* nan_keys(int j) const { return reinterpret_cast<uint32_t*>(scales(j) + 4); }
 };
 
-// Keys [a, b) of the pages of table row `tb` for one query row, one key at a time: a warp, four
-// elements of the head a lane.
-QB_DEVICE void row_keys(const RowParams& p, RowState& s, int64_t tb, int kvh, int a, int b, int lane) {
-  for (int j = a; j < b; ++j) {
-    const int w = j / KV8_PAGE;
-    const int page = w < p.bt_width ? p.bt[tb * p.bt_stride + w] : -1;
-    if (page < 0 || page >= p.num_blocks) {
-      if (lane == 0) qb_set_err(p.err, QB_DEVERR_PAGE);
-      continue;
+// What a CTA works on.
+struct PrefillWork {
+  int b, q0, lq, shift, kvh;  // sequence, first query position, queries, Lk - Lq
+  int64_t row0;               // row of the sequence's first query
+  int rows, begin, end;       // query rows; keys [begin, end)
+  int n[2];                   // key tiles of query tiles A and B
+};
+
+// Sixteen codes as halves into chunks 2c and 2c + 1 of row r.
+QB_DEVICE void put_codes(uint32_t tile, int r, int c, const uint4& u) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  uint32_t h[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    h[2 * i] = e4m3x2_to_half2(w[i] & 0xffffu);
+    h[2 * i + 1] = e4m3x2_to_half2(w[i] >> 16);
+  }
+  // the eight threads of a row write even chunks of one half and odd chunks of the other at a time
+  const int first = c >> 2;
+  const uint32_t a0 = tile + operand_chunk(r, 2 * c + first), a1 = tile + operand_chunk(r, 2 * c + 1 - first);
+  st_shared16(a0, first ? h[4] : h[0], first ? h[5] : h[1], first ? h[6] : h[2], first ? h[7] : h[3]);
+  st_shared16(a1, first ? h[0] : h[4], first ? h[1] : h[5], first ? h[2] : h[6], first ? h[3] : h[7]);
+}
+// Bits 7 of the bytes of w that hold a NaN code.
+QB_DEVICE uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// ------------------------------------------------------------------ converters
+QB_DEVICE void prefill_convert(const PrefillP& p, const PrefillSmem& sm, const PrefillWork& w) {
+  const int tid = threadIdx.x - 8 * 32, n = max(w.n[0], w.n[1]);
+  const int chunk = tid & 7, row0 = tid >> 3;  // keys row0 + 16 i, i < 8: block i / 4
+  const int first_masked = w.shift + w.q0 + 1;  // keys from here on are behind the first row's last one
+  uint4 kr[8], vr[8];
+  // Codes of key tile j in registers (rows past the keys and tiles without a page: zero)
+  int64_t at[2];
+  auto find = [&](int j) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = w.begin + j * PF_KEYS + h * KV8_BLOCK, col = key / KV8_PAGE;
+      at[h] = -1;
+      if (key >= w.end) continue;
+      const int page = col < p.bt_width ? p.bt[(int64_t)w.b * p.bt_stride + col] : -1;
+      if (page >= 0 && page < p.num_blocks)
+        at[h] = ((int64_t)page * p.hkv + w.kvh) * KV8_SUBS + key % KV8_PAGE / KV8_BLOCK;
+      else if (tid == 0)
+        qb_set_err(p.err, QB_DEVERR_PAGE);
     }
-    const int64_t at = (int64_t)page * p.hkv + kvh;
-    const int64_t row = (at * KV8_PAGE + j % KV8_PAGE) * KV8_D + lane * 4;
-    const uint32_t kw = *reinterpret_cast<const uint32_t*>(p.k + row);
-    const uint32_t vw = *reinterpret_cast<const uint32_t*>(p.v + row);
-    const int sub = j % KV8_PAGE / KV8_BLOCK;
-    const float2 k0 = e4m3x2_to_float2(kw & 0xffffu), k1 = e4m3x2_to_float2(kw >> 16);
-    const float2 v0 = e4m3x2_to_float2(vw & 0xffffu), v1 = e4m3x2_to_float2(vw >> 16);
-    float x = s.q[0] * k0.x + s.q[1] * k0.y + s.q[2] * k1.x + s.q[3] * k1.y;
-    x = warp_sum(x) * p.ks[at * KV8_SUBS + sub] * p.scale_log2;
-    const float m = fmaxf(s.m, x), alpha = exp2f(s.m - m), e = exp2f(x - m);
-    const float ev = e * p.vs[at * KV8_SUBS + sub];
-    s.m = m;
-    s.l = s.l * alpha + e;
-    s.o[0] = s.o[0] * alpha + ev * v0.x;
-    s.o[1] = s.o[1] * alpha + ev * v0.y;
-    s.o[2] = s.o[2] * alpha + ev * v1.x;
-    s.o[3] = s.o[3] * alpha + ev * v1.y;
+  };
+  auto load = [&](const uint8_t* codes, uint4 (&r)[8], const int64_t (&at)[2], int j) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int key = row0 + 16 * i;
+      r[i] = make_uint4(0, 0, 0, 0);
+      if (at[i >> 2] >= 0 && w.begin + j * PF_KEYS + key < w.end)
+        r[i] = *reinterpret_cast<const uint4*>(codes + at[i >> 2] * KV8_TILE + (key % KV8_BLOCK) * KV8_D + chunk * 16);
+    }
+  };
+  find(0);
+  int64_t now[2] = {at[0], at[1]};
+  load(p.k, kr, now, 0);
+  load(p.v, vr, now, 0);
+  for (int j = 0; j < n; ++j) {
+    const int s = j % PF_STAGES;
+    const uint32_t ph = ((uint32_t)(j / PF_STAGES) & 1u) ^ 1u;
+    if (j + 1 < n) find(j + 1);
+    if (!mbar_wait(sm.k_empty(s), ph, sm.abort_flag(), p.err)) return;
+    if (tid < 2) {
+      sm.scales(j)[tid] = now[tid] >= 0 ? p.ks[now[tid]] : -1.f;
+      sm.scales(j)[2 + tid] = now[tid] >= 0 ? p.vs[now[tid]] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) put_codes(sm.k(s), row0 + 16 * i, chunk, kr[i]);
+    if (j + 1 < n) load(p.k, kr, at, j + 1);
+    fence_async_shared();
+    mbar_arrive(sm.k_full(s));
+    if (!mbar_wait(sm.v_empty(s), ph, sm.abort_flag(), p.err)) return;
+    if (w.begin + (j + 1) * PF_KEYS > first_masked) {
+      // some row sees this tile in part: no NaN may reach the product of a masked key
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t bad[4] = {nan_bytes(vr[i].x), nan_bytes(vr[i].y), nan_bytes(vr[i].z), nan_bytes(vr[i].w)};
+        if (bad[0] | bad[1] | bad[2] | bad[3]) {
+          vr[i].x &= ~((bad[0] >> 7) * 0xffu);
+          vr[i].y &= ~((bad[1] >> 7) * 0xffu);
+          vr[i].z &= ~((bad[2] >> 7) * 0xffu);
+          vr[i].w &= ~((bad[3] >> 7) * 0xffu);
+          const int key = row0 + 16 * i;
+          atomicOr(&sm.nan_keys(j)[key >> 5], 1u << (key & 31));
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) put_codes(sm.v(s), row0 + 16 * i, chunk, vr[i]);
+    if (j + 1 < n) load(p.v, vr, at, j + 1);
+    now[0] = at[0];
+    now[1] = at[1];
+    fence_async_shared();
+    mbar_arrive(sm.v_full(s));
   }
 }
-QB_DEVICE void row_begin(const RowParams& p, RowState& s, int64_t row, int h, int lane) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p.q + row * p.q_stride + h * KV8_D + lane * 4);
-  const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y);
-  s.q[0] = a.x; s.q[1] = a.y; s.q[2] = b.x; s.q[3] = b.y;
-  s.o[0] = s.o[1] = s.o[2] = s.o[3] = 0.f;
-  s.m = -INFINITY;
-  s.l = 0.f;
-}
-QB_DEVICE void row_end(const RowParams& p, const RowState& s, int64_t row, int h, int lane) {
-  const float inv = s.l > 0.f ? 1.f / s.l : (s.l == 0.f ? 0.f : s.l);
-  uint2 u;
-  u.x = pack_bf16x2(s.o[0] * inv, s.o[1] * inv);
-  u.y = pack_bf16x2(s.o[2] * inv, s.o[3] * inv);
-  *reinterpret_cast<uint2*>(p.out + row * p.out_stride + h * KV8_D + lane * 4) = u;
+
+// ------------------------------------------------------------------ MMA issuer
+QB_DEVICE void prefill_mma(const PrefillP& p, const PrefillSmem& sm, const PrefillWork& w, uint32_t tmem) {
+  volatile int* ab = sm.abort_flag();
+  const int n = max(w.n[0], w.n[1]);
+  bool ok = mbar_wait(sm.q_full(0), 0, ab, p.err) && (w.n[1] == 0 || mbar_wait(sm.q_full(1), 0, ab, p.err));
+  auto scores = [&](int x, int j) {
+    const uint32_t k = sm.k(j % PF_STAGES);
+    tc_fence_after();
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      umma_bf16(tmem + PF_COL_S + x * 128, sw128_kmajor_desc(sm.q(x) + (i >> 2) * PF_HALF + (i & 3) * 32),
+                sw128_kmajor_desc(k + (i >> 2) * PF_HALF + (i & 3) * 32), PF_IDESC_S, i > 0);
+    umma_commit(sm.s_full(x));
+  };
+  ok = ok && mbar_wait(sm.k_full(0), 0, ab, p.err);
+  if (ok) {
+    for (int x = 0; x < 2; ++x)
+      if (w.n[x] > 0) scores(x, 0);
+    umma_commit(sm.k_empty(0));
+  }
+  for (int j = 0; ok && j < n; ++j) {
+    const int s = j % PF_STAGES;
+    ok = mbar_wait(sm.v_full(s), (uint32_t)(j / PF_STAGES) & 1u, ab, p.err);
+    if (ok && j + 1 < n) ok = mbar_wait(sm.k_full((j + 1) % PF_STAGES), (uint32_t)((j + 1) / PF_STAGES) & 1u, ab, p.err);
+    for (int x = 0; ok && x < 2; ++x) {
+      if (j >= w.n[x]) continue;
+      if (!(ok = mbar_wait(sm.p_ready(x), (uint32_t)j & 1u, ab, p.err))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < 8; ++i)  // 128 keys in steps of 16: P columns 8 i, V rows 16 i
+        umma_bf16_ts(tmem + PF_COL_O + x * 128, tmem + PF_COL_S + x * 128 + 8 * i,
+                     sw128_mn_desc(sm.v(s) + i * 16 * 128, PF_HALF), PF_IDESC_O, (j > 0 || i > 0) ? 1u : 0u);
+      umma_commit(sm.pv_done(x));
+      if (j + 1 < w.n[x]) {  // the next scores go over P's columns: its product has to be through
+        if (!(ok = mbar_wait(sm.pv_done(x), (uint32_t)j & 1u, ab, p.err))) break;
+        scores(x, j + 1);
+      }
+    }
+    if (ok) {
+      umma_commit(sm.v_empty(s));
+      if (j + 1 < n) umma_commit(sm.k_empty((j + 1) % PF_STAGES));
+    }
+  }
+  // no MMA may still be reading shared memory or writing TMEM when the CTA leaves
+  umma_commit(sm.all_done());
+  mbar_drain(sm.all_done(), 0);
 }
 
+// ------------------------------------------------------------------ softmax
+// Query tile x into shared memory as halves: a half-warp per row, 16 rows each.
+QB_DEVICE void prefill_load_q(const PrefillP& p, const PrefillSmem& sm, const PrefillWork& w, int x) {
+  const int tid = threadIdx.x & 127, l = tid & 15, group = p.hq / p.hkv;
+#pragma unroll 4
+  for (int i = 0; i < 16; ++i) {
+    const int r = (tid >> 4) + 8 * i, R = x * PF_ROWS + r;
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (R < w.rows)
+      u = *reinterpret_cast<const uint4*>(p.q + (w.row0 + w.q0 + R / group) * p.q_stride +
+                                          (w.kvh * group + R % group) * KV8_D + l * 8);
+    const uint32_t raw[4] = {u.x, u.y, u.z, u.w};
+    float f[8], top = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 g = unpack_bf16x2(raw[k]);
+      f[2 * k] = g.x;
+      f[2 * k + 1] = g.y;
+      top = fmaxf(top, fmaxf(fabsf(g.x), fabsf(g.y)));
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int e = max((int)(__float_as_uint(top) >> 23), 10);
+    float mul = __uint_as_float((uint32_t)(263 - e) << 23);
+    if (p.scale_log2 < 0.f) mul = -mul;  // the scores' factor is then positive
+    if (l == 0) sm.row_fac()[R] = __uint_as_float((uint32_t)(e - 9) << 23) * fabsf(p.scale_log2);
+    st_shared16(sm.q(x) + operand_chunk(r, l), pack_half2(f[0] * mul, f[1] * mul), pack_half2(f[2] * mul, f[3] * mul),
+                pack_half2(f[4] * mul, f[5] * mul), pack_half2(f[6] * mul, f[7] * mul));
+  }
+  fence_async_shared();
+}
+
+QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const PrefillWork& w, uint32_t tmem, int x,
+                               int split) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = (warp & 3) * 32 + lane, R = x * PF_ROWS + r;
+  const int group = p.hq / p.hkv, n = w.n[x];
+  if (n == 0) return;
+  prefill_load_q(p, sm, w, x);
+  mbar_arrive(sm.q_full(x));
+  // the factors of this warp's rows come from other warps: wait for all 128 threads
+  volatile int* ab = sm.abort_flag();
+  bool ok = __all_sync(0xffffffffu, mbar_wait(sm.q_full(x), 0, ab, p.err));
+  const float fac = ok ? sm.row_fac()[R] : 0.f;
+  const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+  const uint32_t s_at = lanes + PF_COL_S + x * 128, o_at = lanes + PF_COL_O + x * 128;
+  const bool live = R < w.rows;
+  const int pos = w.q0 + R / group;
+  const int last = live ? min(w.shift + pos, w.end - 1) : w.begin - 1;  // the row's last key here
+  float ref = -INFINITY, l = 0.f, vref = 0.f;
+  for (int j = 0; ok && j < n; ++j) {
+    // tcgen05 loads and stores are warp-collective: every decision that leads to them is warp-uniform
+    if (!__all_sync(0xffffffffu, mbar_wait(sm.s_full(x), (uint32_t)j & 1u, ab, p.err))) {
+      ok = false;
+      break;
+    }
+    tc_fence_after();
+    const float* sc = sm.scales(j);
+    const float ks0 = sc[0], ks1 = sc[1], vs0 = sc[2], vs1 = sc[3];
+    const int k0 = w.begin + j * PF_KEYS;
+    const int seen = last - k0 + 1;  // keys of the tile that the row sees
+    const bool whole = __all_sync(0xffffffffu, seen >= PF_KEYS) && ks0 >= 0.f && ks1 >= 0.f;
+    float top[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t v[64];
+      tmem_ld32_nowait(s_at + 64 * h, v);
+      tmem_ld32_nowait(s_at + 64 * h + 32, v + 32);
+      tmem_ld_wait();
+      float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) m[i & 3] = fmaxf(m[i & 3], __uint_as_float(v[i]));
+      } else if ((h ? ks1 : ks0) >= 0.f) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+          if (64 * h + i < seen) m[i & 3] = fmaxf(m[i & 3], __uint_as_float(v[i]));
+      }
+      top[h] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    }
+    const float f0 = fac * fmaxf(ks0, 0.f), f1 = fac * fmaxf(ks1, 0.f);
+    // -inf (nothing seen) times a factor of zero would be NaN
+    const float t0 = top[0] == -INFINITY ? -INFINITY : top[0] * f0, t1 = top[1] == -INFINITY ? -INFINITY : top[1] * f1;
+    const float mt = fmaxf(t0, t1);
+    const bool need = mt > ref + PF_SLACK;
+    const float vtop = fmaxf(vs0, vs1);
+    const bool vneed = vtop > vref * PF_VSLACK;  // the same for every thread of the CTA
+    float a = 1.f;
+    if (need) {
+      const float to = mt - PF_HEAD;
+      a = ref == -INFINITY ? 0.f : fast_exp2(ref - to);
+      ref = to;
+      l *= a;
+    }
+    if (vneed) {
+      a *= vref / vtop;
+      vref = vtop;
+    }
+    if (j > 0 && __any_sync(0xffffffffu, need || vneed)) {
+      // O holds the tiles before: wait for the last of them, weigh them anew
+      if (!__all_sync(0xffffffffu, mbar_wait(sm.pv_done(x), (uint32_t)(j - 1) & 1u, ab, p.err))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < 128; c += 32) {
+        uint32_t o[32];
+        tmem_ld32(o_at + c, o);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+        tmem_st32(o_at + c, o);
+      }
+    }
+    const float base = ref == -INFINITY ? 0.f : ref;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float f = h ? f1 : f0, vs = h ? vs1 : vs0;
+      const bool page = (h ? ks1 : ks0) >= 0.f;
+      const float rv = vref > 0.f ? vs / vref : 0.f;
+      const bool folded = rv >= PF_VLOW;  // weigh in the exponent, take it out of the sum again
+      const float shift = folded ? log2f(rv) - base : -base;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t v[32], pk[16];
+        tmem_ld32(s_at + 64 * h + 32 * q, v);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          float y = fmaf(__uint_as_float(v[i]), f, shift);
+          if (!whole && (64 * h + 32 * q + i >= seen || !page)) y = -INFINITY;
+          const float e = fast_exp2(y);
+          sum[i & 3] += e;
+          v[i] = __float_as_uint(folded ? e : e * rv);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pk[i] = pack_half2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+        tmem_st16(s_at + 32 * h + 16 * q, pk);
+      }
+      const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      l += folded ? total / rv : total;
+    }
+    tmem_st_wait();
+    tc_fence_before();
+    mbar_arrive(sm.p_ready(x));
+  }
+  if (!ok || !__all_sync(0xffffffffu, mbar_wait(sm.pv_done(x), (uint32_t)(n - 1) & 1u, ab, p.err))) return;
+  tc_fence_after();
+  float inv = l == 0.f ? 0.f : vref / l;
+  // NaN values that the converters took out of the tiles some row sees in part (every V has been read)
+  for (int j = max(0, w.shift + w.q0 + 1 - w.begin) / PF_KEYS; j < n; ++j)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int m = last - (w.begin + j * PF_KEYS + 32 * k) + 1;  // keys of the word that the row sees
+      const uint32_t mine = m >= 32 ? 0xffffffffu : (m <= 0 ? 0u : (1u << m) - 1u);
+      if (sm.nan_keys(j)[k] & mine) inv = __int_as_float(0x7fffffff);
+    }
+  const int64_t row = w.row0 + pos;
+  const int head = w.kvh * group + R % group;
+  bf16* out = p.out + row * p.o_stride + head * KV8_D;
+  float* ws = p.ws + (p.n_splits > 1 ? ((row * p.hq + head) * p.n_splits + split) * PF_WS_ROW : 0);
+#pragma unroll 1
+  for (int c = 0; c < 128; c += 32) {
+    uint32_t o[32];
+    tmem_ld32(o_at + c, o);
+    if (!live) continue;
+    if (p.n_splits > 1) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        reinterpret_cast<float4*>(ws + c)[i] =
+            make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
+                        __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint4 u;
+        u.x = pack_bf16x2(__uint_as_float(o[8 * i + 0]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
+        u.y = pack_bf16x2(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
+        u.z = pack_bf16x2(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
+        u.w = pack_bf16x2(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
+        reinterpret_cast<uint4*>(out + c)[i] = u;
+      }
+    }
+  }
+  if (live && p.n_splits > 1) ws[KV8_D] = l == 0.f ? -INFINITY : ref + log2f(l);
+}
+
+__global__ void __launch_bounds__(PF_THREADS, 1)
+prefill_fp8_kernel(PrefillP p) {
+  qb_pdl_wait();  // metadata and operands may come from the kernel before; also before any exit
+  extern __shared__ uint8_t smem_raw[];
+  PrefillWork w;
+  const int group = p.hq / p.hkv, subs = p.unit / p.pos_per_cta;
+  const int tile = blockIdx.x / subs, sub = blockIdx.x % subs, split = blockIdx.z;
+  w.kvh = blockIdx.y;
+  w.b = p.tiles ? p.tiles[2 * tile] : tile / p.tiles_per_seq;
+  const int start = p.tiles ? p.tiles[2 * tile + 1] : tile % p.tiles_per_seq * p.unit;
+  if (w.b < 0 || w.b >= p.batch || start < 0 || start % p.unit != 0) {
+    // a 64-row tile whose rows belong to the CTA of an earlier one
+    if ((w.b < 0 || w.b >= p.batch || start < 0) && threadIdx.x == 0) qb_set_err(p.err, QB_DEVERR_SHAPE);
+    return;
+  }
+  w.row0 = p.cu_q[w.b];
+  w.lq = p.cu_q[w.b + 1] - (int)w.row0;
+  const int lk = p.cu_k[w.b + 1] - p.cu_k[w.b];
+  w.q0 = start + sub * p.pos_per_cta;
+  if (w.q0 >= w.lq) return;
+  if (lk < w.lq || w.row0 < 0 || w.row0 + w.lq > p.total_q) {
+    if (threadIdx.x == 0) qb_set_err(p.err, QB_DEVERR_SHAPE);
+    return;
+  }
+  w.shift = lk - w.lq;
+  const int positions = min(p.pos_per_cta, w.lq - w.q0);
+  w.rows = positions * group;
+  w.begin = split * p.split_keys;
+  w.end = min(w.shift + w.q0 + positions, p.n_splits > 1 ? w.begin + p.split_keys : INT32_MAX);
+  if (p.n_splits > 1 && split == p.n_splits - 1 && w.end < w.shift + w.q0 + positions && threadIdx.x == 0)
+    qb_set_err(p.err, QB_DEVERR_SHAPE);  // keys past the last split
+  if (w.begin >= w.end) return;  // uniform across the CTA, before any barrier or TMEM exists
+  const int rows_a = min(w.rows, PF_ROWS);
+  const int end_a = min(w.end, w.shift + w.q0 + (rows_a - 1) / group + 1);  // tile A's last row's keys
+  // tile A may see none of a late split's keys; a tile is kept all the same: its rows' sums are zero
+  w.n[0] = (max(end_a - w.begin, 1) + PF_KEYS - 1) / PF_KEYS;
+  w.n[1] = w.rows > PF_ROWS ? (w.end - w.begin + PF_KEYS - 1) / PF_KEYS : 0;
+
+  PrefillSmem sm;
+  const uint32_t raw = smem_u32(smem_raw);
+  sm.base = (raw + 1023) & ~1023u;
+  sm.ptr = smem_raw + (sm.base - raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(sm.q_full(i), 128);
+      mbar_init(sm.k_full(i), 128);
+      mbar_init(sm.k_empty(i), 1);
+      mbar_init(sm.v_full(i), 128);
+      mbar_init(sm.v_empty(i), 1);
+      mbar_init(sm.s_full(i), 1);
+      mbar_init(sm.p_ready(i), 128);
+      mbar_init(sm.pv_done(i), 1);
+    }
+    mbar_init(sm.all_done(), 1);
+    *sm.abort_flag() = 0;
+    // tiles that some row sees in part are the last three at most: their slots are used once
+    for (int j = 0; j < PF_SLOTS; ++j)
+      for (int k = 0; k < 4; ++k) sm.nan_keys(j)[k] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(sm.tmem_slot())),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *sm.tmem_slot();
+  qb_pdl_trigger();  // after the TMEM allocation: the next kernel cannot take it from this CTA
+  if (warp < 8) {
+    prefill_softmax(p, sm, w, tmem, warp >> 2, split);
+  } else if (warp < 12) {
+    prefill_convert(p, sm, w);
+  } else if (lane == 0) {
+    prefill_mma(p, sm, w, tmem);
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
+// Joins the key splits of a (row, head): a warp each, weights 2^(lse - largest lse), over the splits that
+// hold keys of the row.
 __global__ void __launch_bounds__(128)
-prefill_rows_kernel(RowParams p, int64_t total) {
+prefill_fp8_join_kernel(PrefillP p) {
   qb_pdl_trigger();
   qb_pdl_wait();
   const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const int h = (int)(item % p.hq), kvh = h / (p.hq / p.hkv);
-  const int64_t t = item / p.hq;
-  if (t >= total) return;
-  int b = 0;
-  while (b < p.batch && p.cu_q[b + 1] <= t) ++b;
-  if (b >= p.batch) return;
-  const int lq = p.cu_q[b + 1] - p.cu_q[b], lk = p.cu_k[b + 1] - p.cu_k[b];
-  if (lk < lq) {
-    if (lane == 0) qb_set_err(p.err, QB_DEVERR_SHAPE);
-    return;
+  const int lane = threadIdx.x & 31, head = (int)(item % p.hq);
+  const int64_t row = item / p.hq;
+  if (row >= p.total_q) return;
+  int lo = 0, hi = p.batch;  // the sequence whose rows hold `row`: the last with cu_q <= row
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (p.cu_q[mid] <= row) lo = mid;
+    else hi = mid;
   }
-  RowState s;
-  row_begin(p, s, t, h, lane);
-  row_keys(p, s, b, kvh, 0, lk - lq + (int)(t - p.cu_q[b]) + 1, lane);
-  row_end(p, s, t, h, lane);
+  const int lq = p.cu_q[lo + 1] - p.cu_q[lo], lk = p.cu_k[lo + 1] - p.cu_k[lo], i = (int)row - p.cu_q[lo];
+  if (i < 0 || i >= lq || lk < lq || p.cu_q[lo + 1] > p.total_q) return;
+  const int n = min(p.n_splits, (lk - lq + i) / p.split_keys + 1);
+  const float* ws = p.ws + (row * p.hq + head) * p.n_splits * PF_WS_ROW;
+  float m = -INFINITY;
+  for (int s = lane; s < n; s += 32) m = fmaxf(m, ws[(int64_t)s * PF_WS_ROW + KV8_D]);
+  m = warp_max(m);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < n; ++s) {
+    const float* at = ws + (int64_t)s * PF_WS_ROW;
+    const float lse = at[KV8_D], f = lse == -INFINITY ? 0.f : exp2f(lse - m);
+    const float4 x = *reinterpret_cast<const float4*>(at + lane * 4);
+    sum += f;
+    acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint2 u;
+  u.x = pack_bf16x2(acc.x * inv, acc.y * inv);
+  u.y = pack_bf16x2(acc.z * inv, acc.w * inv);
+  *reinterpret_cast<uint2*>(p.out + row * p.o_stride + head * KV8_D + lane * 4) = u;
 }
 
 }  // namespace
+
+extern "C" size_t qb_attn_paged_prefill_fp8_workspace_bytes(int64_t total_q, int hq, int n_splits) {
+  return n_splits <= 1 ? 0 : (size_t)total_q * hq * n_splits * PF_WS_ROW * 4;
+}
 
 extern "C" int qb_attn_paged_prefill_fp8(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
                                          const float* k_scale, const float* v_scale, int64_t num_blocks, int page_size,
                                          const int32_t* block_tables, int64_t bt_stride, int bt_width,
                                          const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,
                                          const int32_t* tile_info, int n_tiles, int tiles_per_seq, int hq, int hkv,
-                                         int D, float scale, void* out, int64_t o_stride, int64_t total_q, int* err,
-                                         qb_stream_t stream) {
+                                         int D, float scale, int split_keys, int n_splits, float* workspace, void* out,
+                                         int64_t o_stride, int64_t total_q, int* err, qb_stream_t stream) {
   if (D != KV8_D || page_size != KV8_PAGE) return QB_ERR_UNSUPPORTED;
   QB_CHECK_ARG(batch >= 0 && total_q >= 0 && total_q <= INT32_MAX && n_tiles >= 0 && tiles_per_seq >= 0);
+  QB_CHECK_ARG(n_splits >= 1 && n_splits <= 65535 && (n_splits == 1 || (split_keys > 0 && split_keys % PF_KEYS == 0 &&
+               (int64_t)split_keys * n_splits <= INT32_MAX / 2)));
   if (batch == 0 || total_q == 0) return QB_OK;
-  const int st = kv8_check_cache(q, q_stride, k_cache, v_cache, k_scale, v_scale, num_blocks, block_tables, bt_stride, bt_width,
-                             hq, hkv, out);
-  if (st != QB_OK) return st;
-  QB_CHECK_ARG(cu_seqlens_q && cu_seqlens_k && o_stride >= (int64_t)hq * KV8_D && o_stride % 8 == 0);
-  (void)tile_info;
-  RowParams p{(const bf16*)q, q_stride, (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale, num_blocks,
-              block_tables, bt_stride, bt_width, nullptr, 0, batch, hq, hkv, scale * KV8_LOG2E, 0, nullptr, nullptr, nullptr,
-              cu_seqlens_q, cu_seqlens_k, (bf16*)out, o_stride, err};
-  return qb_launch(prefill_rows_kernel, dim3((unsigned)((total_q * hq + 3) / 4)), dim3(128), 0, (cudaStream_t)stream, 1,
-                   p, total_q);
+  const int ok = kv8_check_cache(q, q_stride, k_cache, v_cache, k_scale, v_scale, num_blocks, block_tables, bt_stride,
+                                 bt_width, hq, hkv, out);
+  if (ok != QB_OK) return ok;
+  QB_CHECK_ARG(cu_seqlens_q && cu_seqlens_k && o_stride >= (int64_t)hq * KV8_D && o_stride % 8 == 0 && hkv <= 65535);
+  QB_CHECK_ARG(n_splits == 1 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0));
+  PrefillP p{};
+  p.q = (const bf16*)q; p.q_stride = q_stride; p.k = (const uint8_t*)k_cache; p.v = (const uint8_t*)v_cache;
+  p.ks = k_scale; p.vs = v_scale; p.num_blocks = num_blocks; p.bt = block_tables; p.bt_stride = bt_stride;
+  p.bt_width = bt_width; p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k; p.batch = batch; p.tiles = tile_info;
+  p.hq = hq; p.hkv = hkv;
+  p.pos_per_cta = 16;
+  while (p.pos_per_cta * 2 * (hq / hkv) <= 2 * PF_ROWS) p.pos_per_cta *= 2;
+  p.unit = p.pos_per_cta > 64 ? p.pos_per_cta : 64;
+  p.tiles_per_seq = (int)(((int64_t)tiles_per_seq * 64 + p.unit - 1) / p.unit);
+  p.scale_log2 = scale * KV8_LOG2E;
+  p.split_keys = n_splits > 1 ? split_keys : 0; p.n_splits = n_splits; p.ws = workspace; p.out = (bf16*)out;
+  p.o_stride = o_stride; p.total_q = total_q; p.err = err;
+  const int64_t grid = (tile_info ? (int64_t)n_tiles : (int64_t)batch * p.tiles_per_seq) * (p.unit / p.pos_per_cta);
+  QB_CHECK_ARG(grid <= INT32_MAX);
+  if (grid == 0) return QB_OK;
+  static bool attr = false;
+  if (!attr) {
+    if (cudaFuncSetAttribute(prefill_fp8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PF_SMEM) != cudaSuccess)
+      return qb_launch_status();
+    attr = true;
+  }
+  const cudaStream_t st = (cudaStream_t)stream;
+  const int rc = qb_launch_ex(prefill_fp8_kernel, dim3((unsigned)grid, (unsigned)hkv, (unsigned)n_splits), dim3(PF_THREADS),
+                              PF_SMEM, st, 1, true, p);
+  if (rc != QB_OK || n_splits == 1) return rc;
+  const int64_t items = total_q * hq;
+  if ((items + 3) / 4 > INT32_MAX) return QB_ERR_INVALID;
+  return qb_launch_ex(prefill_fp8_join_kernel, dim3((unsigned)((items + 3) / 4)), dim3(128), 0, st, 1, true, p);
 }

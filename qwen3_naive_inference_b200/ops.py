@@ -28,7 +28,7 @@ __all__ = [
     "grpo_loss", "mask_sum", "build_tiles", "decode_split_plan", "lm_head_logprob",
     "grpo_logit_loss", "kv_cache_fp8", "qk_norm_rope_store_fp8", "paged_decode_attention_fp8",
     "paged_decode_attention_grouped_fp8", "attention_paged_prefill_fp8", "decode_split_plan_fp8",
-    "grouped_decode_plan_fp8",
+    "grouped_decode_plan_fp8", "prefill_split_plan_fp8",
 ]
 
 BF16 = torch.bfloat16
@@ -701,10 +701,26 @@ def paged_decode_attention_grouped_fp8(q, k_cache, v_cache, k_scale, v_scale, bl
     return out
 
 
+def prefill_split_plan_fp8(batch, total_q, max_q, max_k, hq, hkv, sm_count=148):
+    """(split_keys, n_splits) of :func:`attention_paged_prefill_fp8`: keys are split where the query tiles
+    are too few to cover the GPU, in parts of at least 512."""
+    positions = 16
+    while positions * 2 * (hq // hkv) <= 256:
+        positions *= 2
+    tiles = min(batch * math.ceil(max_q / positions), batch + total_q // positions)  # ragged: close above the count
+    want = min(sm_count // max(1, tiles * hkv), math.ceil(max_k / 512))
+    if want <= 1:
+        return 0, 1
+    split = math.ceil(max_k / want / 128) * 128
+    return (0, 1) if split >= max_k else (split, math.ceil(max_k / split))
+
+
 def attention_paged_prefill_fp8(q, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
-                                block_tables, scale, tiles=None, out=None):
+                                block_tables, scale, tiles=None, out=None, max_seqlen_k=None):
     """:func:`attention_paged_prefill` over the 8-bit cache; any hq / hkv up to 16.  Query row i of a
-    sequence with Lq rows and Lk keys attends keys 0 .. Lk - Lq + i; rows in no sequence are left out."""
+    sequence with Lq rows and Lk keys attends keys 0 .. Lk - Lq + i; rows in no sequence are left out of
+    ``out``.  ``max_seqlen_k`` bounds the longest Lk (keys beyond it may be left out, and are then reported);
+    default: what block_tables can name."""
     what = "attention_paged_prefill_fp8"
     num_blocks, hkv = _check_kv_fp8(what, k_cache, v_cache, k_scale, v_scale, q, cu_seqlens_q, cu_seqlens_k,
                                     block_tables, tiles)
@@ -717,13 +733,20 @@ def attention_paged_prefill_fp8(q, k_cache, v_cache, k_scale, v_scale, cu_seqlen
     if tiles is not None:
         _fp8_ints(what, tiles)
     out = _fp8_out(what, out, q, strided=True)
-    tps = (int(max_seqlen_q) + 63) // 64
+    max_q = int(max_seqlen_q)
+    max_k = block_tables.shape[1] * KV_FP8_PAGE if max_seqlen_k is None else int(max_seqlen_k)
+    split_keys, n_splits = prefill_split_plan_fp8(batch, Tq, max_q, max_k, hq, hkv)
+    ws = None
+    if n_splits > 1:
+        ws = torch.empty(lib().qb_attn_paged_prefill_fp8_workspace_bytes(Tq, hq, n_splits) // 4, dtype=torch.float32,
+                         device=q.device)
     n_tiles = 0 if tiles is None else tiles.numel() // 2
     check(lib().qb_attn_paged_prefill_fp8(_p(q), q.stride(0), _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale),
                                           num_blocks, KV_FP8_PAGE, _p(block_tables), block_tables.stride(0),
                                           block_tables.shape[1], _p(cu_seqlens_q), _p(cu_seqlens_k), batch, _p(tiles),
-                                          n_tiles, tps, hq, hkv, 128, scale, _p(out), out.stride(0), Tq,
-                                          _p(err_flag()), stream_ptr()), "qb_attn_paged_prefill_fp8")
+                                          n_tiles, (max_q + 63) // 64, hq, hkv, 128, scale, split_keys, n_splits, _p(ws),
+                                          _p(out), out.stride(0), Tq, _p(err_flag()), stream_ptr()),
+          "qb_attn_paged_prefill_fp8", kernels=2 if n_splits > 1 else 1)
     return out
 
 

@@ -42,13 +42,14 @@ def test_grouped_refusals():
 def test_prefill_refusals():
     lib = _lib.load()
 
-    def call(q=A, cu=A, batch=1, total=4, o_stride=2048, n_tiles=0, tps=1, page=256, hq=16):
+    def call(q=A, cu=A, batch=1, total=4, o_stride=2048, n_tiles=0, tps=1, page=256, hq=16, split=(0, 1), ws=None):
         return lib.qb_attn_paged_prefill_fp8(q, 2048, A, A, A, A, 4, page, A, 1, 1, cu, A, batch, None, n_tiles, tps, hq, 8, 128,
-                                             1.0, A, o_stride, total, None, None)
+                                             1.0, *split, ws, A, o_stride, total, None, None)
 
     assert call(page=64) == 2
     for kw in ({"q": None}, {"cu": None}, {"batch": -1}, {"total": -1}, {"o_stride": 2044}, {"o_stride": 8}, {"tps": -1},
-               {"n_tiles": -1}, {"hq": 17}, {"total": 1 << 31}):
+               {"n_tiles": -1}, {"hq": 17}, {"total": 1 << 31}, {"split": (128, 0)}, {"split": (128, 2)}, {"split": (64, 2), "ws": A},
+               {"split": (0, 2), "ws": A}, {"split": (128, 70000), "ws": A}):
         assert call(**kw) == 1, kw
     assert call(batch=0) == 0 and call(total=0) == 0
 
@@ -73,6 +74,8 @@ def test_workspace_size():
     assert lib.qb_paged_decode_fp8_workspace_bytes(4, 16, 1) == 0
     assert lib.qb_paged_decode_fp8_workspace_bytes(4, 16, 3) == 4 * 16 * 3 * 132 * 4
     assert lib.qb_paged_decode_fp8_workspace_bytes(4096, 128, 512) == 4096 * 128 * 512 * 132 * 4  # past 32 bits
+    assert lib.qb_attn_paged_prefill_fp8_workspace_bytes(10, 16, 1) == 0
+    assert lib.qb_attn_paged_prefill_fp8_workspace_bytes(1 << 20, 16, 64) == (1 << 30) * 132 * 4
 
 
 def test_cpu_tensors_are_refused():
@@ -92,3 +95,10 @@ def test_plans_cover_the_context(batch, hkv, ctx):
     sh, ns, ow, no = ops.grouped_decode_plan_fp8(batch, max(1, batch // 8), 2 * hkv, hkv, ctx, ctx)
     for split, n in ((sh, ns), (ow, no)):
         assert split % 64 == 0 and 64 <= split <= 8192 and n >= 1 and split * n >= ctx
+
+@pytest.mark.parametrize("batch,total_q,max_q", [(1, 1, 1), (1, 20, 20), (4, 40, 30), (64, 64, 1), (1, 2048, 2048), (300, 300, 1)])
+@pytest.mark.parametrize("hq,hkv", [(16, 8), (16, 1), (8, 8)])
+@pytest.mark.parametrize("max_k", [1, 511, 1025, 32768, 40961])
+def test_prefill_plan_covers_the_keys(batch, total_q, max_q, hq, hkv, max_k):
+    split, n = ops.prefill_split_plan_fp8(batch, total_q, max_q, max_k, hq, hkv)
+    assert (split, n) == (0, 1) or (split % 128 == 0 and n > 1 and (n - 1) * split < max_k <= n * split)
