@@ -27,6 +27,8 @@
 // Few rows over many keys: the keys are split over CTAs, which write normalised partial outputs and the
 // rows' log-sums for a second kernel to join.
 // Every wait is bounded (~2 s): on timeout QB_DEVERR_TIMEOUT is raised, all roles leave, TMEM is freed.
+#include <float.h>
+
 #include "attn_fp8.cuh"
 #include "tcgen05.cuh"
 
@@ -82,6 +84,23 @@ QB_DEVICE uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// Two fp32 multiply-adds, two sums in one instruction.
+QB_DEVICE float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+QB_DEVICE float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 QB_DEVICE void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 QB_DEVICE void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -132,11 +151,9 @@ QB_DEVICE void put_codes(uint32_t tile, int r, int c, const uint4& u) {
     h[2 * i] = e4m3x2_to_half2(w[i] & 0xffffu);
     h[2 * i + 1] = e4m3x2_to_half2(w[i] >> 16);
   }
-  // the eight threads of a row write even chunks of one half and odd chunks of the other at a time
-  const int first = c >> 2;
-  const uint32_t a0 = tile + operand_chunk(r, 2 * c + first), a1 = tile + operand_chunk(r, 2 * c + 1 - first);
-  st_shared16(a0, first ? h[4] : h[0], first ? h[5] : h[1], first ? h[6] : h[2], first ? h[7] : h[3]);
-  st_shared16(a1, first ? h[0] : h[4], first ? h[1] : h[5], first ? h[2] : h[6], first ? h[3] : h[7]);
+  const uint32_t at = tile + operand_chunk(r, 2 * c);
+  st_shared16(at, h[0], h[1], h[2], h[3]);
+  st_shared16(at ^ 16u, h[4], h[5], h[6], h[7]);
 }
 // Bits 7 of the bytes of w that hold a NaN code.
 QB_DEVICE uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
@@ -144,7 +161,9 @@ QB_DEVICE uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x0101010
 // ------------------------------------------------------------------ converters
 QB_DEVICE void prefill_convert(const PrefillP& p, const PrefillSmem& sm, const PrefillWork& w) {
   const int tid = threadIdx.x - 8 * 32, n = max(w.n[0], w.n[1]);
-  const int chunk = tid & 7, row0 = tid >> 3;  // keys row0 + 16 i, i < 8: block i / 4
+  // keys row0 + 16 i, i < 8 (block i / 4); eight threads in a row store to eight different bank groups:
+  // even chunks of one element half of two neighbouring keys
+  const int chunk = (tid & 3) | ((tid >> 1) & 4), row0 = ((tid >> 4) << 1) | ((tid >> 2) & 1);
   const int first_masked = w.shift + w.q0 + 1;  // keys from here on are behind the first row's last one
   uint4 kr[8], vr[8];
   // Codes of key tile j in registers (rows past the keys and tiles without a page: zero)
@@ -238,7 +257,7 @@ QB_DEVICE void prefill_mma(const PrefillP& p, const PrefillSmem& sm, const Prefi
   for (int j = 0; ok && j < n; ++j) {
     const int s = j % PF_STAGES;
     ok = mbar_wait(sm.v_full(s), (uint32_t)(j / PF_STAGES) & 1u, ab, p.err);
-    if (ok && j + 1 < n) ok = mbar_wait(sm.k_full((j + 1) % PF_STAGES), (uint32_t)((j + 1) / PF_STAGES) & 1u, ab, p.err);
+    bool have_k = false;
     for (int x = 0; ok && x < 2; ++x) {
       if (j >= w.n[x]) continue;
       if (!(ok = mbar_wait(sm.p_ready(x), (uint32_t)j & 1u, ab, p.err))) break;
@@ -249,6 +268,10 @@ QB_DEVICE void prefill_mma(const PrefillP& p, const PrefillSmem& sm, const Prefi
                      sw128_mn_desc(sm.v(s) + i * 16 * 128, PF_HALF), PF_IDESC_O, (j > 0 || i > 0) ? 1u : 0u);
       umma_commit(sm.pv_done(x));
       if (j + 1 < w.n[x]) {  // the next scores go over P's columns: its product has to be through
+        if (!have_k &&
+            !(ok = mbar_wait(sm.k_full((j + 1) % PF_STAGES), (uint32_t)((j + 1) / PF_STAGES) & 1u, ab, p.err)))
+          break;
+        have_k = true;
         if (!(ok = mbar_wait(sm.pv_done(x), (uint32_t)j & 1u, ab, p.err))) break;
         scores(x, j + 1);
       }
@@ -335,17 +358,16 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
       if (whole) {
 #pragma unroll
         for (int i = 0; i < 64; ++i) m[i & 3] = fmaxf(m[i & 3], __uint_as_float(v[i]));
-      } else if ((h ? ks1 : ks0) >= 0.f) {
+      } else {
+        const int mine = (h ? ks1 : ks0) < 0.f ? 0 : seen - 64 * h;
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
-          if (64 * h + i < seen) m[i & 3] = fmaxf(m[i & 3], __uint_as_float(v[i]));
+        for (int i = 0; i < 64; ++i) m[i & 3] = fmaxf(m[i & 3], i < mine ? __uint_as_float(v[i]) : -INFINITY);
       }
       top[h] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
     }
-    const float f0 = fac * fmaxf(ks0, 0.f), f1 = fac * fmaxf(ks1, 0.f);
-    // -inf (nothing seen) times a factor of zero would be NaN
-    const float t0 = top[0] == -INFINITY ? -INFINITY : top[0] * f0, t1 = top[1] == -INFINITY ? -INFINITY : top[1] * f1;
-    const float mt = fmaxf(t0, t1);
+    // not zero: -inf (a key not seen) has to stay -inf
+    const float f0 = fmaxf(fac * ks0, FLT_MIN), f1 = fmaxf(fac * ks1, FLT_MIN);
+    const float mt = fmaxf(top[0] * f0, top[1] * f1);
     const bool need = mt > ref + PF_SLACK;
     const float vtop = fmaxf(vs0, vs1);
     const bool vneed = vtop > vref * PF_VSLACK;  // the same for every thread of the CTA
@@ -380,28 +402,40 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float f = h ? f1 : f0, vs = h ? vs1 : vs0;
-      const bool page = (h ? ks1 : ks0) >= 0.f;
       const float rv = vref > 0.f ? vs / vref : 0.f;
       const bool folded = rv >= PF_VLOW;  // weigh in the exponent, take it out of the sum again
       const float shift = folded ? log2f(rv) - base : -base;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const float2 ff = make_float2(f, f), ss = make_float2(shift, shift);
+      // keys of the half that the row sees
+      const int mine = whole ? 64 : ((h ? ks1 : ks0) < 0.f ? 0 : seen - 64 * h);
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         uint32_t v[32], pk[16];
         tmem_ld32(s_at + 64 * h + 32 * q, v);
+        if (!whole) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float y = fmaf(__uint_as_float(v[i]), f, shift);
-          if (!whole && (64 * h + 32 * q + i >= seen || !page)) y = -INFINITY;
-          const float e = fast_exp2(y);
-          sum[i & 3] += e;
-          v[i] = __float_as_uint(folded ? e : e * rv);
+          for (int i = 0; i < 32; ++i)
+            if (32 * q + i >= mine) v[i] = __float_as_uint(-INFINITY);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float2 y = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ff, ss);
+          y.x = fast_exp2(y.x);
+          y.y = fast_exp2(y.y);
+          sum[i & 1] = add2(sum[i & 1], y);
+          v[2 * i] = __float_as_uint(y.x);
+          v[2 * i + 1] = __float_as_uint(y.y);
+        }
+        if (!folded) {  // the same for every thread of the CTA
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * rv);
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) pk[i] = pack_half2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
         tmem_st16(s_at + 32 * h + 16 * q, pk);
       }
-      const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      const float total = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       l += folded ? total / rv : total;
     }
     tmem_st_wait();
