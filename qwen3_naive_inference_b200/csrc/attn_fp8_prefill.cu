@@ -11,7 +11,7 @@
 //   warps 0-3, 4-7  softmax of tile A, of tile B: a thread per row
 //   warps 8-11      convert: codes come from global memory a tile ahead, become halves (exactly) and go
 //                   to shared memory in the swizzled layout of the MMA operands
-//   warp 12         one thread issues the MMAs:  S_x = Q_x K^T (both operands in shared memory),
+//   warp 12         (of a warpgroup otherwise idle) one thread issues the MMAs:  S_x = Q_x K^T (both operands in shared memory),
 //                   O_x += P_x V (P_x from TMEM, over the columns of S_x)
 // While one tile's softmax runs, the tensor pipe works on the other's products.  TMEM: S_A, S_B, O_A, O_B
 // of 128 columns each.
@@ -36,7 +36,9 @@ namespace {
 
 constexpr int PF_KEYS = 128;                       // keys of a tile: two blocks
 constexpr int PF_ROWS = 128;                       // rows of a query tile
-constexpr int PF_THREADS = 13 * 32;
+constexpr int PF_THREADS = 16 * 32;                // 128 registers a thread at launch, 65536 in all ...
+constexpr int PF_REG_SOFTMAX = 176, PF_REG_CONVERT = 104, PF_REG_MMA = 56;  // ... shared out by warpgroup
+static_assert(256 * PF_REG_SOFTMAX + 128 * PF_REG_CONVERT + 128 * PF_REG_MMA == 65536, "the launch's registers");
 constexpr int PF_HALF = 128 * 64 * 2;              // [128 x 64] halves: 16 KB
 constexpr int PF_TILE = 2 * PF_HALF;               // [128 x 128]: element halves 0-63, 64-127
 constexpr int PF_STAGES = 2;
@@ -44,8 +46,9 @@ constexpr int PF_Q = 0, PF_K = 2 * PF_TILE, PF_V = PF_K + PF_STAGES * PF_TILE;
 constexpr int PF_META = PF_V + PF_STAGES * PF_TILE;
 constexpr int PF_SLOTS = 4;                        // tiles whose scales are held
 constexpr int PF_BARS = 17;
-// barriers; TMEM slot, abort flag; row factors; per slot two ks, two vs, four words of NaN keys
-constexpr int PF_SMEM = PF_META + PF_BARS * 8 + 8 + 2 * PF_ROWS * 4 + PF_SLOTS * 32 + 1024 /*align*/;
+// barriers; TMEM slot, abort flag; row factors; per slot the tile's scales and NaN keys
+constexpr int PF_SLOT = 16;                        // words of a slot
+constexpr int PF_SMEM = PF_META + PF_BARS * 8 + 8 + 2 * PF_ROWS * 4 + PF_SLOTS * PF_SLOT * 4 + 1024 /*align*/;
 constexpr uint32_t PF_COL_S = 0, PF_COL_O = 256;   // + 128 * tile
 constexpr float PF_HEAD = 4.f, PF_SLACK = 12.f, PF_VSLACK = 8.f, PF_VLOW = 1.f / 1024;
 constexpr int PF_WS_ROW = KV8_D + 4;
@@ -129,9 +132,12 @@ struct PrefillSmem {
   QB_DEVICE uint32_t* tmem_slot() const { return reinterpret_cast<uint32_t*>(ptr + PF_META + 8 * PF_BARS); }
   QB_DEVICE volatile int* abort_flag() const { return reinterpret_cast<volatile int*>(tmem_slot() + 1); }
   QB_DEVICE float* row_fac() const { return reinterpret_cast<float*>(tmem_slot() + 2); }
-  // slot of tile j: ks of its two blocks (negative: no such page), vs of both, bits of its NaN keys
-  QB_DEVICE float* scales(int j) const { return row_fac() + 2 * PF_ROWS + (j % PF_SLOTS) * 8; }
-  QB_DEVICE uint32_t* nan_keys(int j) const { return reinterpret_cast<uint32_t*>(scales(j) + 4); }
+  // slot of tile j; of its blocks h = 0, 1:
+  //   [h] ks (negative: no such page), [2 + h] the exponent that weighs P by vs / vref (0: it is not
+  //   weighed there), [4 + h] the factor that takes this out of the sum, [6 + h] the factor of P after it;
+  //   [8] what O is multiplied by before the tile (vref has moved), [9] vref; [12..15] bits of NaN keys
+  QB_DEVICE float* scales(int j) const { return row_fac() + 2 * PF_ROWS + (j % PF_SLOTS) * PF_SLOT; }
+  QB_DEVICE uint32_t* nan_keys(int j) const { return reinterpret_cast<uint32_t*>(scales(j) + 12); }
 };
 
 // What a CTA works on.
@@ -181,7 +187,7 @@ QB_DEVICE void prefill_convert(const PrefillP& p, const PrefillSmem& sm, const P
         qb_set_err(p.err, QB_DEVERR_PAGE);
     }
   };
-  auto load = [&](const uint8_t* codes, uint4 (&r)[8], const int64_t (&at)[2], int j) {
+  auto load = [&](const uint8_t* codes, uint4 (&r)[8], int j) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int key = row0 + 16 * i;
@@ -190,22 +196,48 @@ QB_DEVICE void prefill_convert(const PrefillP& p, const PrefillSmem& sm, const P
         r[i] = *reinterpret_cast<const uint4*>(codes + at[i >> 2] * KV8_TILE + (key % KV8_BLOCK) * KV8_D + chunk * 16);
     }
   };
+  float ks_next[2], vs_next[2], vref = 0.f;  // thread 0: the scales of the next tile
+  auto load_scales = [&]() {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      ks_next[h] = tid == 0 && at[h] >= 0 ? p.ks[at[h]] : -1.f;
+      vs_next[h] = tid == 0 && at[h] >= 0 ? p.vs[at[h]] : 0.f;
+    }
+  };
   find(0);
-  int64_t now[2] = {at[0], at[1]};
-  load(p.k, kr, now, 0);
-  load(p.v, vr, now, 0);
+  load(p.k, kr, 0);
+  load_scales();
+  load(p.v, vr, 0);
   for (int j = 0; j < n; ++j) {
     const int s = j % PF_STAGES;
     const uint32_t ph = ((uint32_t)(j / PF_STAGES) & 1u) ^ 1u;
     if (j + 1 < n) find(j + 1);
     if (!mbar_wait(sm.k_empty(s), ph, sm.abort_flag(), p.err)) return;
-    if (tid < 2) {
-      sm.scales(j)[tid] = now[tid] >= 0 ? p.ks[now[tid]] : -1.f;
-      sm.scales(j)[2 + tid] = now[tid] >= 0 ? p.vs[now[tid]] : 0.f;
+    if (tid == 0) {
+      float* sc = sm.scales(j);
+      const float top = fmaxf(vs_next[0], vs_next[1]);
+      sc[8] = 1.f;
+      if (top > vref * PF_VSLACK) {
+        sc[8] = vref / top;
+        vref = top;
+      }
+      sc[9] = vref;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float rv = vref > 0.f ? vs_next[h] / vref : 0.f;
+        const bool folded = rv >= PF_VLOW;
+        sc[h] = ks_next[h];
+        sc[2 + h] = folded ? log2f(rv) : 0.f;
+        sc[4 + h] = folded ? 1.f / rv : 1.f;
+        sc[6 + h] = folded ? 1.f : rv;
+      }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) put_codes(sm.k(s), row0 + 16 * i, chunk, kr[i]);
-    if (j + 1 < n) load(p.k, kr, at, j + 1);
+    if (j + 1 < n) {
+      load(p.k, kr, j + 1);
+      load_scales();
+    }
     fence_async_shared();
     mbar_arrive(sm.k_full(s));
     if (!mbar_wait(sm.v_empty(s), ph, sm.abort_flag(), p.err)) return;
@@ -226,9 +258,7 @@ QB_DEVICE void prefill_convert(const PrefillP& p, const PrefillSmem& sm, const P
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) put_codes(sm.v(s), row0 + 16 * i, chunk, vr[i]);
-    if (j + 1 < n) load(p.v, vr, at, j + 1);
-    now[0] = at[0];
-    now[1] = at[1];
+    if (j + 1 < n) load(p.v, vr, j + 1);
     fence_async_shared();
     mbar_arrive(sm.v_full(s));
   }
@@ -342,35 +372,36 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
       break;
     }
     tc_fence_after();
+    uint32_t v[128];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) tmem_ld32_nowait(s_at + 32 * c, v + 32 * c);
     const float* sc = sm.scales(j);
-    const float ks0 = sc[0], ks1 = sc[1], vs0 = sc[2], vs1 = sc[3];
+    const float ks0 = sc[0], ks1 = sc[1], vfac = sc[8];
+    vref = sc[9];
     const int k0 = w.begin + j * PF_KEYS;
     const int seen = last - k0 + 1;  // keys of the tile that the row sees
     const bool whole = __all_sync(0xffffffffu, seen >= PF_KEYS) && ks0 >= 0.f && ks1 >= 0.f;
-    float top[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t v[64];
-      tmem_ld32_nowait(s_at + 64 * h, v);
-      tmem_ld32_nowait(s_at + 64 * h + 32, v + 32);
-      tmem_ld_wait();
-      float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      if (whole) {
-#pragma unroll
-        for (int i = 0; i < 64; ++i) m[i & 3] = fmaxf(m[i & 3], __uint_as_float(v[i]));
-      } else {
-        const int mine = (h ? ks1 : ks0) < 0.f ? 0 : seen - 64 * h;
-#pragma unroll
-        for (int i = 0; i < 64; ++i) m[i & 3] = fmaxf(m[i & 3], i < mine ? __uint_as_float(v[i]) : -INFINITY);
-      }
-      top[h] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-    }
     // not zero: -inf (a key not seen) has to stay -inf
     const float f0 = fmaxf(fac * ks0, FLT_MIN), f1 = fmaxf(fac * ks1, FLT_MIN);
-    const float mt = fmaxf(top[0] * f0, top[1] * f1);
+    tmem_ld_wait();
+    if (!whole) {
+      const int see0 = ks0 < 0.f ? 0 : seen, see1 = ks1 < 0.f ? 0 : seen - 64;
+#pragma unroll
+      for (int i = 0; i < 64; ++i) {
+        if (i >= see0) v[i] = __float_as_uint(-INFINITY);
+        if (i >= see1) v[64 + i] = __float_as_uint(-INFINITY);
+      }
+    }
+    float top[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top[i] = __uint_as_float(v[16 * i]);
+#pragma unroll
+    for (int i = 1; i < 16; ++i)
+#pragma unroll
+      for (int c = 0; c < 8; ++c) top[c] = fmaxf(top[c], __uint_as_float(v[16 * c + i]));
+    const float mt = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f0,
+                           fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])) * f1);
     const bool need = mt > ref + PF_SLACK;
-    const float vtop = fmaxf(vs0, vs1);
-    const bool vneed = vtop > vref * PF_VSLACK;  // the same for every thread of the CTA
     float a = 1.f;
     if (need) {
       const float to = mt - PF_HEAD;
@@ -378,11 +409,8 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
       ref = to;
       l *= a;
     }
-    if (vneed) {
-      a *= vref / vtop;
-      vref = vtop;
-    }
-    if (j > 0 && __any_sync(0xffffffffu, need || vneed)) {
+    a *= vfac;
+    if (j > 0 && (__any_sync(0xffffffffu, need) || vfac != 1.f)) {
       // O holds the tiles before: wait for the last of them, weigh them anew
       if (!__all_sync(0xffffffffu, mbar_wait(sm.pv_done(x), (uint32_t)(j - 1) & 1u, ab, p.err))) {
         ok = false;
@@ -401,42 +429,36 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
     const float base = ref == -INFINITY ? 0.f : ref;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float f = h ? f1 : f0, vs = h ? vs1 : vs0;
-      const float rv = vref > 0.f ? vs / vref : 0.f;
-      const bool folded = rv >= PF_VLOW;  // weigh in the exponent, take it out of the sum again
-      const float shift = folded ? log2f(rv) - base : -base;
-      const float2 ff = make_float2(f, f), ss = make_float2(shift, shift);
-      // keys of the half that the row sees
-      const int mine = whole ? 64 : ((h ? ks1 : ks0) < 0.f ? 0 : seen - 64 * h);
-      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      const float2 ff = make_float2(h ? f1 : f0, h ? f1 : f0);
+      const float shift = sc[2 + h] - base;
+      const float2 ss = make_float2(shift, shift);
+      float2 sum[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sum[c] = make_float2(0.f, 0.f);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        uint32_t v[32], pk[16];
-        tmem_ld32(s_at + 64 * h + 32 * q, v);
-        if (!whole) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (32 * q + i >= mine) v[i] = __float_as_uint(-INFINITY);
-        }
+        uint32_t* u = v + 64 * h + 32 * q;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          float2 y = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ff, ss);
+          float2 y = fma2(make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])), ff, ss);
           y.x = fast_exp2(y.x);
           y.y = fast_exp2(y.y);
-          sum[i & 1] = add2(sum[i & 1], y);
-          v[2 * i] = __float_as_uint(y.x);
-          v[2 * i + 1] = __float_as_uint(y.y);
+          sum[i & 3] = add2(sum[i & 3], y);
+          u[2 * i] = __float_as_uint(y.x);
+          u[2 * i + 1] = __float_as_uint(y.y);
         }
-        if (!folded) {  // the same for every thread of the CTA
+        if (sc[6 + h] != 1.f) {  // the same for every thread of the CTA
+          const float rv = sc[6 + h];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * rv);
+          for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * rv);
         }
+        uint32_t pk[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) pk[i] = pack_half2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+        for (int i = 0; i < 16; ++i) pk[i] = pack_half2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
         tmem_st16(s_at + 32 * h + 16 * q, pk);
       }
-      const float total = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-      l += folded ? total / rv : total;
+      const float2 s2 = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+      l = fmaf(s2.x + s2.y, sc[4 + h], l);
     }
     tmem_st_wait();
     tc_fence_before();
@@ -555,11 +577,14 @@ prefill_fp8_kernel(PrefillP p) {
   const uint32_t tmem = *sm.tmem_slot();
   qb_pdl_trigger();  // after the TMEM allocation: the next kernel cannot take it from this CTA
   if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PF_REG_SOFTMAX));
     prefill_softmax(p, sm, w, tmem, warp >> 2, split);
   } else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_REG_CONVERT));
     prefill_convert(p, sm, w);
-  } else if (lane == 0) {
-    prefill_mma(p, sm, w, tmem);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_REG_MMA));
+    if (warp == 12 && lane == 0) prefill_mma(p, sm, w, tmem);
   }
   __syncwarp();
   tc_fence_before();
