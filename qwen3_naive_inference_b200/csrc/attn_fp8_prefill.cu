@@ -7,14 +7,14 @@
 //
 // A CTA takes up to 256 query rows of one sequence and kv head -- row R is query position R / group, head
 // R % group, so the group's heads share every key -- as two tiles of 128 rows, A and B, and walks the
-// keys in tiles of 128:
+// keys a block of 64 at a time:
 //   warps 0-3, 4-7  softmax of tile A, of tile B: a thread per row
-//   warps 8-11      convert: codes come from global memory a tile ahead, become halves (exactly) and go
-//                   to shared memory in the swizzled layout of the MMA operands
-//   warp 12         (of a warpgroup otherwise idle) one thread issues the MMAs:  S_x = Q_x K^T (both operands in shared memory),
-//                   O_x += P_x V (P_x from TMEM, over the columns of S_x)
-// While one tile's softmax runs, the tensor pipe works on the other's products.  TMEM: S_A, S_B, O_A, O_B
-// of 128 columns each.
+//   warps 8-11      convert: codes come from global memory a block ahead, become halves (exactly) and go
+//                   to shared memory in the swizzled layout of the MMA operands (rings of four blocks)
+//   warp 12         one thread issues the MMAs:  S_x = Q_x K^T (both operands in shared memory),
+//                   O_x += P_x V (P_x from TMEM, over the columns of its S_x)
+// S_x has two buffers in TMEM, so the scores of block j + 1 are ready when the softmax is done with block
+// j: the softmax warps never wait for the tensor pipe.  TMEM: four S buffers of 64 columns, O_A, O_B of 128.
 // Q enters as halves scaled by a power of two per row (its largest value in [2^9, 2^10): bf16 values stay
 // exact down to 2^-23 of it); ks and the softmax scale meet the fp32 scores.  P = 2^(x - ref) is rounded
 // to halves: ref is set 4 below the largest score and moved when a score passes it by 12.  vs joins P
@@ -34,28 +34,25 @@
 
 namespace {
 
-constexpr int PF_KEYS = 128;                       // keys of a tile: two blocks
+constexpr int PF_KEYS = KV8_BLOCK;                 // keys of a tile: one block, one ks, one vs
 constexpr int PF_ROWS = 128;                       // rows of a query tile
-constexpr int PF_THREADS = 16 * 32;                // 128 registers a thread at launch, 65536 in all ...
-constexpr int PF_REG_SOFTMAX = 176, PF_REG_CONVERT = 104, PF_REG_MMA = 56;  // ... shared out by warpgroup
-static_assert(256 * PF_REG_SOFTMAX + 128 * PF_REG_CONVERT + 128 * PF_REG_MMA == 65536, "the launch's registers");
-constexpr int PF_HALF = 128 * 64 * 2;              // [128 x 64] halves: 16 KB
-constexpr int PF_TILE = 2 * PF_HALF;               // [128 x 128]: element halves 0-63, 64-127
-constexpr int PF_STAGES = 2;
-constexpr int PF_Q = 0, PF_K = 2 * PF_TILE, PF_V = PF_K + PF_STAGES * PF_TILE;
-constexpr int PF_META = PF_V + PF_STAGES * PF_TILE;
-constexpr int PF_SLOTS = 4;                        // tiles whose scales are held
-constexpr int PF_BARS = 17;
+constexpr int PF_THREADS = 13 * 32;
+constexpr int PF_Q_HALF = PF_ROWS * 64 * 2, PF_Q_TILE = 2 * PF_Q_HALF;  // element halves 0-63, 64-127
+constexpr int PF_KV_HALF = PF_KEYS * 64 * 2, PF_KV_TILE = 2 * PF_KV_HALF;
+constexpr int PF_STAGES = 4;
+constexpr int PF_Q = 0, PF_K = 2 * PF_Q_TILE, PF_V = PF_K + PF_STAGES * PF_KV_TILE;
+constexpr int PF_META = PF_V + PF_STAGES * PF_KV_TILE;
+constexpr int PF_SLOTS = 8, PF_SLOT = 8;           // tiles whose scales are held, words of one
+constexpr int PF_BARS = 4 * PF_STAGES + 15;
 // barriers; TMEM slot, abort flag; row factors; per slot the tile's scales and NaN keys
-constexpr int PF_SLOT = 16;                        // words of a slot
 constexpr int PF_SMEM = PF_META + PF_BARS * 8 + 8 + 2 * PF_ROWS * 4 + PF_SLOTS * PF_SLOT * 4 + 1024 /*align*/;
-constexpr uint32_t PF_COL_S = 0, PF_COL_O = 256;   // + 128 * tile
+constexpr uint32_t PF_COL_S = 0, PF_COL_O = 256;   // S: + 128 * query tile + 64 * buffer; O: + 128 * query tile
 constexpr float PF_HEAD = 4.f, PF_SLACK = 12.f, PF_VSLACK = 8.f, PF_VLOW = 1.f / 1024;
 constexpr int PF_WS_ROW = KV8_D + 4;
 
-// kind::f16, D fp32, A and B f16, M = N = 128; S: both K-major, O: B (V) MN-major.
-constexpr uint32_t PF_IDESC_S = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
-constexpr uint32_t PF_IDESC_O = PF_IDESC_S | (1u << 16);
+// kind::f16, D fp32, A and B f16, M = 128; S: N = 64, both K-major; O: N = 128, B (V) MN-major.
+constexpr uint32_t PF_IDESC_S = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
+constexpr uint32_t PF_IDESC_O = (1u << 4) | (1u << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
 
 struct PrefillP {
   const bf16* q;
@@ -108,36 +105,43 @@ QB_DEVICE void fence_async_shared() { asm volatile("fence.proxy.async.shared::ct
 QB_DEVICE void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-// 16-byte chunk c (of 16) of row r of a [128 x 128] half tile in the swizzled operand layout
-QB_DEVICE uint32_t operand_chunk(int r, int c) {
-  return (uint32_t)((c >> 3) * PF_HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+// 16-byte chunk c (of 16) of row r of a tile of halves in the swizzled operand layout, its element halves
+// `half` bytes apart
+QB_DEVICE uint32_t operand_chunk(int r, int c, int half) {
+  return (uint32_t)((c >> 3) * half + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
 struct PrefillSmem {
   uint32_t base;
   uint8_t* ptr;
-  QB_DEVICE uint32_t q(int x) const { return base + PF_Q + x * PF_TILE; }
-  QB_DEVICE uint32_t k(int s) const { return base + PF_K + s * PF_TILE; }
-  QB_DEVICE uint32_t v(int s) const { return base + PF_V + s * PF_TILE; }
+  QB_DEVICE uint32_t q(int x) const { return base + PF_Q + x * PF_Q_TILE; }
+  QB_DEVICE uint32_t k(int j) const { return base + PF_K + j % PF_STAGES * PF_KV_TILE; }
+  QB_DEVICE uint32_t v(int j) const { return base + PF_V + j % PF_STAGES * PF_KV_TILE; }
+  // barriers; those of key tile j, and the phase of the ring that j is in
   QB_DEVICE uint32_t bar(int i) const { return base + PF_META + 8 * i; }
-  QB_DEVICE uint32_t q_full(int x) const { return bar(x); }
-  QB_DEVICE uint32_t k_full(int s) const { return bar(2 + s); }
-  QB_DEVICE uint32_t k_empty(int s) const { return bar(4 + s); }
-  QB_DEVICE uint32_t v_full(int s) const { return bar(6 + s); }
-  QB_DEVICE uint32_t v_empty(int s) const { return bar(8 + s); }
-  QB_DEVICE uint32_t s_full(int x) const { return bar(10 + x); }
-  QB_DEVICE uint32_t p_ready(int x) const { return bar(12 + x); }
-  QB_DEVICE uint32_t pv_done(int x) const { return bar(14 + x); }
-  QB_DEVICE uint32_t all_done() const { return bar(16); }
+  QB_DEVICE uint32_t k_full(int j) const { return bar(j % PF_STAGES); }
+  QB_DEVICE uint32_t k_empty(int j) const { return bar(PF_STAGES + j % PF_STAGES); }
+  QB_DEVICE uint32_t v_full(int j) const { return bar(2 * PF_STAGES + j % PF_STAGES); }
+  QB_DEVICE uint32_t v_empty(int j) const { return bar(3 * PF_STAGES + j % PF_STAGES); }
+  QB_DEVICE uint32_t phase(int j) const { return (uint32_t)(j / PF_STAGES) & 1u; }
+  // A waiter tells a barrier's phases apart by their parity, so it may be one phase late and no more:
+  // S and P of tile j + 1 can be complete before P of j has been waited for, so each has a barrier per
+  // buffer (phase j / 2); pv_done (phase j) is waited for by those without whom j + 1 does not begin.
+  QB_DEVICE uint32_t s_full(int x, int j) const { return bar(4 * PF_STAGES + 2 * x + (j & 1)); }
+  QB_DEVICE uint32_t p_ready(int x, int j) const { return bar(4 * PF_STAGES + 4 + 2 * x + (j & 1)); }
+  QB_DEVICE uint32_t pv_done(int x) const { return bar(4 * PF_STAGES + 8 + x); }  // but for the last tile:
+  QB_DEVICE uint32_t o_last(int x) const { return bar(4 * PF_STAGES + 10 + x); }
+  QB_DEVICE uint32_t q_full(int x) const { return bar(4 * PF_STAGES + 12 + x); }
+  QB_DEVICE uint32_t all_done() const { return bar(4 * PF_STAGES + 14); }
   QB_DEVICE uint32_t* tmem_slot() const { return reinterpret_cast<uint32_t*>(ptr + PF_META + 8 * PF_BARS); }
   QB_DEVICE volatile int* abort_flag() const { return reinterpret_cast<volatile int*>(tmem_slot() + 1); }
   QB_DEVICE float* row_fac() const { return reinterpret_cast<float*>(tmem_slot() + 2); }
-  // slot of tile j; of its blocks h = 0, 1:
-  //   [h] ks (negative: no such page), [2 + h] the exponent that weighs P by vs / vref (0: it is not
-  //   weighed there), [4 + h] the factor that takes this out of the sum, [6 + h] the factor of P after it;
-  //   [8] what O is multiplied by before the tile (vref has moved), [9] vref; [12..15] bits of NaN keys
-  QB_DEVICE float* scales(int j) const { return row_fac() + 2 * PF_ROWS + (j % PF_SLOTS) * PF_SLOT; }
-  QB_DEVICE uint32_t* nan_keys(int j) const { return reinterpret_cast<uint32_t*>(scales(j) + 12); }
+  // slot of key tile j: [0] ks (negative: no such page), [1] the exponent that weighs P by vs / vref (0: it
+  // is not weighed there), [2] the factor that takes this out of the sum, [3] the factor of P after it,
+  // [4] what O is multiplied by before the tile (vref has moved), [5] vref; [6], [7] bits of NaN keys.
+  // Eight slots: a slot is written for tile j + 8 when S of j + 4 is done, so the softmax is past j + 2.
+  QB_DEVICE float* scales(int j) const { return row_fac() + 2 * PF_ROWS + j % PF_SLOTS * PF_SLOT; }
+  QB_DEVICE uint32_t* nan_keys(int j) const { return reinterpret_cast<uint32_t*>(scales(j) + 6); }
 };
 
 // What a CTA works on.
@@ -157,7 +161,7 @@ QB_DEVICE void put_codes(uint32_t tile, int r, int c, const uint4& u) {
     h[2 * i] = e4m3x2_to_half2(w[i] & 0xffffu);
     h[2 * i + 1] = e4m3x2_to_half2(w[i] >> 16);
   }
-  const uint32_t at = tile + operand_chunk(r, 2 * c);
+  const uint32_t at = tile + operand_chunk(r, 2 * c, PF_KV_HALF);
   st_shared16(at, h[0], h[1], h[2], h[3]);
   st_shared16(at ^ 16u, h[4], h[5], h[6], h[7]);
 }
@@ -167,84 +171,73 @@ QB_DEVICE uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x0101010
 // ------------------------------------------------------------------ converters
 QB_DEVICE void prefill_convert(const PrefillP& p, const PrefillSmem& sm, const PrefillWork& w) {
   const int tid = threadIdx.x - 8 * 32, n = max(w.n[0], w.n[1]);
-  // keys row0 + 16 i, i < 8 (block i / 4); eight threads in a row store to eight different bank groups:
-  // even chunks of one element half of two neighbouring keys
+  // keys row0 + 16 i, i < 4; eight threads in a row store to eight different bank groups: even chunks of
+  // one element half of two neighbouring keys
   const int chunk = (tid & 3) | ((tid >> 1) & 4), row0 = ((tid >> 4) << 1) | ((tid >> 2) & 1);
   const int first_masked = w.shift + w.q0 + 1;  // keys from here on are behind the first row's last one
-  uint4 kr[8], vr[8];
-  // Codes of key tile j in registers (rows past the keys and tiles without a page: zero)
-  int64_t at[2];
+  // Codes of a key tile in registers (rows past the keys and tiles without a page: zero), and, in thread
+  // 0, its scales.
+  uint4 kr[4], vr[4];
+  float ks = -1.f, vs = 0.f, vref = 0.f;
+  int64_t at = -1;  // (page, head, block) of the tile that is loaded
   auto find = [&](int j) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int key = w.begin + j * PF_KEYS + h * KV8_BLOCK, col = key / KV8_PAGE;
-      at[h] = -1;
-      if (key >= w.end) continue;
-      const int page = col < p.bt_width ? p.bt[(int64_t)w.b * p.bt_stride + col] : -1;
-      if (page >= 0 && page < p.num_blocks)
-        at[h] = ((int64_t)page * p.hkv + w.kvh) * KV8_SUBS + key % KV8_PAGE / KV8_BLOCK;
-      else if (tid == 0)
-        qb_set_err(p.err, QB_DEVERR_PAGE);
-    }
+    const int key = w.begin + j * PF_KEYS, col = key / KV8_PAGE;
+    const int page = col < p.bt_width ? p.bt[(int64_t)w.b * p.bt_stride + col] : -1;
+    at = -1;
+    if (page >= 0 && page < p.num_blocks)
+      at = ((int64_t)page * p.hkv + w.kvh) * KV8_SUBS + key % KV8_PAGE / KV8_BLOCK;
+    else if (tid == 0)
+      qb_set_err(p.err, QB_DEVERR_PAGE);
   };
-  auto load = [&](const uint8_t* codes, uint4 (&r)[8], int j) {
+  auto load = [&](const uint8_t* codes, uint4 (&r)[4], int j) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const int key = row0 + 16 * i;
       r[i] = make_uint4(0, 0, 0, 0);
-      if (at[i >> 2] >= 0 && w.begin + j * PF_KEYS + key < w.end)
-        r[i] = *reinterpret_cast<const uint4*>(codes + at[i >> 2] * KV8_TILE + (key % KV8_BLOCK) * KV8_D + chunk * 16);
+      if (at >= 0 && w.begin + j * PF_KEYS + key < w.end)
+        r[i] = *reinterpret_cast<const uint4*>(codes + at * KV8_TILE + key * KV8_D + chunk * 16);
     }
   };
-  float ks_next[2], vs_next[2], vref = 0.f;  // thread 0: the scales of the next tile
   auto load_scales = [&]() {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      ks_next[h] = tid == 0 && at[h] >= 0 ? p.ks[at[h]] : -1.f;
-      vs_next[h] = tid == 0 && at[h] >= 0 ? p.vs[at[h]] : 0.f;
-    }
+    if (tid != 0) return;
+    ks = at >= 0 ? p.ks[at] : -1.f;
+    vs = at >= 0 ? p.vs[at] : 0.f;
   };
   find(0);
   load(p.k, kr, 0);
   load_scales();
   load(p.v, vr, 0);
   for (int j = 0; j < n; ++j) {
-    const int s = j % PF_STAGES;
-    const uint32_t ph = ((uint32_t)(j / PF_STAGES) & 1u) ^ 1u;
     if (j + 1 < n) find(j + 1);
-    if (!mbar_wait(sm.k_empty(s), ph, sm.abort_flag(), p.err)) return;
+    if (!mbar_wait(sm.k_empty(j), sm.phase(j) ^ 1, sm.abort_flag(), p.err)) return;
     if (tid == 0) {
       float* sc = sm.scales(j);
-      const float top = fmaxf(vs_next[0], vs_next[1]);
-      sc[8] = 1.f;
-      if (top > vref * PF_VSLACK) {
-        sc[8] = vref / top;
-        vref = top;
+      sc[4] = 1.f;
+      if (vs > vref * PF_VSLACK) {
+        sc[4] = vref / vs;
+        vref = vs;
       }
-      sc[9] = vref;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float rv = vref > 0.f ? vs_next[h] / vref : 0.f;
-        const bool folded = rv >= PF_VLOW;
-        sc[h] = ks_next[h];
-        sc[2 + h] = folded ? log2f(rv) : 0.f;
-        sc[4 + h] = folded ? 1.f / rv : 1.f;
-        sc[6 + h] = folded ? 1.f : rv;
-      }
+      const float rv = vref > 0.f ? vs / vref : 0.f;
+      const bool folded = rv >= PF_VLOW;
+      sc[0] = ks;
+      sc[1] = folded ? log2f(rv) : 0.f;
+      sc[2] = folded ? 1.f / rv : 1.f;
+      sc[3] = folded ? 1.f : rv;
+      sc[5] = vref;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) put_codes(sm.k(s), row0 + 16 * i, chunk, kr[i]);
+    for (int i = 0; i < 4; ++i) put_codes(sm.k(j), row0 + 16 * i, chunk, kr[i]);
     if (j + 1 < n) {
       load(p.k, kr, j + 1);
       load_scales();
     }
     fence_async_shared();
-    mbar_arrive(sm.k_full(s));
-    if (!mbar_wait(sm.v_empty(s), ph, sm.abort_flag(), p.err)) return;
+    mbar_arrive(sm.k_full(j));
+    if (!mbar_wait(sm.v_empty(j), sm.phase(j) ^ 1, sm.abort_flag(), p.err)) return;
     if (w.begin + (j + 1) * PF_KEYS > first_masked) {
       // some row sees this tile in part: no NaN may reach the product of a masked key
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 4; ++i) {
         const uint32_t bad[4] = {nan_bytes(vr[i].x), nan_bytes(vr[i].y), nan_bytes(vr[i].z), nan_bytes(vr[i].w)};
         if (bad[0] | bad[1] | bad[2] | bad[3]) {
           vr[i].x &= ~((bad[0] >> 7) * 0xffu);
@@ -257,10 +250,10 @@ QB_DEVICE void prefill_convert(const PrefillP& p, const PrefillSmem& sm, const P
       }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) put_codes(sm.v(s), row0 + 16 * i, chunk, vr[i]);
+    for (int i = 0; i < 4; ++i) put_codes(sm.v(j), row0 + 16 * i, chunk, vr[i]);
     if (j + 1 < n) load(p.v, vr, j + 1);
     fence_async_shared();
-    mbar_arrive(sm.v_full(s));
+    mbar_arrive(sm.v_full(j));
   }
 }
 
@@ -269,47 +262,37 @@ QB_DEVICE void prefill_mma(const PrefillP& p, const PrefillSmem& sm, const Prefi
   volatile int* ab = sm.abort_flag();
   const int n = max(w.n[0], w.n[1]);
   bool ok = mbar_wait(sm.q_full(0), 0, ab, p.err) && (w.n[1] == 0 || mbar_wait(sm.q_full(1), 0, ab, p.err));
-  auto scores = [&](int x, int j) {
-    const uint32_t k = sm.k(j % PF_STAGES);
-    tc_fence_after();
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      umma_bf16(tmem + PF_COL_S + x * 128, sw128_kmajor_desc(sm.q(x) + (i >> 2) * PF_HALF + (i & 3) * 32),
-                sw128_kmajor_desc(k + (i >> 2) * PF_HALF + (i & 3) * 32), PF_IDESC_S, i > 0);
-    umma_commit(sm.s_full(x));
-  };
-  ok = ok && mbar_wait(sm.k_full(0), 0, ab, p.err);
-  if (ok) {
-    for (int x = 0; x < 2; ++x)
-      if (w.n[x] > 0) scores(x, 0);
-    umma_commit(sm.k_empty(0));
-  }
-  for (int j = 0; ok && j < n; ++j) {
-    const int s = j % PF_STAGES;
-    ok = mbar_wait(sm.v_full(s), (uint32_t)(j / PF_STAGES) & 1u, ab, p.err);
-    bool have_k = false;
-    for (int x = 0; ok && x < 2; ++x) {
+  // S of key tile j for both query tiles.  Its buffer held P of j - 2.
+  auto scores = [&](int j) {
+    if (!mbar_wait(sm.k_full(j), sm.phase(j), ab, p.err)) return false;
+    for (int x = 0; x < 2; ++x) {
       if (j >= w.n[x]) continue;
-      if (!(ok = mbar_wait(sm.p_ready(x), (uint32_t)j & 1u, ab, p.err))) break;
+      if (j >= 2 && !mbar_wait(sm.pv_done(x), (uint32_t)j & 1u, ab, p.err)) return false;
       tc_fence_after();
 #pragma unroll
-      for (int i = 0; i < 8; ++i)  // 128 keys in steps of 16: P columns 8 i, V rows 16 i
-        umma_bf16_ts(tmem + PF_COL_O + x * 128, tmem + PF_COL_S + x * 128 + 8 * i,
-                     sw128_mn_desc(sm.v(s) + i * 16 * 128, PF_HALF), PF_IDESC_O, (j > 0 || i > 0) ? 1u : 0u);
-      umma_commit(sm.pv_done(x));
-      if (j + 1 < w.n[x]) {  // the next scores go over P's columns: its product has to be through
-        if (!have_k &&
-            !(ok = mbar_wait(sm.k_full((j + 1) % PF_STAGES), (uint32_t)((j + 1) / PF_STAGES) & 1u, ab, p.err)))
-          break;
-        have_k = true;
-        if (!(ok = mbar_wait(sm.pv_done(x), (uint32_t)j & 1u, ab, p.err))) break;
-        scores(x, j + 1);
-      }
+      for (int i = 0; i < 8; ++i)  // 128 elements in steps of 16
+        umma_bf16(tmem + PF_COL_S + x * 128 + (j & 1) * 64, sw128_kmajor_desc(sm.q(x) + (i >> 2) * PF_Q_HALF + (i & 3) * 32),
+                  sw128_kmajor_desc(sm.k(j) + (i >> 2) * PF_KV_HALF + (i & 3) * 32), PF_IDESC_S, i > 0);
+      umma_commit(sm.s_full(x, j));
     }
-    if (ok) {
-      umma_commit(sm.v_empty(s));
-      if (j + 1 < n) umma_commit(sm.k_empty((j + 1) % PF_STAGES));
+    umma_commit(sm.k_empty(j));
+    return true;
+  };
+  ok = ok && scores(0);
+  for (int j = 0; ok && j < n; ++j) {
+    if (j + 1 < n && !(ok = scores(j + 1))) break;
+    if (!(ok = mbar_wait(sm.v_full(j), sm.phase(j), ab, p.err))) break;
+    for (int x = 0; ok && x < 2; ++x) {
+      if (j >= w.n[x]) continue;
+      if (!(ok = mbar_wait(sm.p_ready(x, j), (uint32_t)(j >> 1) & 1u, ab, p.err))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)  // 64 keys in steps of 16: P columns 8 i, V rows 16 i
+        umma_bf16_ts(tmem + PF_COL_O + x * 128, tmem + PF_COL_S + x * 128 + (j & 1) * 64 + 8 * i,
+                     sw128_mn_desc(sm.v(j) + i * 16 * 128, PF_KV_HALF), PF_IDESC_O, (j > 0 || i > 0) ? 1u : 0u);
+      umma_commit(j + 1 < w.n[x] ? sm.pv_done(x) : sm.o_last(x));
     }
+    if (ok) umma_commit(sm.v_empty(j));
   }
   // no MMA may still be reading shared memory or writing TMEM when the CTA leaves
   umma_commit(sm.all_done());
@@ -342,7 +325,7 @@ QB_DEVICE void prefill_load_q(const PrefillP& p, const PrefillSmem& sm, const Pr
     float mul = __uint_as_float((uint32_t)(263 - e) << 23);
     if (p.scale_log2 < 0.f) mul = -mul;  // the scores' factor is then positive
     if (l == 0) sm.row_fac()[R] = __uint_as_float((uint32_t)(e - 9) << 23) * fabsf(p.scale_log2);
-    st_shared16(sm.q(x) + operand_chunk(r, l), pack_half2(f[0] * mul, f[1] * mul), pack_half2(f[2] * mul, f[3] * mul),
+    st_shared16(sm.q(x) + operand_chunk(r, l, PF_Q_HALF), pack_half2(f[0] * mul, f[1] * mul), pack_half2(f[2] * mul, f[3] * mul),
                 pack_half2(f[4] * mul, f[5] * mul), pack_half2(f[6] * mul, f[7] * mul));
   }
   fence_async_shared();
@@ -360,117 +343,103 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
   bool ok = __all_sync(0xffffffffu, mbar_wait(sm.q_full(x), 0, ab, p.err));
   const float fac = ok ? sm.row_fac()[R] : 0.f;
   const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-  const uint32_t s_at = lanes + PF_COL_S + x * 128, o_at = lanes + PF_COL_O + x * 128;
+  const uint32_t o_at = lanes + PF_COL_O + x * 128;
   const bool live = R < w.rows;
   const int pos = w.q0 + R / group;
   const int last = live ? min(w.shift + pos, w.end - 1) : w.begin - 1;  // the row's last key here
   float ref = -INFINITY, l = 0.f, vref = 0.f;
   for (int j = 0; ok && j < n; ++j) {
     // tcgen05 loads and stores are warp-collective: every decision that leads to them is warp-uniform
-    if (!__all_sync(0xffffffffu, mbar_wait(sm.s_full(x), (uint32_t)j & 1u, ab, p.err))) {
+    if (!__all_sync(0xffffffffu, mbar_wait(sm.s_full(x, j), (uint32_t)(j >> 1) & 1u, ab, p.err))) {
       ok = false;
       break;
     }
     tc_fence_after();
-    uint32_t v[128];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) tmem_ld32_nowait(s_at + 32 * c, v + 32 * c);
+    const uint32_t s_at = lanes + PF_COL_S + x * 128 + (j & 1) * 64;
+    uint32_t v[64];
+    tmem_ld32_nowait(s_at, v);
+    tmem_ld32_nowait(s_at + 32, v + 32);
     const float* sc = sm.scales(j);
-    const float ks0 = sc[0], ks1 = sc[1], vfac = sc[8];
-    vref = sc[9];
-    const int k0 = w.begin + j * PF_KEYS;
-    const int seen = last - k0 + 1;  // keys of the tile that the row sees
-    const bool whole = __all_sync(0xffffffffu, seen >= PF_KEYS) && ks0 >= 0.f && ks1 >= 0.f;
-    // not zero: -inf (a key not seen) has to stay -inf
-    const float f0 = fmaxf(fac * ks0, FLT_MIN), f1 = fmaxf(fac * ks1, FLT_MIN);
+    const float ks = sc[0], weight = sc[1], unweigh = sc[2], after = sc[3], vfac = sc[4];
+    vref = sc[5];
+    const int seen = ks < 0.f ? 0 : last - (w.begin + j * PF_KEYS) + 1;  // keys of the tile that the row sees
+    const float f = fmaxf(fac * ks, FLT_MIN);  // not zero: -inf (a key not seen) has to stay -inf
+    const bool whole = __all_sync(0xffffffffu, seen >= PF_KEYS);
     tmem_ld_wait();
-    if (!whole) {
-      const int see0 = ks0 < 0.f ? 0 : seen, see1 = ks1 < 0.f ? 0 : seen - 64;
 #pragma unroll
-      for (int i = 0; i < 64; ++i) {
-        if (i >= see0) v[i] = __float_as_uint(-INFINITY);
-        if (i >= see1) v[64 + i] = __float_as_uint(-INFINITY);
-      }
+    for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(v[i]));  // no use of a score moves above the wait
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < 64; ++i)
+        if (i >= seen) v[i] = __float_as_uint(-INFINITY);
     }
     float top[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top[i] = __uint_as_float(v[16 * i]);
+    for (int c = 0; c < 8; ++c) top[c] = __uint_as_float(v[c]);
 #pragma unroll
-    for (int i = 1; i < 16; ++i)
-#pragma unroll
-      for (int c = 0; c < 8; ++c) top[c] = fmaxf(top[c], __uint_as_float(v[16 * c + i]));
-    const float mt = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f0,
-                           fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])) * f1);
+    for (int i = 8; i < 64; ++i) top[i & 7] = fmaxf(top[i & 7], __uint_as_float(v[i]));
+    const float mt = f * fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])),
+                               fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])));
     const bool need = mt > ref + PF_SLACK;
-    float a = 1.f;
-    if (need) {
-      const float to = mt - PF_HEAD;
-      a = ref == -INFINITY ? 0.f : fast_exp2(ref - to);
-      ref = to;
-      l *= a;
-    }
-    a *= vfac;
-    if (j > 0 && (__any_sync(0xffffffffu, need) || vfac != 1.f)) {
-      // O holds the tiles before: wait for the last of them, weigh them anew
-      if (!__all_sync(0xffffffffu, mbar_wait(sm.pv_done(x), (uint32_t)(j - 1) & 1u, ab, p.err))) {
-        ok = false;
-        break;
+    if (__any_sync(0xffffffffu, need) || vfac != 1.f) {
+      float a = vfac;
+      if (need) {
+        const float to = mt - PF_HEAD, alpha = ref == -INFINITY ? 0.f : fast_exp2(ref - to);
+        ref = to;
+        l *= alpha;
+        a *= alpha;
       }
-      tc_fence_after();
+      if (j > 0) {  // O holds the tiles before: wait for the last of them, weigh them anew
+        if (!__all_sync(0xffffffffu, mbar_wait(sm.pv_done(x), (uint32_t)(j - 1) & 1u, ab, p.err))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
 #pragma unroll 1
-      for (int c = 0; c < 128; c += 32) {
-        uint32_t o[32];
-        tmem_ld32(o_at + c, o);
+        for (int c = 0; c < 128; c += 16) {
+          uint32_t o[16];
+          tmem_ld16(o_at + c, o);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
-        tmem_st32(o_at + c, o);
+          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+          tmem_st16(o_at + c, o);
+        }
       }
     }
-    const float base = ref == -INFINITY ? 0.f : ref;
+    const float shift = weight - (ref == -INFINITY ? 0.f : ref);
+    const float2 ff = make_float2(f, f), ss = make_float2(shift, shift);
+    float2 sum[4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float2 ff = make_float2(h ? f1 : f0, h ? f1 : f0);
-      const float shift = sc[2 + h] - base;
-      const float2 ss = make_float2(shift, shift);
-      float2 sum[4];
+    for (int c = 0; c < 4; ++c) sum[c] = make_float2(0.f, 0.f);
+    uint32_t pk[32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) sum[c] = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t* u = v + 64 * h + 32 * q;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float2 y = fma2(make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])), ff, ss);
-          y.x = fast_exp2(y.x);
-          y.y = fast_exp2(y.y);
-          sum[i & 3] = add2(sum[i & 3], y);
-          u[2 * i] = __float_as_uint(y.x);
-          u[2 * i + 1] = __float_as_uint(y.y);
-        }
-        if (sc[6 + h] != 1.f) {  // the same for every thread of the CTA
-          const float rv = sc[6 + h];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * rv);
-        }
-        uint32_t pk[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) pk[i] = pack_half2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
-        tmem_st16(s_at + 32 * h + 16 * q, pk);
-      }
-      const float2 s2 = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
-      l = fmaf(s2.x + s2.y, sc[4 + h], l);
+    for (int i = 0; i < 32; ++i) {
+      float2 y = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ff, ss);
+      y.x = fast_exp2(y.x);
+      y.y = fast_exp2(y.y);
+      sum[i & 3] = add2(sum[i & 3], y);
+      pk[i] = pack_half2(y.x, y.y);
     }
+    if (after != 1.f) {  // (the same for every thread of the CTA) weigh in fp32, from the probabilities again
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float2 y = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ff, ss);
+        pk[i] = pack_half2(fast_exp2(y.x) * after, fast_exp2(y.y) * after);
+      }
+    }
+    tmem_st32(s_at, pk);
+    const float2 s2 = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+    l = fmaf(s2.x + s2.y, unweigh, l);
     tmem_st_wait();
     tc_fence_before();
-    mbar_arrive(sm.p_ready(x));
+    mbar_arrive(sm.p_ready(x, j));
   }
-  if (!ok || !__all_sync(0xffffffffu, mbar_wait(sm.pv_done(x), (uint32_t)(n - 1) & 1u, ab, p.err))) return;
+  if (!ok || !__all_sync(0xffffffffu, mbar_wait(sm.o_last(x), 0, ab, p.err))) return;
   tc_fence_after();
   float inv = l == 0.f ? 0.f : vref / l;
   // NaN values that the converters took out of the tiles some row sees in part (every V has been read)
   for (int j = max(0, w.shift + w.q0 + 1 - w.begin) / PF_KEYS; j < n; ++j)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 2; ++k) {
       const int m = last - (w.begin + j * PF_KEYS + 32 * k) + 1;  // keys of the word that the row sees
       const uint32_t mine = m >= 32 ? 0xffffffffu : (m <= 0 ? 0u : (1u << m) - 1u);
       if (sm.nan_keys(j)[k] & mine) inv = __int_as_float(0x7fffffff);
@@ -549,21 +518,25 @@ prefill_fp8_kernel(PrefillP p) {
   sm.ptr = smem_raw + (sm.base - raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(sm.q_full(i), 128);
+    for (int i = 0; i < PF_STAGES; ++i) {
       mbar_init(sm.k_full(i), 128);
       mbar_init(sm.k_empty(i), 1);
       mbar_init(sm.v_full(i), 128);
       mbar_init(sm.v_empty(i), 1);
-      mbar_init(sm.s_full(i), 1);
-      mbar_init(sm.p_ready(i), 128);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(sm.q_full(i), 128);
+      mbar_init(sm.s_full(i, 0), 1);
+      mbar_init(sm.s_full(i, 1), 1);
+      mbar_init(sm.p_ready(i, 0), 128);
+      mbar_init(sm.p_ready(i, 1), 128);
       mbar_init(sm.pv_done(i), 1);
+      mbar_init(sm.o_last(i), 1);
     }
     mbar_init(sm.all_done(), 1);
     *sm.abort_flag() = 0;
-    // tiles that some row sees in part are the last three at most: their slots are used once
-    for (int j = 0; j < PF_SLOTS; ++j)
-      for (int k = 0; k < 4; ++k) sm.nan_keys(j)[k] = 0;
+    // tiles that some row sees in part are the last five at most: their slots' NaN keys are written once
+    for (int j = 0; j < PF_SLOTS; ++j) sm.nan_keys(j)[0] = sm.nan_keys(j)[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 12) {
@@ -577,14 +550,11 @@ prefill_fp8_kernel(PrefillP p) {
   const uint32_t tmem = *sm.tmem_slot();
   qb_pdl_trigger();  // after the TMEM allocation: the next kernel cannot take it from this CTA
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PF_REG_SOFTMAX));
     prefill_softmax(p, sm, w, tmem, warp >> 2, split);
   } else if (warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_REG_CONVERT));
     prefill_convert(p, sm, w);
-  } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_REG_MMA));
-    if (warp == 12 && lane == 0) prefill_mma(p, sm, w, tmem);
+  } else if (lane == 0) {
+    prefill_mma(p, sm, w, tmem);
   }
   __syncwarp();
   tc_fence_before();
@@ -650,7 +620,7 @@ extern "C" int qb_attn_paged_prefill_fp8(const void* q, int64_t q_stride, const 
                                          int64_t o_stride, int64_t total_q, int* err, qb_stream_t stream) {
   if (D != KV8_D || page_size != KV8_PAGE) return QB_ERR_UNSUPPORTED;
   QB_CHECK_ARG(batch >= 0 && total_q >= 0 && total_q <= INT32_MAX && n_tiles >= 0 && tiles_per_seq >= 0);
-  QB_CHECK_ARG(n_splits >= 1 && n_splits <= 65535 && (n_splits == 1 || (split_keys > 0 && split_keys % PF_KEYS == 0 &&
+  QB_CHECK_ARG(n_splits >= 1 && n_splits <= 65535 && (n_splits == 1 || (split_keys > 0 && split_keys % (2 * PF_KEYS) == 0 &&
                (int64_t)split_keys * n_splits <= INT32_MAX / 2)));
   if (batch == 0 || total_q == 0) return QB_OK;
   const int ok = kv8_check_cache(q, q_stride, k_cache, v_cache, k_scale, v_scale, num_blocks, block_tables, bt_stride,

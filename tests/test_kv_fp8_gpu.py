@@ -356,6 +356,29 @@ def test_prefill(cuda, hq, hkv, seqs, tiled):
     ops.check_device_errors()
 
 
+@pytest.mark.parametrize("seqs", [[(0, 512)] * 8, [(3000, 300), (0, 1000), (511, 129)], [(0, 256), (0, 257), (4000, 256)] * 3])
+def test_prefill_many_tiles(cuda, seqs):
+    """Full waves of CTAs, tiles of all depths side by side, the call repeated back to back: no wait gives up."""
+    g = gen(len(seqs))
+    lens, nq = [p + n for p, n in seqs], [n for _, n in seqs]
+    nb = sum(-(-n // PAGE) for n in lens)
+    k, v, ks, vs = random_cache(g, nb, 8)
+    table = paged(g, lens, nb)
+    cu_q = torch.tensor([0] + np.cumsum(nq).tolist(), dtype=torch.int32)
+    cu_k = torch.tensor([0] + np.cumsum(lens).tolist(), dtype=torch.int32)
+    q = torch.randn(sum(nq), 16, D, generator=g).to(BF)
+    args = on(cuda, q, k, v, ks, vs, cu_q, cu_k)
+    outs = [ops.attention_paged_prefill_fp8(*args, max(nq), table.to(cuda), 0.1) for _ in range(12)]
+    ops.check_device_errors()
+    assert all(torch.equal(o, outs[0]) for o in outs[1:])
+    k64, v64 = values(k, ks), values(v, vs)
+    for b, (past, n) in enumerate(seqs):
+        rows = slice(int(cu_q[b]), int(cu_q[b + 1]))
+        for h in (b % 16, 15 - b):
+            kv = [rows_of(c, table[b], 0, lens[b], h // 2) for c in (k64, v64)]
+            check_attention(outs[0][rows, h], *attend(q[rows, h], [kv], 0.1, past), f"sequence {b} head {h}")
+
+
 def test_prefill_nan_in_later_keys(cuda):
     """NaN in keys and values behind a row's last key, inside its own tile, stays out of the row; the rows
     that attend them are NaN."""
