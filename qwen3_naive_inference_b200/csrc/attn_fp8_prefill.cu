@@ -11,7 +11,7 @@
 //   warps 0-3, 4-7  softmax of tile A, of tile B: a thread per row
 //   warps 8-11      convert: codes come from global memory a block ahead, become halves (exactly) and go
 //                   to shared memory in the swizzled layout of the MMA operands (rings of four blocks)
-//   warp 12         one thread issues the MMAs:  S_x = Q_x K^T (both operands in shared memory),
+//   warp 12         issues the MMAs:  S_x = Q_x K^T (both operands in shared memory),
 //                   O_x += P_x V (P_x from TMEM, over the columns of its S_x)
 // S_x has two buffers in TMEM, so the scores of block j + 1 are ready when the softmax is done with block
 // j: the softmax warps never wait for the tensor pipe.  TMEM: four S buffers of 64 columns, O_A, O_B of 128.
@@ -258,45 +258,64 @@ QB_DEVICE void prefill_convert(const PrefillP& p, const PrefillSmem& sm, const P
 }
 
 // ------------------------------------------------------------------ MMA issuer
+// The whole warp walks the loop and one elected lane issues, so that everything an MMA takes is computed
+// once for the warp, in uniform registers: with a single thread in the loop the issue of the 24 MMAs and 6
+// commits of a block took longer than their execution (2800 clocks a block against 1300).
 QB_DEVICE void prefill_mma(const PrefillP& p, const PrefillSmem& sm, const PrefillWork& w, uint32_t tmem) {
   volatile int* ab = sm.abort_flag();
   const int n = max(w.n[0], w.n[1]);
-  bool ok = mbar_wait(sm.q_full(0), 0, ab, p.err) && (w.n[1] == 0 || mbar_wait(sm.q_full(1), 0, ab, p.err));
+  uint32_t pred;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(pred));
+  const bool one = pred != 0;
+  auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, ab, p.err)) != 0; };
+  const uint64_t qd[2] = {sw128_kmajor_desc(sm.q(0)), sw128_kmajor_desc(sm.q(1))};
+  const uint64_t kd = sw128_kmajor_desc(sm.k(0)), vd = sw128_mn_desc(sm.v(0), PF_KV_HALF);
   // S of key tile j for both query tiles.  Its buffer held P of j - 2.
   auto scores = [&](int j) {
-    if (!mbar_wait(sm.k_full(j), sm.phase(j), ab, p.err)) return false;
+    if (!wait(sm.k_full(j), sm.phase(j))) return false;
+    const uint64_t k = kd + (uint64_t)(j % PF_STAGES * (PF_KV_TILE >> 4));
+#pragma unroll
     for (int x = 0; x < 2; ++x) {
       if (j >= w.n[x]) continue;
-      if (j >= 2 && !mbar_wait(sm.pv_done(x), (uint32_t)j & 1u, ab, p.err)) return false;
+      if (j >= 2 && !wait(sm.pv_done(x), (uint32_t)j & 1u)) return false;
       tc_fence_after();
+      if (one) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)  // 128 elements in steps of 16
-        umma_bf16(tmem + PF_COL_S + x * 128 + (j & 1) * 64, sw128_kmajor_desc(sm.q(x) + (i >> 2) * PF_Q_HALF + (i & 3) * 32),
-                  sw128_kmajor_desc(sm.k(j) + (i >> 2) * PF_KV_HALF + (i & 3) * 32), PF_IDESC_S, i > 0);
-      umma_commit(sm.s_full(x, j));
+        for (int i = 0; i < 8; ++i)  // 128 elements in steps of 16
+          umma_bf16(tmem + PF_COL_S + x * 128 + (j & 1) * 64, qd[x] + (((i >> 2) * PF_Q_HALF + (i & 3) * 32) >> 4),
+                    k + (((i >> 2) * PF_KV_HALF + (i & 3) * 32) >> 4), PF_IDESC_S, i > 0);
+        umma_commit(sm.s_full(x, j));
+      }
     }
-    umma_commit(sm.k_empty(j));
+    if (one) umma_commit(sm.k_empty(j));
     return true;
   };
+  bool ok = wait(sm.q_full(0), 0) && (w.n[1] == 0 || wait(sm.q_full(1), 0));
   ok = ok && scores(0);
   for (int j = 0; ok && j < n; ++j) {
     if (j + 1 < n && !(ok = scores(j + 1))) break;
-    if (!(ok = mbar_wait(sm.v_full(j), sm.phase(j), ab, p.err))) break;
-    for (int x = 0; ok && x < 2; ++x) {
-      if (j >= w.n[x]) continue;
-      if (!(ok = mbar_wait(sm.p_ready(x, j), (uint32_t)(j >> 1) & 1u, ab, p.err))) break;
-      tc_fence_after();
+    if (!(ok = wait(sm.v_full(j), sm.phase(j)))) break;
+    const uint64_t v = vd + (uint64_t)(j % PF_STAGES * (PF_KV_TILE >> 4));
 #pragma unroll
-      for (int i = 0; i < 4; ++i)  // 64 keys in steps of 16: P columns 8 i, V rows 16 i
-        umma_bf16_ts(tmem + PF_COL_O + x * 128, tmem + PF_COL_S + x * 128 + (j & 1) * 64 + 8 * i,
-                     sw128_mn_desc(sm.v(j) + i * 16 * 128, PF_KV_HALF), PF_IDESC_O, (j > 0 || i > 0) ? 1u : 0u);
-      umma_commit(j + 1 < w.n[x] ? sm.pv_done(x) : sm.o_last(x));
+    for (int x = 0; x < 2; ++x) {
+      if (!ok || j >= w.n[x]) continue;
+      if (!(ok = wait(sm.p_ready(x, j), (uint32_t)(j >> 1) & 1u))) continue;
+      tc_fence_after();
+      if (one) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // 64 keys in steps of 16: P columns 8 i, V rows 16 i
+          umma_bf16_ts(tmem + PF_COL_O + x * 128, tmem + PF_COL_S + x * 128 + (j & 1) * 64 + 8 * i,
+                       v + ((i * 16 * 128) >> 4), PF_IDESC_O, (j > 0 || i > 0) ? 1u : 0u);
+        umma_commit(j + 1 < w.n[x] ? sm.pv_done(x) : sm.o_last(x));
+      }
     }
-    if (ok) umma_commit(sm.v_empty(j));
+    if (ok && one) umma_commit(sm.v_empty(j));
   }
   // no MMA may still be reading shared memory or writing TMEM when the CTA leaves
-  umma_commit(sm.all_done());
-  mbar_drain(sm.all_done(), 0);
+  if (one) {
+    umma_commit(sm.all_done());
+    mbar_drain(sm.all_done(), 0);
+  }
 }
 
 // ------------------------------------------------------------------ softmax
@@ -516,7 +535,7 @@ prefill_fp8_kernel(PrefillP p) {
   const uint32_t raw = smem_u32(smem_raw);
   sm.base = (raw + 1023) & ~1023u;
   sm.ptr = smem_raw + (sm.base - raw);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     for (int i = 0; i < PF_STAGES; ++i) {
       mbar_init(sm.k_full(i), 128);
@@ -553,7 +572,7 @@ prefill_fp8_kernel(PrefillP p) {
     prefill_softmax(p, sm, w, tmem, warp >> 2, split);
   } else if (warp < 12) {
     prefill_convert(p, sm, w);
-  } else if (lane == 0) {
+  } else {
     prefill_mma(p, sm, w, tmem);
   }
   __syncwarp();
