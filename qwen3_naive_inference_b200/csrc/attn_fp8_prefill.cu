@@ -11,8 +11,9 @@
 //   warps 0-3, 4-7  softmax of tile A, of tile B: a thread per row
 //   warps 8-11      convert: codes come from global memory a block ahead, become halves (exactly) and go
 //                   to shared memory in the swizzled layout of the MMA operands (rings of four blocks)
-//   warp 12         issues the MMAs:  S_x = Q_x K^T (both operands in shared memory),
-//                   O_x += P_x V (P_x from TMEM, over the columns of its S_x)
+//   warps 12, 13    issue S_A, S_B = Q_x K^T (both operands in shared memory)
+//   warps 14, 15    issue O_A, O_B += P_x V (P_x from TMEM, over the columns of its S_x); each of the four
+//                   waits for its own inputs only, so no wait holds up another's MMAs
 // S_x has two buffers in TMEM, so the scores of block j + 1 are ready when the softmax is done with block
 // j: the softmax warps never wait for the tensor pipe.  TMEM: four S buffers of 64 columns, O_A, O_B of 128.
 // Q enters as halves scaled by a power of two per row (its largest value in [2^9, 2^10): bf16 values stay
@@ -36,14 +37,14 @@ namespace {
 
 constexpr int PF_KEYS = KV8_BLOCK;                 // keys of a tile: one block, one ks, one vs
 constexpr int PF_ROWS = 128;                       // rows of a query tile
-constexpr int PF_THREADS = 13 * 32;
+constexpr int PF_THREADS = 16 * 32;
 constexpr int PF_Q_HALF = PF_ROWS * 64 * 2, PF_Q_TILE = 2 * PF_Q_HALF;  // element halves 0-63, 64-127
 constexpr int PF_KV_HALF = PF_KEYS * 64 * 2, PF_KV_TILE = 2 * PF_KV_HALF;
 constexpr int PF_STAGES = 4;
 constexpr int PF_Q = 0, PF_K = 2 * PF_Q_TILE, PF_V = PF_K + PF_STAGES * PF_KV_TILE;
 constexpr int PF_META = PF_V + PF_STAGES * PF_KV_TILE;
 constexpr int PF_SLOTS = 8, PF_SLOT = 8;           // tiles whose scales are held, words of one
-constexpr int PF_BARS = 4 * PF_STAGES + 15;
+constexpr int PF_BARS = 4 * PF_STAGES + 20;
 // barriers; TMEM slot, abort flag; row factors; per slot the tile's scales and NaN keys
 constexpr int PF_SMEM = PF_META + PF_BARS * 8 + 8 + 2 * PF_ROWS * 4 + PF_SLOTS * PF_SLOT * 4 + 1024 /*align*/;
 constexpr uint32_t PF_COL_S = 0, PF_COL_O = 256;   // S: + 128 * query tile + 64 * buffer; O: + 128 * query tile
@@ -124,15 +125,16 @@ struct PrefillSmem {
   QB_DEVICE uint32_t v_full(int j) const { return bar(2 * PF_STAGES + j % PF_STAGES); }
   QB_DEVICE uint32_t v_empty(int j) const { return bar(3 * PF_STAGES + j % PF_STAGES); }
   QB_DEVICE uint32_t phase(int j) const { return (uint32_t)(j / PF_STAGES) & 1u; }
-  // A waiter tells a barrier's phases apart by their parity, so it may be one phase late and no more:
-  // S and P of tile j + 1 can be complete before P of j has been waited for, so each has a barrier per
-  // buffer (phase j / 2); pv_done (phase j) is waited for by those without whom j + 1 does not begin.
+  // A waiter tells a barrier's phases apart by their parity, so it may be one phase late and no more.  S, P
+  // and P V of tile j + 1 can be complete before those of j have been waited for, so each has a barrier per
+  // buffer, whose next phase (tile j + 2) does not begin without the waiter.  Phase of tile j: j / 2.
   QB_DEVICE uint32_t s_full(int x, int j) const { return bar(4 * PF_STAGES + 2 * x + (j & 1)); }
   QB_DEVICE uint32_t p_ready(int x, int j) const { return bar(4 * PF_STAGES + 4 + 2 * x + (j & 1)); }
-  QB_DEVICE uint32_t pv_done(int x) const { return bar(4 * PF_STAGES + 8 + x); }  // but for the last tile:
-  QB_DEVICE uint32_t o_last(int x) const { return bar(4 * PF_STAGES + 10 + x); }
-  QB_DEVICE uint32_t q_full(int x) const { return bar(4 * PF_STAGES + 12 + x); }
-  QB_DEVICE uint32_t all_done() const { return bar(4 * PF_STAGES + 14); }
+  QB_DEVICE uint32_t pv_done(int x, int j) const { return bar(4 * PF_STAGES + 8 + 2 * x + (j & 1)); }
+  QB_DEVICE uint32_t buffer_phase(int j) const { return (uint32_t)(j >> 1) & 1u; }
+  QB_DEVICE uint32_t o_last(int x) const { return bar(4 * PF_STAGES + 12 + x); }  // the last tile's P V
+  QB_DEVICE uint32_t q_full(int x) const { return bar(4 * PF_STAGES + 14 + x); }
+  QB_DEVICE uint32_t all_done(int i) const { return bar(4 * PF_STAGES + 16 + i); }
   QB_DEVICE uint32_t* tmem_slot() const { return reinterpret_cast<uint32_t*>(ptr + PF_META + 8 * PF_BARS); }
   QB_DEVICE volatile int* abort_flag() const { return reinterpret_cast<volatile int*>(tmem_slot() + 1); }
   QB_DEVICE float* row_fac() const { return reinterpret_cast<float*>(tmem_slot() + 2); }
@@ -257,64 +259,68 @@ QB_DEVICE void prefill_convert(const PrefillP& p, const PrefillSmem& sm, const P
   }
 }
 
-// ------------------------------------------------------------------ MMA issuer
-// The whole warp walks the loop and one elected lane issues, so that everything an MMA takes is computed
-// once for the warp, in uniform registers: with a single thread in the loop the issue of the 24 MMAs and 6
-// commits of a block took longer than their execution (2800 clocks a block against 1300).
-QB_DEVICE void prefill_mma(const PrefillP& p, const PrefillSmem& sm, const PrefillWork& w, uint32_t tmem) {
+// ------------------------------------------------------------------ MMA issuers
+// A warp for S and a warp for O of query tile x.  The whole warp walks the loop and one elected lane
+// issues, so that what an MMA takes is computed once for the warp, in uniform registers: a single thread
+// in the loop needs longer to issue the MMAs than the tensor pipe to execute them.
+QB_DEVICE void prefill_issue(const PrefillP& p, const PrefillSmem& sm, const PrefillWork& w, uint32_t tmem, int x,
+                             bool scores) {
   volatile int* ab = sm.abort_flag();
-  const int n = max(w.n[0], w.n[1]);
+  const int n = max(w.n[0], w.n[1]), mine = w.n[x];
   uint32_t pred;
   asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(pred));
   const bool one = pred != 0;
   auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, ab, p.err)) != 0; };
-  const uint64_t qd[2] = {sw128_kmajor_desc(sm.q(0)), sw128_kmajor_desc(sm.q(1))};
-  const uint64_t kd = sw128_kmajor_desc(sm.k(0)), vd = sw128_mn_desc(sm.v(0), PF_KV_HALF);
-  // S of key tile j for both query tiles.  Its buffer held P of j - 2.
-  auto scores = [&](int j) {
-    if (!wait(sm.k_full(j), sm.phase(j))) return false;
-    const uint64_t k = kd + (uint64_t)(j % PF_STAGES * (PF_KV_TILE >> 4));
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      if (j >= w.n[x]) continue;
-      if (j >= 2 && !wait(sm.pv_done(x), (uint32_t)j & 1u)) return false;
+  const uint32_t s_at = tmem + PF_COL_S + x * 128, o_at = tmem + PF_COL_O + x * 128;
+  bool ok = true;
+  if (scores) {
+    const uint64_t q = sw128_kmajor_desc(sm.q(x)), k0 = sw128_kmajor_desc(sm.k(0));
+    ok = mine == 0 || wait(sm.q_full(x), 0);
+    for (int j = 0; ok && j < n; ++j) {
+      if (!(ok = wait(sm.k_full(j), sm.phase(j)))) break;
+      if (j >= mine) {  // past this query tile's last key: the stage is free as far as it goes
+        if (one) mbar_arrive(sm.k_empty(j));
+        continue;
+      }
+      // the buffer held P of j - 2
+      if (j >= 2 && !(ok = wait(sm.pv_done(x, j), sm.buffer_phase(j - 2)))) break;
       tc_fence_after();
       if (one) {
+        const uint64_t k = k0 + (uint64_t)(j % PF_STAGES * (PF_KV_TILE >> 4));
 #pragma unroll
         for (int i = 0; i < 8; ++i)  // 128 elements in steps of 16
-          umma_bf16(tmem + PF_COL_S + x * 128 + (j & 1) * 64, qd[x] + (((i >> 2) * PF_Q_HALF + (i & 3) * 32) >> 4),
+          umma_bf16(s_at + (j & 1) * 64, q + (((i >> 2) * PF_Q_HALF + (i & 3) * 32) >> 4),
                     k + (((i >> 2) * PF_KV_HALF + (i & 3) * 32) >> 4), PF_IDESC_S, i > 0);
         umma_commit(sm.s_full(x, j));
+        umma_commit(sm.k_empty(j));
       }
     }
-    if (one) umma_commit(sm.k_empty(j));
-    return true;
-  };
-  bool ok = wait(sm.q_full(0), 0) && (w.n[1] == 0 || wait(sm.q_full(1), 0));
-  ok = ok && scores(0);
-  for (int j = 0; ok && j < n; ++j) {
-    if (j + 1 < n && !(ok = scores(j + 1))) break;
-    if (!(ok = wait(sm.v_full(j), sm.phase(j)))) break;
-    const uint64_t v = vd + (uint64_t)(j % PF_STAGES * (PF_KV_TILE >> 4));
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      if (!ok || j >= w.n[x]) continue;
-      if (!(ok = wait(sm.p_ready(x, j), (uint32_t)(j >> 1) & 1u))) continue;
+  } else {
+    const uint64_t v0 = sw128_mn_desc(sm.v(0), PF_KV_HALF);
+    for (int j = 0; ok && j < n; ++j) {
+      if (!(ok = wait(sm.v_full(j), sm.phase(j)))) break;
+      if (j >= mine) {
+        if (one) mbar_arrive(sm.v_empty(j));
+        continue;
+      }
+      if (!(ok = wait(sm.p_ready(x, j), sm.buffer_phase(j)))) break;
       tc_fence_after();
       if (one) {
+        const uint64_t v = v0 + (uint64_t)(j % PF_STAGES * (PF_KV_TILE >> 4));
 #pragma unroll
         for (int i = 0; i < 4; ++i)  // 64 keys in steps of 16: P columns 8 i, V rows 16 i
-          umma_bf16_ts(tmem + PF_COL_O + x * 128, tmem + PF_COL_S + x * 128 + (j & 1) * 64 + 8 * i,
-                       v + ((i * 16 * 128) >> 4), PF_IDESC_O, (j > 0 || i > 0) ? 1u : 0u);
-        umma_commit(j + 1 < w.n[x] ? sm.pv_done(x) : sm.o_last(x));
+          umma_bf16_ts(o_at, s_at + (j & 1) * 64 + 8 * i, v + ((i * 16 * 128) >> 4), PF_IDESC_O, (j > 0 || i > 0) ? 1u : 0u);
+        umma_commit(sm.pv_done(x, j));
+        if (j + 1 == mine) umma_commit(sm.o_last(x));
+        umma_commit(sm.v_empty(j));
       }
     }
-    if (ok && one) umma_commit(sm.v_empty(j));
   }
   // no MMA may still be reading shared memory or writing TMEM when the CTA leaves
   if (one) {
-    umma_commit(sm.all_done());
-    mbar_drain(sm.all_done(), 0);
+    const uint32_t done = sm.all_done(x + (scores ? 0 : 2));
+    umma_commit(done);
+    mbar_drain(done, 0);
   }
 }
 
@@ -369,7 +375,7 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
   float ref = -INFINITY, l = 0.f, vref = 0.f;
   for (int j = 0; ok && j < n; ++j) {
     // tcgen05 loads and stores are warp-collective: every decision that leads to them is warp-uniform
-    if (!__all_sync(0xffffffffu, mbar_wait(sm.s_full(x, j), (uint32_t)(j >> 1) & 1u, ab, p.err))) {
+    if (!__all_sync(0xffffffffu, mbar_wait(sm.s_full(x, j), sm.buffer_phase(j), ab, p.err))) {
       ok = false;
       break;
     }
@@ -409,7 +415,7 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
         a *= alpha;
       }
       if (j > 0) {  // O holds the tiles before: wait for the last of them, weigh them anew
-        if (!__all_sync(0xffffffffu, mbar_wait(sm.pv_done(x), (uint32_t)(j - 1) & 1u, ab, p.err))) {
+        if (!__all_sync(0xffffffffu, mbar_wait(sm.pv_done(x, j - 1), sm.buffer_phase(j - 1), ab, p.err))) {
           ok = false;
           break;
         }
@@ -539,20 +545,20 @@ prefill_fp8_kernel(PrefillP p) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < PF_STAGES; ++i) {
       mbar_init(sm.k_full(i), 128);
-      mbar_init(sm.k_empty(i), 1);
+      mbar_init(sm.k_empty(i), 2);
       mbar_init(sm.v_full(i), 128);
-      mbar_init(sm.v_empty(i), 1);
+      mbar_init(sm.v_empty(i), 2);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(sm.q_full(i), 128);
-      mbar_init(sm.s_full(i, 0), 1);
-      mbar_init(sm.s_full(i, 1), 1);
-      mbar_init(sm.p_ready(i, 0), 128);
-      mbar_init(sm.p_ready(i, 1), 128);
-      mbar_init(sm.pv_done(i), 1);
       mbar_init(sm.o_last(i), 1);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(sm.s_full(i, k), 1);
+        mbar_init(sm.p_ready(i, k), 128);
+        mbar_init(sm.pv_done(i, k), 1);
+        mbar_init(sm.all_done(2 * i + k), 1);
+      }
     }
-    mbar_init(sm.all_done(), 1);
     *sm.abort_flag() = 0;
     // tiles that some row sees in part are the last five at most: their slots' NaN keys are written once
     for (int j = 0; j < PF_SLOTS; ++j) sm.nan_keys(j)[0] = sm.nan_keys(j)[1] = 0;
@@ -573,7 +579,7 @@ prefill_fp8_kernel(PrefillP p) {
   } else if (warp < 12) {
     prefill_convert(p, sm, w);
   } else {
-    prefill_mma(p, sm, w, tmem);
+    prefill_issue(p, sm, w, tmem, warp & 1, warp < 14);
   }
   __syncwarp();
   tc_fence_before();
