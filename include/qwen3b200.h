@@ -232,9 +232,10 @@ int qb_paged_decode_attn_fp8(const void* q, int64_t q_stride, const void* k_cach
                              int* err, qb_stream_t stream);
 /* The grouped form; arguments as qb_paged_decode_attn_grouped, with the shared and the own keys split
  * apart: shared_tokens * shared_splits >= every shared_len, own_tokens * own_splits >= every
- * seqlens[b] + seqlen_add - kv_start[b].  Sequences in no group are left out of `out`; kv_start is a
- * multiple of 64.  workspace: qb_paged_decode_fp8_workspace_bytes(batch, hq, shared_splits +
- * own_splits). */
+ * seqlens[b] + seqlen_add - kv_start[b].  Sequences in no group get zeros; kv_start is a multiple of 64;
+ * entries of group_members that name no sequence set QB_DEVERR_SHAPE.  A sequence is in one group at
+ * most.  workspace: qb_paged_decode_grouped_fp8_workspace_bytes(batch, hq, shared_splits + own_splits),
+ * any contents. */
 int qb_paged_decode_attn_grouped_fp8(const void* q, int64_t q_stride, const void* k_cache,
                                      const void* v_cache, const float* k_scale, const float* v_scale,
                                      int64_t num_blocks, int page_size, const int32_t* block_tables,
@@ -245,6 +246,7 @@ int qb_paged_decode_attn_grouped_fp8(const void* q, int64_t q_stride, const void
                                      int shared_splits, int own_tokens, int own_splits,
                                      float* workspace, void* out, int* err, qb_stream_t stream);
 size_t qb_paged_decode_fp8_workspace_bytes(int batch, int hq, int n_slots);
+size_t qb_paged_decode_grouped_fp8_workspace_bytes(int batch, int hq, int n_slots);
 /* Causal attention of the query rows cu_seqlens_q over the first cu_seqlens_k keys of each sequence in
  * that cache; arguments as the paged form of qb_attn_varlen_fwd.  q and out rows q_stride / o_stride
  * elements apart (multiples of 8).  hq / hkv <= 16.  Rows in no sequence are left as they were.

@@ -61,8 +61,11 @@ struct DecodeP {
   const int32_t* kv_start;
   int n_groups, shared_tokens, shared_splits;
   int chunk, n_chunks;        // members per shared CTA, shared CTAs per group
+  int group_step;             // shared CTA r takes groups r, r + group_step, ...
   unsigned n_shared;          // shared CTAs; the own CTAs follow
+  int* entry_of;              // [batch] in the workspace: where a sequence stands in `members`
 };
+constexpr int DC_GROUPS = 8;  // groups of a shared CTA at most
 
 // What a CTA works on: `rows` query rows over keys [begin, end) of table row `table`.
 struct Work {
@@ -104,10 +107,10 @@ QB_DEVICE int row_sequence(const DecodeP& p, const int32_t* members, int b, int 
 }
 
 // One CTA: the work `w` of kv head `kvh`; NT tiles of eight query rows.  `members`: the chunk's member
-// list (shared work), `b`: the sequence (own work).
+// list (shared work), `b`: the sequence (own work).  `u0` tiles and `item` works came before in this CTA.
 template <int NT, bool SHARED>
 QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtensorMap& tv, uint8_t* smem, uint32_t base,
-                           const Work& w, int kvh, const int32_t* members, int b) {
+                           const Work& w, int kvh, const int32_t* members, int b, int u0, int item) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int n = (w.end - w.begin + KV8_BLOCK - 1) / KV8_BLOCK;
   const int group = p.hq / p.hkv;
@@ -144,7 +147,7 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
     }
     __syncwarp();
     auto issue = [&](int i) {
-      const int s = i % DC_STAGES, page = page_of[i];
+      const int s = (u0 + i) % DC_STAGES, page = page_of[i];
       if (page < 0) {
         mbar_arrive(full(s));
         return;
@@ -156,8 +159,14 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
       tma_load_2d(at + KV8_TILE, &tv, 0, row, full(s));
     };
     int issued = 0;
-    if (lane == 0)
-      for (; issued < min(n, DC_STAGES); ++issued) issue(issued);
+    auto issue_to = [&](int last) {
+      for (; issued < last; ++issued) {
+        const int u = u0 + issued;
+        if (u >= DC_STAGES && !mbar_wait(empty(u % DC_STAGES), (uint32_t)(u / DC_STAGES - 1) & 1u, abort_flag, p.err)) break;
+        issue(issued);
+      }
+    };
+    if (lane == 0) issue_to(min(n, DC_STAGES));
 #pragma unroll
     for (int j = 0; j < DC_MAX_TILES / 32; ++j)
       if (lane + 32 * j < n) {
@@ -167,13 +176,10 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
     __syncwarp();
     if (lane == 0) {
       mbar_arrive(ready);
-      for (; issued < n; ++issued) {
-        if (!mbar_wait(empty(issued % DC_STAGES), (uint32_t)(issued / DC_STAGES - 1) & 1u, abort_flag, p.err)) break;
-        issue(issued);
-      }
+      issue_to(n);
       // never leave with a copy in flight into this CTA's shared memory
       for (int i = max(0, issued - DC_STAGES); i < issued; ++i)
-        mbar_drain(full(i % DC_STAGES), (uint32_t)(i / DC_STAGES) & 1u);
+        mbar_drain(full((u0 + i) % DC_STAGES), (uint32_t)((u0 + i) / DC_STAGES) & 1u);
     }
     __syncwarp();
     __syncthreads();
@@ -230,10 +236,10 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
   }
-  bool ok = __all_sync(0xffffffffu, mbar_wait(ready, 0, abort_flag, p.err));
+  bool ok = __all_sync(0xffffffffu, mbar_wait(ready, (uint32_t)item & 1u, abort_flag, p.err));
   for (int i = 0; ok && i < n; ++i) {
-    const int s = i % DC_STAGES;
-    if (!__all_sync(0xffffffffu, mbar_wait(full(s), (uint32_t)(i / DC_STAGES) & 1u, abort_flag, p.err))) {
+    const int s = (u0 + i) % DC_STAGES;
+    if (!__all_sync(0xffffffffu, mbar_wait(full(s), (uint32_t)((u0 + i) / DC_STAGES) & 1u, abort_flag, p.err))) {
       ok = false;
       break;
     }
@@ -439,32 +445,44 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     i /= p.shared_splits;
     const int kvh = i % p.hkv;
     i /= p.hkv;
-    const int c = i % p.n_chunks, grp = i / p.n_chunks;
-    const int32_t* members = p.members + grp * 8 + c * p.chunk;
-    const int donor = p.members[grp * 8], keys = p.shared_len[grp];
-    Work w;
-    w.rows = min(p.chunk, 8 - c * p.chunk) * group;
-    w.table = donor;
-    w.begin = split * p.shared_tokens;
-    w.end = min(keys, w.begin + p.shared_tokens);
-    w.slot = split;
-    bool any = false;
-    for (int m = 0; m < 8 - c * p.chunk && m < p.chunk; ++m) any |= members[m] >= 0 && members[m] < p.batch;
-    if (split == p.shared_splits - 1 && w.end < keys && threadIdx.x == 0) qb_set_err(p.err, QB_DEVERR_SHAPE);
-    if (!any || w.begin >= w.end || donor < 0 || donor >= p.batch) return;
-    decode_work<NTS == 0 ? 1 : NTS, true>(p, tk, tv, smem, base, w, kvh, members, 0);
+    const int c = i % p.n_chunks, first = i / p.n_chunks;
+    int u0 = 0, item = 0;
+    for (int grp = first; grp < p.n_groups; grp += p.group_step) {
+      const int32_t* members = p.members + grp * 8 + c * p.chunk;
+      const int donor = p.members[grp * 8], keys = p.shared_len[grp];
+      Work w;
+      const int n_members = min(p.chunk, 8 - c * p.chunk);
+      w.rows = n_members * group;
+      w.table = donor;
+      w.begin = split * p.shared_tokens;
+      w.end = min(keys, w.begin + p.shared_tokens);
+      w.slot = split;
+      bool any = false;
+      for (int m = 0; m < n_members; ++m) {
+        const int b = members[m];
+        any |= b >= 0 && b < p.batch;
+        if (kvh == 0 && split == 0 && threadIdx.x == 0) {
+          if (b >= p.batch) qb_set_err(p.err, QB_DEVERR_SHAPE);
+          else if (b >= 0) p.entry_of[b] = grp * 8 + c * p.chunk + m;
+        }
+      }
+      if (split == p.shared_splits - 1 && w.end < keys && threadIdx.x == 0) qb_set_err(p.err, QB_DEVERR_SHAPE);
+      if (!any || w.begin >= w.end || donor < 0 || donor >= p.batch) continue;
+      if (item > 0) {  // the stages, which the join wrote to, go back to the copies
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
+      }
+      decode_work<NTS == 0 ? 1 : NTS, true>(p, tk, tv, smem, base, w, kvh, members, 0, u0, item);
+      u0 += (w.end - w.begin + KV8_BLOCK - 1) / KV8_BLOCK;
+      ++item;
+    }
     return;
   }
   i -= p.n_shared;
   const int split = i % p.own_splits;
   i /= p.own_splits;
   const int kvh = i % p.hkv;
-  int b = i / p.hkv;
-  if (NTS > 0) b = p.members[b];
-  if (b < 0 || b >= p.batch) {
-    if (b >= p.batch && threadIdx.x == 0) qb_set_err(p.err, QB_DEVERR_SHAPE);
-    return;
-  }
+  const int b = i / p.hkv;
   const int len = p.seqlens[b] + p.seqlen_add, first = own_first(p, b);
   const int64_t begin = (int64_t)first + (int64_t)split * p.own_tokens;
   if ((first < 0 || (split == p.own_splits - 1 && begin + p.own_tokens < len)) && threadIdx.x == 0)
@@ -482,7 +500,7 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         reinterpret_cast<uint2*>(p.out + ((int64_t)b * p.hq + kvh * group) * KV8_D)[k] = make_uint2(0, 0);
     return;
   }
-  decode_work<NTO, false>(p, tk, tv, smem, base, w, kvh, nullptr, b);
+  decode_work<NTO, false>(p, tk, tv, smem, base, w, kvh, nullptr, b, 0, 0);
 }
 
 // Joins the splits of a (sequence, head): a warp each, weights 2^(lse - largest lse).  Only the splits
@@ -494,17 +512,21 @@ decode_fp8_join_kernel(DecodeP p) {
   const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const int h = (int)(item % p.hq);
-  const int64_t entry = item / p.hq;
-  if (entry >= (p.members ? p.n_groups * 8 : p.batch)) return;
-  int b = (int)entry, n_shared = 0;
+  const int b = (int)(item / p.hq);
+  if (b >= p.batch) return;
+  int n_shared = 0;
+  bool member = true;
   if (p.members) {
-    b = p.members[entry];
-    const int donor = p.members[entry / 8 * 8], keys = p.shared_len[entry / 8];
-    if (b < 0 || b >= p.batch) return;
-    if (donor >= 0 && donor < p.batch && keys > 0)
-      n_shared = min(p.shared_splits, (keys + p.shared_tokens - 1) / p.shared_tokens);
+    // entry_of holds whatever was there for a sequence in no group: it counts where `members` agrees
+    const int e = p.entry_of[b];
+    member = e >= 0 && e < p.n_groups * 8 && p.members[e] == b;
+    if (member) {
+      const int donor = p.members[e / 8 * 8], keys = p.shared_len[e / 8];
+      if (donor >= 0 && donor < p.batch && keys > 0)
+        n_shared = min(p.shared_splits, (keys + p.shared_tokens - 1) / p.shared_tokens);
+    }
   }
-  const int own0 = p.members ? p.shared_splits : 0, n = n_shared + own_live(p, b);
+  const int own0 = p.members ? p.shared_splits : 0, n = member ? n_shared + own_live(p, b) : 0;
   const float* ws = p.ws + ((int64_t)b * p.hq + h) * p.n_slots * DC_WS_ROW;
   auto slot = [&](int s) { return ws + (int64_t)(s < n_shared ? s : own0 + s - n_shared) * DC_WS_ROW; };
   float m = -INFINITY;
@@ -528,7 +550,7 @@ decode_fp8_join_kernel(DecodeP p) {
 }
 
 template <int NTS, int NTO>
-int launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeP& p, int64_t entries, cudaStream_t st) {
+int launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeP& p, cudaStream_t st) {
   static bool attr = false;
   if (!attr) {
     if (cudaFuncSetAttribute(decode_fp8_kernel<NTS, NTO>, cudaFuncAttributeMaxDynamicSharedMemorySize, DC_SMEM) !=
@@ -536,13 +558,16 @@ int launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeP& p
       return qb_launch_status();
     attr = true;
   }
-  const int64_t ctas = p.n_shared + entries * p.hkv * p.own_splits;
-  if (ctas > INT32_MAX || entries * p.hq > INT32_MAX) return QB_ERR_INVALID;
+  const int64_t ctas = p.n_shared + (int64_t)p.batch * p.hkv * p.own_splits, rows = (int64_t)p.batch * p.hq;
+  if (ctas > INT32_MAX || rows > INT32_MAX) return QB_ERR_INVALID;
   const int rc = qb_launch_ex(decode_fp8_kernel<NTS, NTO>, dim3((unsigned)ctas), dim3(DC_THREADS), DC_SMEM, st, 1, true, tk,
                               tv, p);
   if (rc != QB_OK || p.n_slots == 1) return rc;
-  return qb_launch_ex(decode_fp8_join_kernel, dim3((unsigned)((entries * p.hq + 3) / 4)), dim3(128), 0, st, 1, true, p);
+  return qb_launch_ex(decode_fp8_join_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, 1, true, p);
 }
+
+// floats of the splits' partial outputs
+size_t decode_partials(int batch, int hq, int n_slots) { return (size_t)batch * hq * n_slots * DC_WS_ROW; }
 
 bool split_ok(int tokens, int splits) {
   return tokens > 0 && tokens % KV8_BLOCK == 0 && tokens <= DC_MAX_TILES * KV8_BLOCK && splits >= 1 &&
@@ -573,7 +598,7 @@ extern "C" int qb_paged_decode_attn_fp8(const void* q, int64_t q_stride, const v
   p.own_tokens = split_tokens; p.own_splits = max_splits; p.n_slots = max_splits;
   p.ws = workspace; p.out = (bf16*)out; p.err = err;
   const cudaStream_t st = (cudaStream_t)stream;
-  return hq / hkv <= 8 ? launch_decode<0, 1>(tk, tv, p, batch, st) : launch_decode<0, 2>(tk, tv, p, batch, st);
+  return hq / hkv <= 8 ? launch_decode<0, 1>(tk, tv, p, st) : launch_decode<0, 2>(tk, tv, p, st);
 }
 
 extern "C" int qb_paged_decode_attn_grouped_fp8(
@@ -604,16 +629,23 @@ extern "C" int qb_paged_decode_attn_grouped_fp8(
   const int group = hq / hkv, row_tiles = group == 1 ? 1 : 2;
   p.chunk = min(8, row_tiles * 8 / group);
   p.n_chunks = (8 + p.chunk - 1) / p.chunk;
-  const int64_t shared = (int64_t)n_groups * p.n_chunks * hkv * shared_splits;
+  // A caller's table of groups may have many empty entries behind its live ones (one captured for any
+  // grouping): a shared CTA takes every group_step-th group, so the empty ones cost no CTAs of their own.
+  p.group_step = (n_groups + DC_GROUPS - 1) / DC_GROUPS;
+  p.entry_of = reinterpret_cast<int*>(workspace + decode_partials(batch, hq, p.n_slots));
+  const int64_t shared = (int64_t)p.group_step * p.n_chunks * hkv * shared_splits;
   QB_CHECK_ARG(shared <= INT32_MAX);
   p.n_shared = (unsigned)shared;
   const cudaStream_t st = (cudaStream_t)stream;
-  const int64_t entries = (int64_t)n_groups * 8;
-  if (group == 1) return launch_decode<1, 1>(tk, tv, p, entries, st);
-  if (group <= 8) return launch_decode<2, 1>(tk, tv, p, entries, st);
-  return launch_decode<2, 2>(tk, tv, p, entries, st);
+  if (group == 1) return launch_decode<1, 1>(tk, tv, p, st);
+  if (group <= 8) return launch_decode<2, 1>(tk, tv, p, st);
+  return launch_decode<2, 2>(tk, tv, p, st);
 }
 
 extern "C" size_t qb_paged_decode_fp8_workspace_bytes(int batch, int hq, int n_slots) {
-  return n_slots <= 1 ? 0 : (size_t)batch * hq * n_slots * DC_WS_ROW * 4;
+  return n_slots <= 1 ? 0 : decode_partials(batch, hq, n_slots) * 4;
+}
+
+extern "C" size_t qb_paged_decode_grouped_fp8_workspace_bytes(int batch, int hq, int n_slots) {
+  return decode_partials(batch, hq, n_slots) * 4 + ((size_t)batch * 4 + 15) / 16 * 16;
 }

@@ -635,18 +635,20 @@ def grouped_decode_plan_fp8(batch, n_groups, hq, hkv, max_shared, max_own, sm_co
     return shared, shared_splits, own, own_splits
 
 
-def workspace_fp8(batch, hq, n_slots, device):
-    """Split-K partials of the 8-bit decode attentions; None where there is one split."""
-    nbytes = lib().qb_paged_decode_fp8_workspace_bytes(batch, hq, n_slots)
+def workspace_fp8(batch, hq, n_slots, device, grouped=False):
+    """Workspace of the 8-bit decode attentions (split-K partials); None where none is needed."""
+    f = lib().qb_paged_decode_grouped_fp8_workspace_bytes if grouped else lib().qb_paged_decode_fp8_workspace_bytes
+    nbytes = f(batch, hq, n_slots)
     return torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
 
 
-def _fp8_workspace(what, workspace, batch, hq, n_slots, device):
+def _fp8_workspace(what, workspace, batch, hq, n_slots, device, grouped=False):
     if workspace is None:
-        return workspace_fp8(batch, hq, n_slots, device)
-    if workspace.numel() * workspace.element_size() < lib().qb_paged_decode_fp8_workspace_bytes(batch, hq, n_slots) \
-            or workspace.data_ptr() % 16 or not workspace.is_cuda:
-        raise NativeError(f"{what}: the workspace is too small for {n_slots} splits")
+        return workspace_fp8(batch, hq, n_slots, device, grouped)
+    f = lib().qb_paged_decode_grouped_fp8_workspace_bytes if grouped else lib().qb_paged_decode_fp8_workspace_bytes
+    if workspace.numel() * workspace.element_size() < f(batch, hq, n_slots) or workspace.data_ptr() % 16 \
+            or not workspace.is_contiguous():
+        raise NativeError(f"{what}: the workspace is too small for {n_slots} splits, or not aligned")
     return workspace
 
 
@@ -678,7 +680,7 @@ def paged_decode_attention_grouped_fp8(q, k_cache, v_cache, k_scale, v_scale, bl
                                        group_members, shared_len, kv_start, plan, workspace=None, seqlen_add=1,
                                        out=None):
     """:func:`paged_decode_attention_grouped` over the 8-bit cache; ``plan`` from
-    :func:`grouped_decode_plan_fp8`.  Sequences in no group are left out of ``out``."""
+    :func:`grouped_decode_plan_fp8`.  Sequences in no group get zeros."""
     what = "paged_decode_attention_grouped_fp8"
     num_blocks, hkv = _check_kv_fp8(what, k_cache, v_cache, k_scale, v_scale, q, block_tables, seqlens, group_members,
                                     shared_len, kv_start, workspace)
@@ -692,7 +694,7 @@ def paged_decode_attention_grouped_fp8(q, k_cache, v_cache, k_scale, v_scale, bl
                           "[groups, 8] and shared_len [groups]")
     shared_tokens, shared_splits, own_tokens, own_splits = plan
     out = _fp8_out(what, out, q)
-    ws = _fp8_workspace(what, workspace, B, hq, shared_splits + own_splits, q.device)
+    ws = _fp8_workspace(what, workspace, B, hq, shared_splits + own_splits, q.device, grouped=True)
     check(lib().qb_paged_decode_attn_grouped_fp8(
         _p(q), q.stride(0), _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale), num_blocks, KV_FP8_PAGE,
         _p(block_tables), block_tables.stride(0), block_tables.shape[1], _p(seqlens), seqlen_add, B, hq, hkv, 128, scale,

@@ -275,6 +275,25 @@ def grouped_inputs(g, hq, hkv, groups, dev):
     return q, k, v, ks, vs, parts, dev_args, grp
 
 
+def test_grouped_table_with_empty_entries(cuda):
+    """A table captured for any grouping: live groups anywhere in it, several to one CTA."""
+    g = gen(50)
+    q, k, v, ks, vs, parts, args, grp = grouped_inputs(g, 16, 8, [(300, [5, 70, 64]), (600, [1, 2]), (64, [200] * 8), (90, [3])], cuda)
+    n = q.shape[0]
+    plan = ops.grouped_decode_plan_fp8(n, 4, 16, 8, 600, 200)
+    want = ops.paged_decode_attention_grouped_fp8(*args, 0.1, *grp, plan)
+    for at in ([0, 1, 2, 3], [0, 6, 12, 18], [5, 17, 18, 40], [7, 0, 39, 20]):
+        members = torch.full((41, 8), -1, dtype=torch.int32, device=cuda)
+        shared = torch.zeros(41, dtype=torch.int32, device=cuda)
+        for i, slot in enumerate(at):
+            members[slot], shared[slot] = grp[0][i], grp[1][i]
+        out = ops.paged_decode_attention_grouped_fp8(*args, 0.1, members, shared, grp[2], (64, 24, 128, 8))
+        check = ops.paged_decode_attention_grouped_fp8(*args, 0.1, *grp, (64, 24, 128, 8))
+        assert torch.equal(out, check)
+        assert torch.allclose(out.float(), want.float(), rtol=2.0 ** -6, atol=1e-2)
+    ops.check_device_errors()
+
+
 @pytest.mark.parametrize("hq,hkv,groups", GROUPED)
 @pytest.mark.parametrize("plan", [None, (64, 24, 128, 8)])
 def test_grouped(cuda, hq, hkv, groups, plan):
@@ -297,7 +316,7 @@ def test_grouped(cuda, hq, hkv, groups, plan):
 
 def test_grouped_equals_plain_decode_where_nothing_is_skipped(cuda):
     """Prompts of whole pages: the shared and the unshared kernels attend the same keys; a sequence in no
-    group keeps its output row, a member id outside the batch is reported."""
+    group gets zeros whatever the workspace holds, a member id outside the batch is reported."""
     g = gen(21)
     q, k, v, ks, vs, parts, args, grp = grouped_inputs(g, 16, 8, [(256, [5, 70]), (512, [64])], cuda)
     plan = ops.grouped_decode_plan_fp8(3, 2, 16, 8, 512, 70)
@@ -308,9 +327,12 @@ def test_grouped_equals_plain_decode_where_nothing_is_skipped(cuda):
     lone = int(members[0, 1])
     members[0, 1] = -1
     out = torch.full_like(a, 3.0)
-    ops.paged_decode_attention_grouped_fp8(*args, 0.1, members, *grp[1:], plan, out=out)
     keep = [i for i in range(3) if i != lone]
-    assert torch.equal(out[keep], a[keep]) and bool((out[lone] == 3.0).all())
+    ws = ops.workspace_fp8(3, 16, plan[1] + plan[3], cuda, grouped=True)
+    for fill in (0, -1, 1, 5, 7 << 28):
+        ws.view(torch.int32).fill_(fill)
+        ops.paged_decode_attention_grouped_fp8(*args, 0.1, members, *grp[1:], plan, out=out, workspace=ws)
+        assert torch.equal(out[keep], a[keep]) and not bool(out[lone].any())
     ops.check_device_errors()
     members[0, 1] = 3
     ops.paged_decode_attention_grouped_fp8(*args, 0.1, members, *grp[1:], plan, out=out)
