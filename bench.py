@@ -90,6 +90,8 @@ def parse():
                     help="config 2: the grouped rollout alone (generated tokens/s, rollout roofline, CPU baseline)")
     ap.add_argument("--no-inner-profile", action="store_true",
                     help="skip the extra untimed step under CUPTI that measures the dominant kernel inside the step")
+    ap.add_argument("--kv-dtype", default="bf16", choices=["bf16", "fp8"],
+                    help="paged K/V cache of the rollout: bf16 (the default workload) or e4m3 codes with block scales")
     ap.add_argument("--no-share-prefix", action="store_true",
                     help="roll out with the reference's scheduler (every completion prefilled and stored)")
     ap.add_argument("--no-pdl", action="store_true",
@@ -278,7 +280,12 @@ LM_HEAD_PARAMS = VOCAB * H
 KV_BYTES_PER_KEY_LAYER = 2 * HKV * D * 2                               # K and V, bf16
 
 
-def step_roofline(prompt_lens, group, new, layers, step_s, peaks):
+def kv_bytes_per_key_layer(kv_dtype):
+    """K + V of one key in one layer: bf16, or e4m3 codes and their share of the block scales."""
+    return KV_BYTES_PER_KEY_LAYER if kv_dtype == "bf16" else KV_BYTES_PER_KEY_LAYER // (2 * D) * (D + 4 / 64)
+
+
+def step_roofline(prompt_lens, group, new, layers, step_s, peaks, kv_dtype="bf16"):
     """Roofline time of one GRPO step of this rank's workload, phase by phase: each phase costs
     max(FLOP / tensor peak, bytes / HBM peak) at the sustained measured peaks, summed; the
     fraction is that sum over the measured step time.  FLOPs are 2 per weight per token for
@@ -298,7 +305,7 @@ def step_roofline(prompt_lens, group, new, layers, step_s, peaks):
         keys_read = sum(prompt_lens) + B * (s + 1)  # shared prompts once + each completion's own keys
         ctx_total = sum(L + s + 1 for L in prompt_lens) * group
         flop = B * (lin + 2 * LM_HEAD_PARAMS) + attn(ctx_total)
-        byts = weights + keys_read * KV_BYTES_PER_KEY_LAYER * layers
+        byts = weights + keys_read * kv_bytes_per_key_layer(kv_dtype) * layers
         t_roll += max(flop / tf, byts / bw)
     # log-prob recompute (frozen reference) and the policy's forward + backward, packed sequences
     seqs = [L + new for L in prompt_lens for _ in range(group)]
@@ -415,6 +422,7 @@ def run_ours(args):
         dist.init_process_group("nccl", timeout=datetime.timedelta(seconds=600), device_id=dev)
     cfg = Qwen3Config(num_hidden_layers=args.layers)
     policy = build_model(cfg, device=dev, seed=0)
+    policy.kv_cache_dtype = args.kv_dtype
     ref = G.make_reference_copy(policy)
     max_ctx = args.prompt_max + args.new_tokens
     # pages for every sequence of the step at once (64*8 seqs x 4 pages) plus slack; a larger
@@ -496,9 +504,10 @@ def run_ours(args):
     roof_s = 0.0
     for j in range(args.steps):
         lens = [p.shape[1] for p in make_prompts(args, rank, 100 + j)]
-        roof_s += step_roofline(lens, args.group, args.new_tokens, args.layers, 1.0, peaks)["total_s"]
+        roof_s += step_roofline(lens, args.group, args.new_tokens, args.layers, 1.0, peaks,
+                                args.kv_dtype)["total_s"]
     whole_step = step_roofline([p.shape[1] for p in make_prompts(args, rank, 100)], args.group, args.new_tokens,
-                               args.layers, ms / 1000.0 / args.steps, peaks)
+                               args.layers, ms / 1000.0 / args.steps, peaks, args.kv_dtype)
     whole_step["frac"] = roof_s / (ms / 1000.0)
     whole_step["total_s_all_timed_steps"] = roof_s
     e2e = None
@@ -568,7 +577,7 @@ def run_ours(args):
                 "data": "synthetic",
                 "config": {"workload": WORKLOAD if args.workload == "cfg4" else WORKLOAD5,
                            "prompts_per_gpu": len(make_prompts(args, rank, 0)), "group": args.group,
-                           "kv_pages": policy._num_blocks,
+                           "kv_pages": policy._num_blocks, "kv_dtype": args.kv_dtype,
                            "new_tokens": args.new_tokens, "prompt_len": [args.prompt_min, args.prompt_max],
                            "layers": args.layers, "parallelism": f"dp{world}", "beta_kl": 0.04,
                            "rollout": "reference scheduler" if args.no_share_prefix else
@@ -601,6 +610,7 @@ def run_rollout_only(args):
     torch.cuda.set_device(dev)
     cfg = Qwen3Config(num_hidden_layers=args.layers)
     model = build_model(cfg, device=dev, seed=0)
+    model.kv_cache_dtype = args.kv_dtype
     max_ctx = args.prompt_max + args.new_tokens
     model._num_blocks = args.prompts * args.group * math.ceil(max_ctx / 256) + 64
     model.max_model_len = max_ctx
@@ -633,7 +643,7 @@ def run_rollout_only(args):
     ms = a.elapsed_time(b)
     ops.check_device_errors()
     roof = sum(step_roofline([p.shape[1] for p in ps], args.group, args.new_tokens, args.layers, 1.0,
-                             peaks)["rollout_s"] for ps in host)
+                             peaks, args.kv_dtype)["rollout_s"] for ps in host)
     cpu = None
     if not args.no_cpu_baseline:
         v, sample, th = cpu_rollout_sample()
@@ -644,7 +654,7 @@ def run_rollout_only(args):
                       "config": {"workload": "config 2: grouped rollout, 64 prompts x G=8, prompt U[64,512], "
                                              "512 new tokens, temperature 1, paged KV 256",
                                  "prompts": args.prompts, "group": args.group, "new_tokens": args.new_tokens,
-                                 "layers": args.layers},
+                                 "layers": args.layers, "kv_dtype": args.kv_dtype},
                       "all_tokens_per_s": all_tokens / (ms / 1000),
                       "roofline": {"bound": "hbm (decode) + tensor (prefill)", "roofline_s": roof,
                                    "measured_s": ms / 1000, "frac": roof / (ms / 1000),

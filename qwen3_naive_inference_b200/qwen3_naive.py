@@ -289,6 +289,8 @@ class Qwen3Attention(nn.Module):
         self.k_norm = RMSNorm(self.head_dim, eps=config.rms_norm_eps)
         self.k_cache = None
         self.v_cache = None
+        self.k_scale = None  # scales of an 8-bit cache (ops.kv_cache_fp8); None: a bf16 cache
+        self.v_scale = None
         self.rotary_emb = get_rope(self.head_dim, config.max_position_embeddings, config.rope_theta)
         self.rope_grad = True  # False reproduces the reference's gradient-blocking RoPE
 
@@ -322,25 +324,50 @@ class Qwen3Attention(nn.Module):
         ``decode_tail`` = (n_prefill_rows, context_lens, block_tables, decode_plan): the rows from
         n_prefill_rows on are single decode tokens whose attention runs on the decode kernel of
         ``decode_plan`` (cu_seqlens and ``block_tables`` then describe the prefill rows only)."""
-        # qkv projection with QK-norm, RoPE and the K/V store in the GEMM's epilogue
-        q = ops.qkv_norm_rope_store(x, self.qkv_proj.weight, positions, self._cos_sin(x.device), self.q_norm.weight,
-                                    self.k_norm.weight, self.eps, self.num_heads, self.num_kv_heads, self.k_cache,
-                                    self.v_cache, block_mapping)
+        q = self._project_store(x, positions, block_mapping)
         if block_tables is None:
             raise ValueError("the paged prefill kernel reads K/V through block_tables")
         if decode_tail is None:
-            o = ops.attention_paged_prefill(q, self.k_cache, self.v_cache, cu_seqlens_q, cu_seqlens_k,
-                                            max_seqlen_q, block_tables, self.scale, tiles=tiles)
+            o = self._prefill_attention(q, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, block_tables, tiles)
         else:
             tp, context_lens, bt_d, plan = decode_tail
             o = torch.empty_like(q)
             if tp:
-                ops.attention_paged_prefill(q[:tp], self.k_cache, self.v_cache, cu_seqlens_q, cu_seqlens_k,
-                                            max_seqlen_q, block_tables, self.scale, tiles=tiles, out=o[:tp])
+                self._prefill_attention(q[:tp], cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, block_tables,
+                                        tiles, out=o[:tp])
             self._decode_attention(q[tp:], context_lens, bt_d, plan, out=o[tp:])
         return ops.linear(o.view(x.shape[0], -1), self.o_proj.weight)
 
+    def _project_store(self, x, positions, slots):
+        """Rotated queries [T, heads, head_dim] of hidden states x; their keys and values go to the cache
+        rows ``slots``."""
+        norm = (positions, self._cos_sin(x.device), self.q_norm.weight, self.k_norm.weight, self.eps, self.num_heads,
+                self.num_kv_heads, self.k_cache, self.v_cache)
+        if self.k_scale is not None:
+            return ops.qk_norm_rope_store_fp8(ops.linear(x, self.qkv_proj.weight), *norm, self.k_scale, self.v_scale,
+                                              slots)
+        # qkv projection with QK-norm, RoPE and the K/V store in the GEMM's epilogue
+        return ops.qkv_norm_rope_store(x, self.qkv_proj.weight, *norm, slots)
+
+    def _prefill_attention(self, q, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, block_tables, tiles,
+                           out=None):
+        if self.k_scale is not None:
+            return ops.attention_paged_prefill_fp8(q, self.k_cache, self.v_cache, self.k_scale, self.v_scale,
+                                                   cu_seqlens_q, cu_seqlens_k, max_seqlen_q, block_tables, self.scale,
+                                                   tiles=tiles, out=out, max_seqlen_k=max_seqlen_k)
+        return ops.attention_paged_prefill(q, self.k_cache, self.v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
+                                           block_tables, self.scale, tiles=tiles, out=out)
+
     def _decode_attention(self, q, context_lens, block_tables, decode_plan, out=None):
+        if self.k_scale is not None:
+            cache = (self.k_cache, self.v_cache, self.k_scale, self.v_scale)
+            if decode_plan is not None and decode_plan[0] == "grouped":
+                _, plan, ws, members, shared_len, kv_start = decode_plan
+                return ops.paged_decode_attention_grouped_fp8(q, *cache, block_tables, context_lens, self.scale, members,
+                                                              shared_len, kv_start, plan, workspace=ws, out=out)
+            _, split_tokens, max_splits, ws = decode_plan or (None, None, None, None)
+            return ops.paged_decode_attention_fp8(q, *cache, block_tables, context_lens, self.scale,
+                                                  split_tokens=split_tokens, max_splits=max_splits, workspace=ws, out=out)
         if decode_plan is None:
             o = ops.paged_decode_attention(q, self.k_cache, self.v_cache, block_tables, context_lens, self.scale)
         elif decode_plan[0] == "grouped":
@@ -362,9 +389,7 @@ class Qwen3Attention(nn.Module):
         """One new token per sequence (qwen3_naive.py:642-683); attends to context_lens + 1 keys."""
         if slot_mapping is None:
             raise ValueError("the decode step stores the new token's K/V through slot_mapping")
-        q = ops.qkv_norm_rope_store(x, self.qkv_proj.weight, positions, self._cos_sin(x.device), self.q_norm.weight,
-                                    self.k_norm.weight, self.eps, self.num_heads, self.num_kv_heads, self.k_cache,
-                                    self.v_cache, slot_mapping)
+        q = self._project_store(x, positions, slot_mapping)
         o = self._decode_attention(q, context_lens, block_tables, decode_plan)
         return ops.linear(o.view(x.shape[0], -1), self.o_proj.weight)
 
@@ -577,6 +602,9 @@ class Qwen3ForCausalLM(nn.Module):
         self.use_cuda_graphs = True  # decode steps replay captured graphs (False: eager launches)
         self.pipeline_decode = True  # grouped rollout: submit decode step k+1 before step k's bookkeeping
         self.rollout_stats: dict = {}  # per generate call: steps, decode steps, host time waiting on the GPU
+        # paged K/V cache: "bf16", or "fp8": e4m3 codes with one scale per 64 tokens and kv head (half the bytes
+        # a decode step reads, twice the pages in a pool; the reference has bf16 only)
+        self.kv_cache_dtype = "bf16"
         self.max_model_len = None  # KV positions a sequence may reach; default = prompt + max_new_tokens
 
     def forward(self, x):
@@ -591,7 +619,14 @@ class Qwen3ForCausalLM(nn.Module):
     # ---------------------------------------------------------------- KV cache
     def _block_bytes(self):
         a = self.model.layers[0].self_attn
-        return 2 * len(self.model.layers) * self.BLOCK_SIZE * a.num_kv_heads * a.head_dim * 2
+        # fp8: a byte an element and a 4-byte scale per 64 tokens
+        row = a.head_dim + 4 / ops.KV_FP8_BLOCK if self._kv_fp8() else a.head_dim * 2
+        return int(2 * len(self.model.layers) * self.BLOCK_SIZE * a.num_kv_heads * row)
+
+    def _kv_fp8(self) -> bool:
+        if self.kv_cache_dtype not in ("bf16", "fp8"):
+            raise ValueError(f'kv_cache_dtype is "bf16" or "fp8", not {self.kv_cache_dtype!r}')
+        return self.kv_cache_dtype == "fp8"
 
     def _compute_num_blocks(self, gpu_memory_utilization=0.9):
         """Pages that fit after a 2048-token warm-up (qwen3_naive.py:996-1034)."""
@@ -611,24 +646,38 @@ class Qwen3ForCausalLM(nn.Module):
         return max(available // self._block_bytes(), 1)
 
     def allocate_global_kv_cache(self):
-        """K and V caches [layers, num_blocks, 256, kv_heads, head_dim] bf16; each layer gets a view."""
+        """K and V caches [layers, num_blocks, 256, kv_heads, head_dim] bf16; each layer gets a view.  With
+        ``kv_cache_dtype = "fp8"``: codes [layers, num_blocks, kv_heads, 256, head_dim] e4m3 and scales
+        [layers, num_blocks, kv_heads, 4] fp32."""
         a0 = self.model.layers[0].self_attn
+        fp8 = self._kv_fp8()
         if not self._num_blocks:
             self._num_blocks = self._compute_num_blocks()
-        shape = (self._num_blocks, self.BLOCK_SIZE, a0.num_kv_heads, a0.head_dim)
-        if a0.k_cache is not None and tuple(a0.k_cache.shape) == shape:
+        if fp8:
+            shape = (self._num_blocks, a0.num_kv_heads, self.BLOCK_SIZE, a0.head_dim)
+        else:
+            shape = (self._num_blocks, self.BLOCK_SIZE, a0.num_kv_heads, a0.head_dim)
+        if a0.k_cache is not None and tuple(a0.k_cache.shape) == shape and (a0.k_scale is not None) == fp8:
             return
         dev = self.lm_head.weight.device
         L = len(self.model.layers)
         for layer in self.model.layers:  # drop old views before allocating the new pool
-            layer.self_attn.k_cache = layer.self_attn.v_cache = None
+            at = layer.self_attn
+            at.k_cache = at.v_cache = at.k_scale = at.v_scale = None
         self._graphs.clear()
         self._has_cuda_graphs = False
-        k = torch.empty(L, *shape, dtype=torch.bfloat16, device=dev)
-        v = torch.empty(L, *shape, dtype=torch.bfloat16, device=dev)
+        if fp8:
+            k, v, ks, vs = ops.kv_cache_fp8(L * self._num_blocks, a0.num_kv_heads, dev)
+            ks, vs = (s.view(L, self._num_blocks, *s.shape[1:]) for s in (ks, vs))
+            k, v = k.view(L, *shape), v.view(L, *shape)
+        else:
+            k = torch.empty(L, *shape, dtype=torch.bfloat16, device=dev)
+            v = torch.empty(L, *shape, dtype=torch.bfloat16, device=dev)
         for i, layer in enumerate(self.model.layers):
             layer.self_attn.k_cache = k[i]
             layer.self_attn.v_cache = v[i]
+            if fp8:
+                layer.self_attn.k_scale, layer.self_attn.v_scale = ks[i], vs[i]
 
     # ---------------------------------------------------------------- metadata (reference signatures)
     def _prepare_step(self, seqs: list[Sequence]):
@@ -738,15 +787,27 @@ class Qwen3ForCausalLM(nn.Module):
         dev = self.lm_head.weight.device
         if grouped:
             b = self._graph_bufs
-            plan = ops.grouped_decode_plan(bs, a.num_kv_heads, self._graph_max_shared, self._graph_max_ctx)
-            ws = ops.grouped_workspace(bs, a.num_heads, a.head_dim, plan, dev)
+            plan, ws = self._grouped_plan(bs, self._graph_max_shared, self._graph_max_ctx)
             return ("grouped", plan, ws, b["members"][:bs], b["shared_len"][:bs], b["kv_start"][:bs])
+        if self._kv_fp8():
+            split_tokens, max_splits = ops.decode_split_plan_fp8(bs, a.num_kv_heads, self._graph_max_ctx)
+            return ("split", split_tokens, max_splits, ops.workspace_fp8(bs, a.num_heads, max_splits, dev))
         split_tokens, max_splits = ops.decode_split_plan(bs, a.num_kv_heads, self._graph_max_ctx)
         ws = None
         if max_splits > 1:
             nb = ops.lib().qb_paged_decode_workspace_bytes(bs, a.num_heads, a.head_dim, max_splits)
             ws = torch.empty(nb // 4, dtype=torch.float32, device=dev)
         return ("split", split_tokens, max_splits, ws)
+
+    def _grouped_plan(self, bs, max_shared, max_own):
+        """(plan, workspace) of the grouped decode attention for ``bs`` sequences."""
+        a = self.model.layers[0].self_attn
+        dev = self.lm_head.weight.device
+        if self._kv_fp8():
+            plan = ops.grouped_decode_plan_fp8(bs, max(1, bs // 8), a.num_heads, a.num_kv_heads, max_shared, max_own)
+            return plan, ops.workspace_fp8(bs, a.num_heads, plan[1] + plan[3], dev, grouped=True)
+        plan = ops.grouped_decode_plan(bs, a.num_kv_heads, max_shared, max_own)
+        return plan, ops.grouped_workspace(bs, a.num_heads, a.head_dim, plan, dev)
 
     def _decode_body(self, bs, plan, temperature, top_k):
         b = self._graph_bufs
@@ -1010,7 +1071,6 @@ class Qwen3ForCausalLM(nn.Module):
         prefill's last row) and the read-back."""
         dev, temperature, top_k = ctx["dev"], ctx["temperature"], ctx["top_k"]
         r = None
-        a = self.model.layers[0].self_attn
         nd = len(decode_rows)
         if not prefill:
             if self._has_cuda_graphs:
@@ -1029,12 +1089,10 @@ class Qwen3ForCausalLM(nn.Module):
             if nd:
                 ids_d, pos_d, cl, bt_d, slots = self._decode_arrays(decode_rows)
                 mem, sl, ks = _group_arrays(groups_rows, nd)
-                plan = ops.grouped_decode_plan(nd, a.num_kv_heads, int(sl.max(initial=0)),
-                                               int((cl + 1 - ks).max(initial=1)))
+                plan, ws = self._grouped_plan(nd, int(sl.max(initial=0)), int((cl + 1 - ks).max(initial=1)))
                 (ids, pos, blk_map, cu_q, cu_k, bt, tiles, rows, cl_d, bt_d, mem_d, sl_d, ks_d) = self._staging().put(
                     [np.concatenate([ids, ids_d]), np.concatenate([pos, pos_d]), np.concatenate([blk_map, slots]),
                      cu_q, cu_k, bt, tiles, rows_np, cl, bt_d, mem, sl, ks])
-                ws = ops.grouped_workspace(nd, a.num_heads, a.head_dim, plan, dev)
                 tail = (tp, cl_d, bt_d, ("grouped", plan, ws, mem_d, sl_d, ks_d))
             else:
                 ids, pos, cu_q, cu_k, blk_map, bt, tiles, rows = self._staging().put(
@@ -1052,14 +1110,11 @@ class Qwen3ForCausalLM(nn.Module):
 
     def _grouped_decode_eager(self, ctx, arrays, groups_rows, step):
         """One grouped decode step without graphs (shared-prefix attention); returns (tokens, logp) on the device."""
-        dev = ctx["dev"]
-        a = self.model.layers[0].self_attn
         ids, pos, cl, bt, slots = arrays
         nd = len(ids)
         mem, sl, ks = _group_arrays(groups_rows, nd)
-        plan = ops.grouped_decode_plan(nd, a.num_kv_heads, int(sl.max(initial=0)), int((cl + 1 - ks).max(initial=1)))
+        plan, ws = self._grouped_plan(nd, int(sl.max(initial=0)), int((cl + 1 - ks).max(initial=1)))
         ids, pos, cl, bt, slots, mem_d, sl_d, ks_d = self._staging().put([ids, pos, cl, bt, slots, mem, sl, ks])
-        ws = ops.grouped_workspace(nd, a.num_heads, a.head_dim, plan, dev)
         h = self.model.forward_decode(ids, pos, cl, bt, slots, decode_plan=("grouped", plan, ws, mem_d, sl_d, ks_d))
         logits = ops.linear(h, self.lm_head.weight)
         ctx["rng"][0].fill_(step)
