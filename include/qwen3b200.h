@@ -233,7 +233,9 @@ int qb_paged_decode_attn_fp8(const void* q, int64_t q_stride, const void* k_cach
 /* The grouped form; arguments as qb_paged_decode_attn_grouped, with the shared and the own keys split
  * apart: shared_tokens * shared_splits >= every shared_len, own_tokens * own_splits >= every
  * seqlens[b] + seqlen_add - kv_start[b].  Sequences in no group get zeros; kv_start is a multiple of 64;
- * entries of group_members that name no sequence set QB_DEVERR_SHAPE.  A sequence is in one group at
+ * entries of group_members that name no sequence set QB_DEVERR_SHAPE.  The CTAs of the shared keys take
+ * groups g, g + group_step, ... one after another: the number of live groups expected (a table captured
+ * for any grouping may have many empty entries behind them, which then cost no CTAs), or n_groups.  A sequence is in one group at
  * most.  workspace: qb_paged_decode_grouped_fp8_workspace_bytes(batch, hq, shared_splits + own_splits),
  * any contents. */
 int qb_paged_decode_attn_grouped_fp8(const void* q, int64_t q_stride, const void* k_cache,
@@ -242,8 +244,8 @@ int qb_paged_decode_attn_grouped_fp8(const void* q, int64_t q_stride, const void
                                      int64_t bt_stride, int bt_width, const int32_t* seqlens,
                                      int seqlen_add, int batch, int hq, int hkv, int D, float scale,
                                      const int32_t* group_members, const int32_t* shared_len,
-                                     int n_groups, const int32_t* kv_start, int shared_tokens,
-                                     int shared_splits, int own_tokens, int own_splits,
+                                     int n_groups, const int32_t* kv_start, int group_step,
+                                     int shared_tokens, int shared_splits, int own_tokens, int own_splits,
                                      float* workspace, void* out, int* err, qb_stream_t stream);
 size_t qb_paged_decode_fp8_workspace_bytes(int batch, int hq, int n_slots);
 size_t qb_paged_decode_grouped_fp8_workspace_bytes(int batch, int hq, int n_slots);

@@ -65,7 +65,6 @@ struct DecodeP {
   unsigned n_shared;          // shared CTAs; the own CTAs follow
   int* entry_of;              // [batch] in the workspace: where a sequence stands in `members`
 };
-constexpr int DC_GROUPS = 8;  // groups of a shared CTA at most
 
 // What a CTA works on: `rows` query rows over keys [begin, end) of table row `table`.
 struct Work {
@@ -605,10 +604,10 @@ extern "C" int qb_paged_decode_attn_grouped_fp8(
     const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, const float* k_scale,
     const float* v_scale, int64_t num_blocks, int page_size, const int32_t* block_tables, int64_t bt_stride,
     int bt_width, const int32_t* seqlens, int seqlen_add, int batch, int hq, int hkv, int D, float scale,
-    const int32_t* group_members, const int32_t* shared_len, int n_groups, const int32_t* kv_start, int shared_tokens,
-    int shared_splits, int own_tokens, int own_splits, float* workspace, void* out, int* err, qb_stream_t stream) {
+    const int32_t* group_members, const int32_t* shared_len, int n_groups, const int32_t* kv_start, int group_step,
+    int shared_tokens, int shared_splits, int own_tokens, int own_splits, float* workspace, void* out, int* err, qb_stream_t stream) {
   if (D != KV8_D || page_size != KV8_PAGE) return QB_ERR_UNSUPPORTED;
-  QB_CHECK_ARG(batch >= 0 && n_groups >= 0 && n_groups <= INT32_MAX / 8 && split_ok(shared_tokens, shared_splits) &&
+  QB_CHECK_ARG(batch >= 0 && n_groups >= 0 && n_groups <= INT32_MAX / 8 && group_step >= 1 && split_ok(shared_tokens, shared_splits) &&
                split_ok(own_tokens, own_splits) && shared_splits <= INT32_MAX - own_splits);
   if (batch == 0 || n_groups == 0) return QB_OK;
   const int ok = kv8_check_cache(q, q_stride, k_cache, v_cache, k_scale, v_scale, num_blocks, block_tables, bt_stride,
@@ -629,9 +628,7 @@ extern "C" int qb_paged_decode_attn_grouped_fp8(
   const int group = hq / hkv, row_tiles = group == 1 ? 1 : 2;
   p.chunk = min(8, row_tiles * 8 / group);
   p.n_chunks = (8 + p.chunk - 1) / p.chunk;
-  // A caller's table of groups may have many empty entries behind its live ones (one captured for any
-  // grouping): a shared CTA takes every group_step-th group, so the empty ones cost no CTAs of their own.
-  p.group_step = (n_groups + DC_GROUPS - 1) / DC_GROUPS;
+  p.group_step = min(group_step, n_groups);
   p.entry_of = reinterpret_cast<int*>(workspace + decode_partials(batch, hq, p.n_slots));
   const int64_t shared = (int64_t)p.group_step * p.n_chunks * hkv * shared_splits;
   QB_CHECK_ARG(shared <= INT32_MAX);

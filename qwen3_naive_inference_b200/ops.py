@@ -539,20 +539,19 @@ def kv_cache_fp8(num_blocks: int, hkv: int, device=None):
     return (*codes, *scales)
 
 
-def _check_kv_fp8(what, k_cache, v_cache, k_scale, v_scale, *others):
-    """(num_blocks, hkv) of an 8-bit cache; refuses tensors the kernels cannot take."""
-    if not k_cache.is_cuda:
-        raise NativeError("qwen3_naive_inference_b200 ops need CUDA tensors (no CPU fallback)")
+def _kv_fp8(what, k_cache, v_cache, k_scale, v_scale, others):
+    """(device, num_blocks, hkv) of an 8-bit cache; refuses tensors the kernels cannot take."""
     dev = k_cache.get_device()
+    if dev < 0:
+        raise NativeError("qwen3_naive_inference_b200 ops need CUDA tensors (no CPU fallback)")
     if dev != torch.cuda.current_device():
         raise NativeError(f"{what}: the tensors must be on the current CUDA device")
     shape = k_cache.shape
-    if k_cache.dtype != FP8 or v_cache.dtype != FP8 or len(shape) != 4 or shape[2:] != (KV_FP8_PAGE, 128) \
-            or v_cache.shape != shape:
+    if k_cache.dtype != FP8 or v_cache.dtype != FP8 or v_cache.shape != shape or len(shape) != 4 \
+            or shape[2] != KV_FP8_PAGE or shape[3] != 128:
         raise NativeError(f"{what} needs float8_e4m3fn caches [num_blocks, kv_heads, {KV_FP8_PAGE}, 128]")
-    sshape = (shape[0], shape[1], KV_FP8_PAGE // KV_FP8_BLOCK)
-    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or k_scale.shape != sshape \
-            or v_scale.shape != sshape:
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or k_scale.shape != v_scale.shape \
+            or k_scale.shape != (shape[0], shape[1], KV_FP8_PAGE // KV_FP8_BLOCK):
         raise NativeError(f"{what} needs fp32 scales [num_blocks, kv_heads, {KV_FP8_PAGE // KV_FP8_BLOCK}]")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
             and v_scale.is_contiguous()):
@@ -560,19 +559,21 @@ def _check_kv_fp8(what, k_cache, v_cache, k_scale, v_scale, *others):
     for t in (v_cache, k_scale, v_scale, *others):
         if t is not None and t.get_device() != dev:
             raise NativeError(f"{what}: every tensor must be on the caches' device")
-    return shape[0], shape[1]
+    return dev, shape[0], shape[1]
 
 
 def _fp8_rows(what, q, hkv):
-    """q [n, hq, 128] bf16 with the heads of a row together and rows on 16-byte boundaries."""
+    """(q, rows, heads, elements between rows) of bf16 queries [n, heads, 128], the heads of a row together
+    and rows on 16-byte boundaries (copied where they are not)."""
     if q.dtype != BF16 or q.dim() != 3 or q.shape[2] != 128:
         raise NativeError(f"{what} needs bf16 queries [n, heads, 128]")
-    hq = q.shape[1]
+    n, hq, _ = q.shape
     if hq % hkv or hq > 16 * hkv:
         raise NativeError(f"{what}: {hq} query heads over {hkv} kv heads (a multiple, at most 16 times)")
-    if q.stride(2) != 1 or q.stride(1) != 128 or q.stride(0) % 8 or q.data_ptr() % 16:
-        q = q.contiguous()
-    return q
+    s0, s1, s2 = q.stride()
+    if s2 != 1 or s1 != 128 or s0 < hq * 128 or s0 % 8 or q.data_ptr() % 16:
+        q, s0 = q.contiguous(), hq * 128
+    return q, n, hq, s0
 
 
 def _fp8_ints(what, *ts):
@@ -583,13 +584,22 @@ def _fp8_ints(what, *ts):
 
 def _fp8_out(what, out, q, strided=False):
     if out is None:
-        return torch.empty(q.shape, dtype=BF16, device=q.device)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.dtype != BF16 or out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != 128 \
-            or out.stride(0) % 8 or out.data_ptr() % 16 or out.get_device() != q.get_device():
+            or out.stride(0) < out.shape[1] * 128 or out.stride(0) % 8 or out.data_ptr() % 16 \
+            or out.get_device() != q.get_device():
         raise NativeError(f"{what}: out must be bf16 like q, rows on 16-byte boundaries")
     if not strided and not out.is_contiguous():
         raise NativeError(f"{what}: out must be contiguous")
     return out
+
+
+def _launch_ptrs(dev):
+    """(error word, current stream) of the current device ``dev`` for a launch."""
+    err = _ERR.get(dev)
+    if err is None:
+        err = err_flag(torch.device("cuda", dev))
+    return err.data_ptr(), torch._C._cuda_getCurrentRawStream(dev)
 
 
 def qk_norm_rope_store_fp8(qkv, positions, cos_sin, q_norm_w, k_norm_w, eps, hq, hkv, k_cache, v_cache, k_scale,
@@ -598,26 +608,28 @@ def qk_norm_rope_store_fp8(qkv, positions, cos_sin, q_norm_w, k_norm_w, eps, hq,
     to the rows ``slot_mapping`` (int32, -1 skips) of the 8-bit cache, and the scales of the blocks they
     enter are raised where they have to be (the rows already there are then rounded again).  A call that
     writes the first row of a block begins it anew."""
-    num_blocks, hkv_c = _check_kv_fp8("qk_norm_rope_store_fp8", k_cache, v_cache, k_scale, v_scale, qkv, positions,
-                                      cos_sin, q_norm_w, k_norm_w, slot_mapping)
-    T, ld = qkv.shape
-    if hkv_c != hkv or ld != (hq + 2 * hkv) * 128 or qkv.dtype != BF16:
-        raise NativeError(f"qk_norm_rope_store_fp8 needs a bf16 projection [T, ({hq} + 2 * {hkv}) * 128] and a cache "
-                          f"of {hkv} heads")
+    what = "qk_norm_rope_store_fp8"
+    dev, num_blocks, hkv_c = _kv_fp8(what, k_cache, v_cache, k_scale, v_scale,
+                                     (qkv, positions, cos_sin, q_norm_w, k_norm_w, slot_mapping))
+    T, width = qkv.shape
+    if hkv_c != hkv or width != (hq + 2 * hkv) * 128 or qkv.dtype != BF16:
+        raise NativeError(f"{what} needs a bf16 projection [T, ({hq} + 2 * {hkv}) * 128] and a cache of {hkv} heads")
     if positions.dtype != torch.long or positions.shape != (T,) or slot_mapping.shape != (T,):
-        raise NativeError("qk_norm_rope_store_fp8 needs int64 positions [T] and int32 slots [T]")
-    _fp8_ints("qk_norm_rope_store_fp8", slot_mapping)
+        raise NativeError(f"{what} needs int64 positions [T] and int32 slots [T]")
+    _fp8_ints(what, slot_mapping)
     if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[1] != 128 or not cos_sin.is_contiguous() \
             or q_norm_w.dtype != BF16 or k_norm_w.dtype != BF16 or q_norm_w.numel() != 128 or k_norm_w.numel() != 128:
-        raise NativeError("qk_norm_rope_store_fp8 needs an fp32 rotation table [max_pos, 128] and bf16 norm weights")
-    if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
-        qkv = qkv.contiguous()
+        raise NativeError(f"{what} needs an fp32 rotation table [max_pos, 128] and bf16 norm weights")
+    ld, unit = qkv.stride()
+    if unit != 1 or ld < width or ld % 8 or qkv.data_ptr() % 16:
+        qkv, ld = qkv.contiguous(), width
     positions, q_norm_w, k_norm_w = positions.contiguous(), q_norm_w.contiguous(), k_norm_w.contiguous()
-    q = torch.empty(T, hq, 128, dtype=BF16, device=qkv.device)
-    check(lib().qb_qk_norm_rope_store_fp8(_p(qkv), T, qkv.stride(0), hq, hkv, 128, _p(positions), _p(cos_sin),
-                                          cos_sin.shape[0], _p(q_norm_w), _p(k_norm_w), eps, _p(q), _p(k_cache),
-                                          _p(v_cache), _p(k_scale), _p(v_scale), _p(slot_mapping), num_blocks,
-                                          KV_FP8_PAGE, _p(err_flag()), stream_ptr()), "qb_qk_norm_rope_store_fp8")
+    q = qkv.new_empty((T, hq, 128))
+    err, stream = _launch_ptrs(dev)
+    check(lib().qb_qk_norm_rope_store_fp8(
+        qkv.data_ptr(), T, ld, hq, hkv, 128, positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0],
+        q_norm_w.data_ptr(), k_norm_w.data_ptr(), eps, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        k_scale.data_ptr(), v_scale.data_ptr(), slot_mapping.data_ptr(), num_blocks, KV_FP8_PAGE, err, stream), what)
     return q
 
 
@@ -629,10 +641,11 @@ def decode_split_plan_fp8(batch: int, hkv: int, max_ctx: int, sm_count: int = 14
 
 
 def grouped_decode_plan_fp8(batch, n_groups, hq, hkv, max_shared, max_own, sm_count=148):
-    """(shared_tokens, shared_splits, own_tokens, own_splits) of :func:`paged_decode_attention_grouped_fp8`."""
+    """(group_step, shared_tokens, shared_splits, own_tokens, own_splits) of
+    :func:`paged_decode_attention_grouped_fp8`; ``n_groups``: the live groups expected."""
     own, own_splits = decode_split_plan_fp8(batch, hkv, max(1, max_own), sm_count)
     shared, shared_splits = decode_split_plan_fp8(n_groups, hkv, max(1, max_shared), sm_count)
-    return shared, shared_splits, own, own_splits
+    return n_groups, shared, shared_splits, own, own_splits
 
 
 def workspace_fp8(batch, hq, n_slots, device, grouped=False):
@@ -642,37 +655,42 @@ def workspace_fp8(batch, hq, n_slots, device, grouped=False):
     return torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
 
 
-def _fp8_workspace(what, workspace, batch, hq, n_slots, device, grouped=False):
-    if workspace is None:
-        return workspace_fp8(batch, hq, n_slots, device, grouped)
+def _fp8_workspace(what, workspace, q, batch, hq, n_slots, grouped=False):
+    """The workspace (kept by the caller until the launch) and its address."""
+    if n_slots == 1 and not grouped:
+        return None, 0
     f = lib().qb_paged_decode_grouped_fp8_workspace_bytes if grouped else lib().qb_paged_decode_fp8_workspace_bytes
-    if workspace.numel() * workspace.element_size() < f(batch, hq, n_slots) or workspace.data_ptr() % 16 \
+    nbytes = f(batch, hq, n_slots)
+    if workspace is None:
+        workspace = q.new_empty((nbytes // 2,))
+    elif workspace.numel() * workspace.element_size() < nbytes or workspace.data_ptr() % 16 \
             or not workspace.is_contiguous():
         raise NativeError(f"{what}: the workspace is too small for {n_slots} splits, or not aligned")
-    return workspace
+    return workspace, workspace.data_ptr()
 
 
 def paged_decode_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_tables, seqlens, scale, seqlen_add=1,
                                split_tokens=None, max_splits=None, workspace=None, max_ctx=None, out=None):
     """:func:`paged_decode_attention` over the 8-bit cache; any hq / hkv up to 16.  ``max_ctx`` bounds the
-    longest sequence (keys beyond it are left out and reported); default: what block_tables can name."""
+    longest sequence (keys beyond it may be left out, and are then reported); default: what block_tables
+    can name."""
     what = "paged_decode_attention_fp8"
-    num_blocks, hkv = _check_kv_fp8(what, k_cache, v_cache, k_scale, v_scale, q, block_tables, seqlens, workspace)
-    q = _fp8_rows(what, q, hkv)
-    B, hq, _ = q.shape
+    dev, num_blocks, hkv = _kv_fp8(what, k_cache, v_cache, k_scale, v_scale, (q, block_tables, seqlens, workspace))
+    q, B, hq, q_stride = _fp8_rows(what, q, hkv)
     _fp8_ints(what, block_tables, seqlens)
-    if block_tables.dim() != 2 or block_tables.shape[0] != B or seqlens.shape != (B,):
+    if block_tables.dim() != 2 or seqlens.dim() != 1 or block_tables.shape[0] != B or seqlens.shape[0] != B:
         raise NativeError(f"{what} needs block_tables [batch, width] and seqlens [batch]")
+    width = block_tables.shape[1]
     if split_tokens is None:
-        split_tokens, max_splits = decode_split_plan_fp8(
-            B, hkv, block_tables.shape[1] * KV_FP8_PAGE if max_ctx is None else max_ctx)
+        split_tokens, max_splits = decode_split_plan_fp8(B, hkv, width * KV_FP8_PAGE if max_ctx is None else max_ctx)
     out = _fp8_out(what, out, q)
-    ws = _fp8_workspace(what, workspace, B, hq, max_splits, q.device)
-    check(lib().qb_paged_decode_attn_fp8(_p(q), q.stride(0), _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale),
-                                         num_blocks, KV_FP8_PAGE, _p(block_tables), block_tables.stride(0),
-                                         block_tables.shape[1], _p(seqlens), seqlen_add, B, hq, hkv, 128, scale,
-                                         split_tokens, max_splits, _p(ws), _p(out), _p(err_flag()), stream_ptr()), "qb_paged_decode_attn_fp8",
-          kernels=2 if max_splits > 1 else 1)
+    ws, ws_ptr = _fp8_workspace(what, workspace, q, B, hq, max_splits)
+    err, stream = _launch_ptrs(dev)
+    check(lib().qb_paged_decode_attn_fp8(
+        q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+        num_blocks, KV_FP8_PAGE, block_tables.data_ptr(), block_tables.stride(0), width, seqlens.data_ptr(), seqlen_add,
+        B, hq, hkv, 128, scale, split_tokens, max_splits, ws_ptr, out.data_ptr(), err, stream), what,
+        kernels=2 if max_splits > 1 else 1)
     return out
 
 
@@ -682,24 +700,25 @@ def paged_decode_attention_grouped_fp8(q, k_cache, v_cache, k_scale, v_scale, bl
     """:func:`paged_decode_attention_grouped` over the 8-bit cache; ``plan`` from
     :func:`grouped_decode_plan_fp8`.  Sequences in no group get zeros."""
     what = "paged_decode_attention_grouped_fp8"
-    num_blocks, hkv = _check_kv_fp8(what, k_cache, v_cache, k_scale, v_scale, q, block_tables, seqlens, group_members,
-                                    shared_len, kv_start, workspace)
-    q = _fp8_rows(what, q, hkv)
-    B, hq, _ = q.shape
+    dev, num_blocks, hkv = _kv_fp8(what, k_cache, v_cache, k_scale, v_scale,
+                                   (q, block_tables, seqlens, group_members, shared_len, kv_start, workspace))
+    q, B, hq, q_stride = _fp8_rows(what, q, hkv)
     _fp8_ints(what, block_tables, seqlens, group_members, shared_len, kv_start)
     n_groups = shared_len.shape[0]
     if block_tables.dim() != 2 or block_tables.shape[0] != B or seqlens.shape != (B,) or kv_start.shape != (B,) \
             or group_members.shape != (n_groups, 8) or not group_members.is_contiguous():
         raise NativeError(f"{what} needs block_tables [batch, width], seqlens and kv_start [batch], group_members "
                           "[groups, 8] and shared_len [groups]")
-    shared_tokens, shared_splits, own_tokens, own_splits = plan
+    group_step, shared_tokens, shared_splits, own_tokens, own_splits = plan
     out = _fp8_out(what, out, q)
-    ws = _fp8_workspace(what, workspace, B, hq, shared_splits + own_splits, q.device, grouped=True)
+    ws, ws_ptr = _fp8_workspace(what, workspace, q, B, hq, shared_splits + own_splits, grouped=True)
+    err, stream = _launch_ptrs(dev)
     check(lib().qb_paged_decode_attn_grouped_fp8(
-        _p(q), q.stride(0), _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale), num_blocks, KV_FP8_PAGE,
-        _p(block_tables), block_tables.stride(0), block_tables.shape[1], _p(seqlens), seqlen_add, B, hq, hkv, 128, scale,
-        _p(group_members), _p(shared_len), n_groups, _p(kv_start), shared_tokens, shared_splits, own_tokens, own_splits,
-        _p(ws), _p(out), _p(err_flag()), stream_ptr()), "qb_paged_decode_attn_grouped_fp8", kernels=2)
+        q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+        num_blocks, KV_FP8_PAGE, block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1],
+        seqlens.data_ptr(), seqlen_add, B, hq, hkv, 128, scale, group_members.data_ptr(), shared_len.data_ptr(), n_groups,
+        kv_start.data_ptr(), group_step, shared_tokens, shared_splits, own_tokens, own_splits, ws_ptr, out.data_ptr(),
+        err, stream), what, kernels=2)
     return out
 
 
@@ -724,31 +743,34 @@ def attention_paged_prefill_fp8(q, k_cache, v_cache, k_scale, v_scale, cu_seqlen
     ``out``.  ``max_seqlen_k`` bounds the longest Lk (keys beyond it may be left out, and are then reported);
     default: what block_tables can name."""
     what = "attention_paged_prefill_fp8"
-    num_blocks, hkv = _check_kv_fp8(what, k_cache, v_cache, k_scale, v_scale, q, cu_seqlens_q, cu_seqlens_k,
-                                    block_tables, tiles)
-    q = _fp8_rows(what, q, hkv)
-    Tq, hq, _ = q.shape
+    dev, num_blocks, hkv = _kv_fp8(what, k_cache, v_cache, k_scale, v_scale,
+                                   (q, cu_seqlens_q, cu_seqlens_k, block_tables, tiles))
+    q, Tq, hq, q_stride = _fp8_rows(what, q, hkv)
     _fp8_ints(what, cu_seqlens_q, cu_seqlens_k, block_tables)
     batch = cu_seqlens_q.shape[0] - 1
     if block_tables.dim() != 2 or block_tables.shape[0] < batch or cu_seqlens_k.shape != cu_seqlens_q.shape:
         raise NativeError(f"{what} needs block_tables [batch, width] and cu_seqlens of batch + 1 entries")
+    width = block_tables.shape[1]
+    tiles_ptr = n_tiles = 0
     if tiles is not None:
         _fp8_ints(what, tiles)
+        if not tiles.is_contiguous():
+            raise NativeError(f"{what} needs contiguous tiles")
+        tiles_ptr, n_tiles = tiles.data_ptr(), tiles.numel() // 2
     out = _fp8_out(what, out, q, strided=True)
     max_q = int(max_seqlen_q)
-    max_k = block_tables.shape[1] * KV_FP8_PAGE if max_seqlen_k is None else int(max_seqlen_k)
-    split_keys, n_splits = prefill_split_plan_fp8(batch, Tq, max_q, max_k, hq, hkv)
-    ws = None
+    split_keys, n_splits = prefill_split_plan_fp8(
+        batch, Tq, max_q, width * KV_FP8_PAGE if max_seqlen_k is None else int(max_seqlen_k), hq, hkv)
+    ws, ws_ptr = None, 0
     if n_splits > 1:
-        ws = torch.empty(lib().qb_attn_paged_prefill_fp8_workspace_bytes(Tq, hq, n_splits) // 4, dtype=torch.float32,
-                         device=q.device)
-    n_tiles = 0 if tiles is None else tiles.numel() // 2
-    check(lib().qb_attn_paged_prefill_fp8(_p(q), q.stride(0), _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale),
-                                          num_blocks, KV_FP8_PAGE, _p(block_tables), block_tables.stride(0),
-                                          block_tables.shape[1], _p(cu_seqlens_q), _p(cu_seqlens_k), batch, _p(tiles),
-                                          n_tiles, (max_q + 63) // 64, hq, hkv, 128, scale, split_keys, n_splits, _p(ws),
-                                          _p(out), out.stride(0), Tq, _p(err_flag()), stream_ptr()),
-          "qb_attn_paged_prefill_fp8", kernels=2 if n_splits > 1 else 1)
+        ws = q.new_empty((lib().qb_attn_paged_prefill_fp8_workspace_bytes(Tq, hq, n_splits) // 2,))
+        ws_ptr = ws.data_ptr()
+    err, stream = _launch_ptrs(dev)
+    check(lib().qb_attn_paged_prefill_fp8(
+        q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+        num_blocks, KV_FP8_PAGE, block_tables.data_ptr(), block_tables.stride(0), width, cu_seqlens_q.data_ptr(),
+        cu_seqlens_k.data_ptr(), batch, tiles_ptr, n_tiles, (max_q + 63) // 64, hq, hkv, 128, scale, split_keys, n_splits,
+        ws_ptr, out.data_ptr(), out.stride(0), Tq, err, stream), what, kernels=2 if n_splits > 1 else 1)
     return out
 
 

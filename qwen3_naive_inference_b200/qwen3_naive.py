@@ -805,7 +805,7 @@ class Qwen3ForCausalLM(nn.Module):
         dev = self.lm_head.weight.device
         if self._kv_fp8():
             plan = ops.grouped_decode_plan_fp8(bs, max(1, bs // 8), a.num_heads, a.num_kv_heads, max_shared, max_own)
-            return plan, ops.workspace_fp8(bs, a.num_heads, plan[1] + plan[3], dev, grouped=True)
+            return plan, ops.workspace_fp8(bs, a.num_heads, plan[2] + plan[4], dev, grouped=True)
         plan = ops.grouped_decode_plan(bs, a.num_kv_heads, max_shared, max_own)
         return plan, ops.grouped_workspace(bs, a.num_heads, a.head_dim, plan, dev)
 

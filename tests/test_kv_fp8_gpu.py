@@ -282,20 +282,20 @@ def test_grouped_table_with_empty_entries(cuda):
     n = q.shape[0]
     plan = ops.grouped_decode_plan_fp8(n, 4, 16, 8, 600, 200)
     want = ops.paged_decode_attention_grouped_fp8(*args, 0.1, *grp, plan)
-    for at in ([0, 1, 2, 3], [0, 6, 12, 18], [5, 17, 18, 40], [7, 0, 39, 20]):
+    for step, at in ((41, [0, 1, 2, 3]), (4, [0, 1, 2, 3]), (6, [0, 6, 12, 18]), (5, [5, 17, 18, 40]), (1, [7, 0, 39, 20])):
         members = torch.full((41, 8), -1, dtype=torch.int32, device=cuda)
         shared = torch.zeros(41, dtype=torch.int32, device=cuda)
         for i, slot in enumerate(at):
             members[slot], shared[slot] = grp[0][i], grp[1][i]
-        out = ops.paged_decode_attention_grouped_fp8(*args, 0.1, members, shared, grp[2], (64, 24, 128, 8))
-        check = ops.paged_decode_attention_grouped_fp8(*args, 0.1, *grp, (64, 24, 128, 8))
+        out = ops.paged_decode_attention_grouped_fp8(*args, 0.1, members, shared, grp[2], (step, 64, 24, 128, 8))
+        check = ops.paged_decode_attention_grouped_fp8(*args, 0.1, *grp, (2, 64, 24, 128, 8))
         assert torch.equal(out, check)
         assert torch.allclose(out.float(), want.float(), rtol=2.0 ** -6, atol=1e-2)
     ops.check_device_errors()
 
 
 @pytest.mark.parametrize("hq,hkv,groups", GROUPED)
-@pytest.mark.parametrize("plan", [None, (64, 24, 128, 8)])
+@pytest.mark.parametrize("plan", [None, (2, 64, 24, 128, 8)])
 def test_grouped(cuda, hq, hkv, groups, plan):
     g = gen(hq + len(groups))
     q, k, v, ks, vs, parts, args, grp = grouped_inputs(g, hq, hkv, groups, cuda)
@@ -328,7 +328,7 @@ def test_grouped_equals_plain_decode_where_nothing_is_skipped(cuda):
     members[0, 1] = -1
     out = torch.full_like(a, 3.0)
     keep = [i for i in range(3) if i != lone]
-    ws = ops.workspace_fp8(3, 16, plan[1] + plan[3], cuda, grouped=True)
+    ws = ops.workspace_fp8(3, 16, plan[2] + plan[4], cuda, grouped=True)
     for fill in (0, -1, 1, 5, 7 << 28):
         ws.view(torch.int32).fill_(fill)
         ops.paged_decode_attention_grouped_fp8(*args, 0.1, members, *grp[1:], plan, out=out, workspace=ws)
@@ -747,7 +747,7 @@ def test_refusals(cuda):
         lambda: ops.qk_norm_rope_store_fp8(torch.zeros(1, 5 * D, dtype=BF, device=cuda), n.long(), torch.zeros(8, D, device=cuda),
                                            q[0, 0], q[0, 0], 1e-6, 4, 2, k, v, ks, vs, n),
         lambda: ops.attention_paged_prefill_fp8(q, k, v, ks, vs, i32(0, 1), i32(0, 1, 2), 1, t, 0.1),
-        lambda: ops.paged_decode_attention_grouped_fp8(q, k, v, ks, vs, t, n, 0.1, i32(0, -1).view(1, 2), i32(3), i32(0), (64, 1, 64, 1)),
+        lambda: ops.paged_decode_attention_grouped_fp8(q, k, v, ks, vs, t, n, 0.1, i32(0, -1).view(1, 2), i32(3), i32(0), (1, 64, 1, 64, 1)),
     ]
     for i, f in enumerate(bad):
         with pytest.raises(ops.NativeError):

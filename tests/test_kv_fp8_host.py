@@ -29,12 +29,12 @@ def test_decode_refusals():
 def test_grouped_refusals():
     lib = _lib.load()
 
-    def call(ws=A, members=A, n_groups=1, shared=(64, 1), own=(64, 1), D=128):
+    def call(ws=A, members=A, n_groups=1, shared=(64, 1), own=(64, 1), D=128, step=1):
         return lib.qb_paged_decode_attn_grouped_fp8(A, 2048, A, A, A, A, 4, 256, A, 1, 1, A, 1, 1, 16, 8, D, 1.0, members, A,
-                                                    n_groups, A, *shared, *own, ws, A, None, None)
+                                                    n_groups, A, step, *shared, *own, ws, A, None, None)
 
     assert call(D=96) == 2
-    assert call(ws=None) == 1 and call(members=None) == 1 and call(n_groups=-1) == 1
+    assert call(step=0) == 1 and call(ws=None) == 1 and call(members=None) == 1 and call(n_groups=-1) == 1
     assert call(shared=(100, 1)) == 1 and call(own=(64, 0)) == 1 and call(own=(16384, 1)) == 1
     assert call(n_groups=0) == 0
 
@@ -92,7 +92,8 @@ def test_cpu_tensors_are_refused():
 def test_plans_cover_the_context(batch, hkv, ctx):
     for split, n in [ops.decode_split_plan_fp8(batch, hkv, ctx)]:
         assert split % 64 == 0 and 64 <= split <= 8192 and n >= 1 and split * n >= ctx and (n - 1) * split < max(1, ctx)
-    sh, ns, ow, no = ops.grouped_decode_plan_fp8(batch, max(1, batch // 8), 2 * hkv, hkv, ctx, ctx)
+    step, sh, ns, ow, no = ops.grouped_decode_plan_fp8(batch, max(1, batch // 8), 2 * hkv, hkv, ctx, ctx)
+    assert step == max(1, batch // 8)
     for split, n in ((sh, ns), (ow, no)):
         assert split % 64 == 0 and 64 <= split <= 8192 and n >= 1 and split * n >= ctx
 
