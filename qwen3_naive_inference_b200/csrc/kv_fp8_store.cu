@@ -11,10 +11,12 @@
 // there are rounded again under the new one.  A call that writes row 0 of a block begins it anew (a
 // recycled page's old scale is dropped).
 //
-// Work split: one CTA per window of eight tokens and kv head for K and V, further CTAs for q.  All
-// tokens of the call that fall into one block are handled by the CTA whose window holds the first of
-// them, so a block's scale has one writer; the CTA finds the others by scanning the slots (tokens
-// whose left neighbour is in the same block never scan).  A slot given twice takes the later token.
+// Work split: a CTA per window of tokens and kv heads for K and V, further CTAs for q.  All tokens of the
+// call that fall into one block are handled by the CTA whose window holds the first of them, so a block's
+// scale has one writer; the CTA finds the others by scanning the slots (tokens whose left neighbour is in
+// the same block never scan).  A slot given twice takes the later token.  Windows are eight tokens in a
+// decode step, where each token is in a block of its own (a warp each), 64 in long calls, where most are
+// not, and as many heads share a scan as leave enough CTAs.
 #include <float.h>
 
 #include "kv_fp8.cuh"
@@ -22,7 +24,10 @@
 namespace {
 
 constexpr int ST_THREADS = 256, ST_WARPS = ST_THREADS / 32, ST_HALVES = ST_THREADS / 16;
-constexpr int ST_WIN = ST_WARPS;               // tokens of a window: a warp each in a decode step
+constexpr int ST_GROUP = ST_WARPS;             // blocks taken at a time: a warp each in a decode step
+constexpr int ST_LONG = 64;                    // tokens of a window in a long call ...
+constexpr int ST_LONG_CALL = 768;              // ... of more tokens than a decode step has
+constexpr int ST_ENOUGH = 512;                 // working K/V CTAs that keep the GPU busy
 constexpr int ST_ROWS = KV8_BLOCK / ST_HALVES;  // rows of a block per half-warp
 constexpr int ST_QH = 4;                       // q heads per half-warp item (one rotation-table row for all)
 
@@ -45,7 +50,8 @@ struct StoreParams {
   float* scales[2];
   const int32_t* slots;
   int64_t num_slots;
-  int n_kv_ctas;
+  int window, heads;  // tokens and kv heads of a K/V CTA
+  int64_t n_kv_ctas;
   int* err;
 };
 
@@ -171,146 +177,177 @@ QB_DEVICE void store_q(const StoreParams& p, int64_t cta) {
   }
 }
 
+// What a K/V CTA knows of up to ST_GROUP blocks whose first token may be in its window.
+struct Found {
+  int block[ST_GROUP];               // -1: none, or its first token is elsewhere
+  int head[ST_GROUP];                // the run head that brought it
+  int first[ST_GROUP];               // the call's first token in the block
+  int rows[ST_GROUP];                // distinct rows written
+  int row_src[ST_GROUP][KV8_BLOCK];  // the token that writes each row, -1: none
+};
+
+QB_DEVICE void note_token(Found& f, int n, int t, int slot) {
+  const int blk = slot >> 6;  // a skipped slot (-1) matches no block
+#pragma unroll
+  for (int i = 0; i < ST_GROUP; ++i)
+    if (i < n && blk == f.block[i]) {
+      atomicMin(&f.first[i], t);
+      if (atomicMax(&f.row_src[i][slot & (KV8_BLOCK - 1)], t) < 0) atomicAdd(&f.rows[i], 1);
+    }
+}
+
+// One token in each block (a decode step): a warp per block, its first half K, its second half V.
+QB_DEVICE void store_single(const StoreParams& p, const Found& f, int head, const float (&kw)[8]) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & 15, which = lane >> 4;
+  const int blk = f.block[warp];
+  if (blk < 0) return;  // uniform across the warp; no barrier follows in here
+  const int row = p.slots[f.head[warp]] & (KV8_BLOCK - 1);
+  const int64_t t = f.row_src[warp][row];  // the later one where a slot is given twice
+  const int64_t at = ((int64_t)(blk / KV8_SUBS) * p.hkv + head) * KV8_SUBS + blk % KV8_SUBS;
+  float* scale = p.scales[which] + at;
+  uint8_t* block = p.codes[which] + at * KV8_TILE;
+  const float old = *scale;
+  float v[8], y[8], c[8], s[8];
+  unpack_row(ld_row(p.qkv + t * p.ld + (p.hq + (which ? p.hkv : 0) + head) * KV8_D + l * 8), v);
+  ld_rotation(p, checked_pos(p, t, false), l, c, s);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = v[i];
+  norm_rope(y, kw, c, s, p.eps, l);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = which ? v[i] : y[i];
+  const bool anew = row == 0;
+  const float now = joined_scale(old, half_max(finite_max(v)), anew);
+  st_codes(block + row * KV8_D + l * 8, v, 1.f / now);
+  if (l == 0) *scale = now;
+  if (!anew && now > old) round_again(block, f.row_src[warp], old / now, l, 16);
+}
+
+// A block that takes several tokens (a prompt chunk): 16 half-warps on 64 rows.
+QB_DEVICE void store_many(const StoreParams& p, const Found& f, int i, int head, const float (&kw)[8], unsigned* top) {
+  const int tid = threadIdx.x, lane = tid & 31, l = tid & 15, blk = f.block[i];
+  __syncthreads();  // `top` of the block before has been read
+  if (tid < 2) top[tid] = 0;
+  __syncthreads();
+  const int64_t at = ((int64_t)(blk / KV8_SUBS) * p.hkv + head) * KV8_SUBS + blk % KV8_SUBS;
+  const int kcol = (p.hq + head) * KV8_D + l * 8, vcol = kcol + p.hkv * KV8_D;
+  const float old_k = p.scales[0][at], old_v = p.scales[1][at];
+  float k[ST_ROWS][8];
+  Row8 v[ST_ROWS];
+  float top_k = 0.f, top_v = 0.f;
+#pragma unroll
+  for (int r = 0; r < ST_ROWS; ++r) {
+    const int64_t t = f.row_src[i][(tid >> 4) + r * ST_HALVES];
+    const bool live = t >= 0;
+    unpack_row(live ? ld_row(p.qkv + t * p.ld + kcol) : Row8{}, k[r]);
+    v[r] = live ? ld_row(p.qkv + t * p.ld + vcol) : Row8{};
+  }
+#pragma unroll
+  for (int r = 0; r < ST_ROWS; ++r) {
+    const int64_t t = f.row_src[i][(tid >> 4) + r * ST_HALVES];
+    float c[8], s[8];
+    ld_rotation(p, t >= 0 ? checked_pos(p, t, false) : 0, l, c, s);
+    norm_rope(k[r], kw, c, s, p.eps, l);
+    float x[8];
+    unpack_row(v[r], x);
+    top_k = fmaxf(top_k, t >= 0 ? finite_max(k[r]) : 0.f);
+    top_v = fmaxf(top_v, finite_max(x));
+  }
+  top_k = warp_max(top_k);
+  top_v = warp_max(top_v);
+  if (lane == 0) {  // magnitudes are not negative: their bits order as they do
+    atomicMax(&top[0], __float_as_uint(top_k));
+    atomicMax(&top[1], __float_as_uint(top_v));
+  }
+  __syncthreads();
+  const bool anew = f.row_src[i][0] >= 0;
+  const float now_k = joined_scale(old_k, __uint_as_float(top[0]), anew);
+  const float now_v = joined_scale(old_v, __uint_as_float(top[1]), anew);
+  uint8_t* kb = p.codes[0] + at * KV8_TILE;
+  uint8_t* vb = p.codes[1] + at * KV8_TILE;
+#pragma unroll
+  for (int r = 0; r < ST_ROWS; ++r) {
+    const int row = (tid >> 4) + r * ST_HALVES;
+    if (f.row_src[i][row] < 0) continue;
+    float x[8];
+    unpack_row(v[r], x);
+    st_codes(kb + row * KV8_D + l * 8, k[r], 1.f / now_k);
+    st_codes(vb + row * KV8_D + l * 8, x, 1.f / now_v);
+  }
+  if (!anew && now_k > old_k) round_again(kb, f.row_src[i], old_k / now_k, tid, ST_THREADS);
+  if (!anew && now_v > old_v) round_again(vb, f.row_src[i], old_v / now_v, tid, ST_THREADS);
+  if (tid == 0) {
+    p.scales[0][at] = now_k;
+    p.scales[1][at] = now_v;
+  }
+}
+
 __global__ void __launch_bounds__(ST_THREADS)
 kv_fp8_store_kernel(StoreParams p) {
   qb_pdl_trigger();
   qb_pdl_wait();
-  __shared__ int row_src[ST_WIN][KV8_BLOCK];  // per run head of the window: the token of each row, or -1
-  __shared__ int first[ST_WIN], blocks[ST_WIN], rows[ST_WIN];
+  __shared__ Found f;
+  __shared__ int heads[ST_LONG], n_heads;  // run heads of the window: tokens whose left neighbour is in another block
   __shared__ unsigned top[2];
   if ((int64_t)blockIdx.x >= p.n_kv_ctas) {
     store_q(p, (int64_t)blockIdx.x - p.n_kv_ctas);
     return;
   }
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, l = tid & 15;
-  const int head = blockIdx.x % p.hkv;
-  const int64_t t0 = (int64_t)(blockIdx.x / p.hkv) * ST_WIN;
-
-  // run heads of the window: tokens whose left neighbour is in another block
-  bool heads_here = false;
-  if (tid < ST_WIN) {
-    const int64_t t = t0 + tid;
-    int blk = -1;
-    if (t < p.T) {
-      const int64_t slot = p.slots[t];
-      if (slot >= 0 && slot < p.num_slots) {
-        blk = (int)(slot / KV8_BLOCK);
-        if (t > 0 && p.slots[t - 1] >= 0 && p.slots[t - 1] / KV8_BLOCK == blk) blk = -1;
-      } else if (slot != -1 && head == 0) {
-        qb_set_err(p.err, QB_DEVERR_SLOT);
-      }
+  const int tid = threadIdx.x, head_groups = (p.hkv + p.heads - 1) / p.heads;
+  const int head0 = (int)(blockIdx.x % head_groups) * p.heads, head1 = min(p.hkv, head0 + p.heads);
+  const int64_t t0 = (int64_t)(blockIdx.x / head_groups) * p.window;
+  if (tid == 0) n_heads = 0;
+  __syncthreads();
+  if (tid < p.window && t0 + tid < p.T) {
+    const int64_t t = t0 + tid, slot = p.slots[t];
+    if (slot >= 0 && slot < p.num_slots) {
+      const int before = t > 0 ? p.slots[t - 1] : -1;
+      if (before >> 6 != (int)slot >> 6) heads[atomicAdd(&n_heads, 1)] = (int)t;
+    } else if (slot != -1 && head0 == 0) {
+      qb_set_err(p.err, QB_DEVERR_SLOT);
     }
-    blocks[tid] = blk;
-    first[tid] = INT32_MAX;
-    rows[tid] = 0;
-    heads_here = blk >= 0;
-  }
-  for (int i = tid; i < ST_WIN * KV8_BLOCK; i += ST_THREADS) (&row_src[0][0])[i] = -1;
-  if (!__syncthreads_or(heads_here)) return;
-  // every token of the call in one of those blocks
-  for (int64_t t = tid; t < p.T; t += ST_THREADS) {
-    const int slot = p.slots[t];
-    const int blk = slot >= 0 ? slot / KV8_BLOCK : -2;
-#pragma unroll
-    for (int i = 0; i < ST_WIN; ++i)
-      if (blk == blocks[i]) {
-        atomicMin(&first[i], (int)t);
-        if (atomicMax(&row_src[i][slot % KV8_BLOCK], (int)t) < 0) atomicAdd(&rows[i], 1);
-      }
   }
   __syncthreads();
-  bool many = false;
-  if (tid < ST_WIN) {
-    if (blocks[tid] >= 0 && first[tid] != (int)(t0 + tid)) blocks[tid] = -1;  // another run head came first
-    many = blocks[tid] >= 0 && rows[tid] > 1;
-  }
-  many = __syncthreads_or(many);
-
+  const int n = n_heads;
+  if (n == 0) return;
   float kw[8];
-  unpack_row(ld_row(p.kw + l * 8), kw);
-  const int kcol = (p.hq + head) * KV8_D + l * 8, vcol = kcol + p.hkv * KV8_D;
-  if (!many) {
-    // one token per block (a decode step): a warp each, its first half K, its second half V
-    const int blk = blocks[warp];
-    if (blk < 0) return;  // uniform across the warp; no barrier follows
-    const int which = lane >> 4;
-    const int row = p.slots[t0 + warp] % KV8_BLOCK;
-    const int64_t t = row_src[warp][row];  // the later one where a slot is given twice
-    const int64_t at = (int64_t)(blk / KV8_SUBS) * p.hkv + head;  // (page, head)
-    float* scale = p.scales[which] + at * KV8_SUBS + blk % KV8_SUBS;
-    uint8_t* block = p.codes[which] + (at * KV8_SUBS + blk % KV8_SUBS) * KV8_TILE;
-    const float old = *scale;
-    float v[8], y[8], c[8], s[8];
-    unpack_row(ld_row(p.qkv + t * p.ld + (which ? vcol : kcol)), v);
-    ld_rotation(p, checked_pos(p, t, lane == 0 && head == 0), l, c, s);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = v[i];
-    norm_rope(y, kw, c, s, p.eps, l);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = which ? v[i] : y[i];
-    const bool anew = row == 0;
-    const float now = joined_scale(old, half_max(finite_max(v)), anew);
-    st_codes(block + row * KV8_D + l * 8, v, 1.f / now);
-    if (l == 0) *scale = now;
-    if (!anew && now > old) round_again(block, row_src[warp], old / now, l, 16);
-    return;
-  }
-  // blocks that take several tokens (prompt chunks), one after another: 16 half-warps on 64 rows
-  for (int i = 0; i < ST_WIN; ++i) {
-    const int blk = blocks[i];
-    if (blk < 0) continue;  // uniform across the CTA
-    __syncthreads();        // `top` of the block before has been read
-    if (tid < 2) top[tid] = 0;
+  unpack_row(ld_row(p.kw + (tid & 15) * 8), kw);
+  const bool aligned = (reinterpret_cast<uintptr_t>(p.slots) & 15) == 0;
+  for (int g0 = 0; g0 < n; g0 += ST_GROUP) {
+    const int m = min(ST_GROUP, n - g0);
+    __syncthreads();  // the group before is done
+    if (tid < ST_GROUP) {
+      f.head[tid] = tid < m ? heads[g0 + tid] : -1;
+      f.block[tid] = tid < m ? p.slots[f.head[tid]] >> 6 : -1;
+      f.first[tid] = INT32_MAX;
+      f.rows[tid] = 0;
+    }
+    for (int i = tid; i < ST_GROUP * KV8_BLOCK; i += ST_THREADS) (&f.row_src[0][0])[i] = -1;
     __syncthreads();
-    const int64_t at = ((int64_t)(blk / KV8_SUBS) * p.hkv + head) * KV8_SUBS + blk % KV8_SUBS;
-    const float old_k = p.scales[0][at], old_v = p.scales[1][at];
-    float k[ST_ROWS][8];
-    Row8 v[ST_ROWS];
-    float top_k = 0.f, top_v = 0.f;
-#pragma unroll
-    for (int r = 0; r < ST_ROWS; ++r) {
-      const int64_t t = row_src[i][(tid >> 4) + r * ST_HALVES];
-      const bool live = t >= 0;
-      unpack_row(live ? ld_row(p.qkv + t * p.ld + kcol) : Row8{}, k[r]);
-      v[r] = live ? ld_row(p.qkv + t * p.ld + vcol) : Row8{};
+    // every token of the call in one of those blocks
+    const int64_t quads = aligned ? p.T / 4 : 0;
+#pragma unroll 4
+    for (int64_t t = tid; t < quads; t += ST_THREADS) {
+      const int4 s = reinterpret_cast<const int4*>(p.slots)[t];
+      note_token(f, m, (int)(4 * t), s.x);
+      note_token(f, m, (int)(4 * t + 1), s.y);
+      note_token(f, m, (int)(4 * t + 2), s.z);
+      note_token(f, m, (int)(4 * t + 3), s.w);
     }
-#pragma unroll
-    for (int r = 0; r < ST_ROWS; ++r) {
-      const int64_t t = row_src[i][(tid >> 4) + r * ST_HALVES];
-      float c[8], s[8];
-      ld_rotation(p, t >= 0 ? checked_pos(p, t, l == 0 && head == 0) : 0, l, c, s);
-      norm_rope(k[r], kw, c, s, p.eps, l);
-      float x[8];
-      unpack_row(v[r], x);
-      top_k = fmaxf(top_k, t >= 0 ? finite_max(k[r]) : 0.f);
-      top_v = fmaxf(top_v, finite_max(x));
-    }
-    top_k = warp_max(top_k);
-    top_v = warp_max(top_v);
-    if (lane == 0) {  // magnitudes are not negative: their bits order as they do
-      atomicMax(&top[0], __float_as_uint(top_k));
-      atomicMax(&top[1], __float_as_uint(top_v));
-    }
+    for (int64_t t = 4 * quads + tid; t < p.T; t += ST_THREADS) note_token(f, m, (int)t, p.slots[t]);
     __syncthreads();
-    const bool anew = row_src[i][0] >= 0;
-    const float now_k = joined_scale(old_k, __uint_as_float(top[0]), anew);
-    const float now_v = joined_scale(old_v, __uint_as_float(top[1]), anew);
-    uint8_t* kb = p.codes[0] + at * KV8_TILE;
-    uint8_t* vb = p.codes[1] + at * KV8_TILE;
-#pragma unroll
-    for (int r = 0; r < ST_ROWS; ++r) {
-      const int row = (tid >> 4) + r * ST_HALVES;
-      if (row_src[i][row] < 0) continue;
-      float x[8];
-      unpack_row(v[r], x);
-      st_codes(kb + row * KV8_D + l * 8, k[r], 1.f / now_k);
-      st_codes(vb + row * KV8_D + l * 8, x, 1.f / now_v);
+    bool many = false;
+    if (tid < ST_GROUP) {
+      if (f.block[tid] >= 0 && f.first[tid] != f.head[tid]) f.block[tid] = -1;  // another run head came first
+      many = f.block[tid] >= 0 && f.rows[tid] > 1;
     }
-    if (!anew && now_k > old_k) round_again(kb, row_src[i], old_k / now_k, tid, ST_THREADS);
-    if (!anew && now_v > old_v) round_again(vb, row_src[i], old_v / now_v, tid, ST_THREADS);
-    if (tid == 0) {
-      p.scales[0][at] = now_k;
-      p.scales[1][at] = now_v;
+    many = __syncthreads_or(many);
+    for (int head = head0; head < head1; ++head) {
+      if (!many) {
+        store_single(p, f, head, kw);
+        continue;
+      }
+      for (int i = 0; i < m; ++i)
+        if (f.block[i] >= 0) store_many(p, f, i, head, kw, top);  // uniform across the CTA
     }
   }
 }
@@ -333,11 +370,16 @@ extern "C" int qb_qk_norm_rope_store_fp8(const void* qkv, int64_t T, int64_t ld_
   QB_CHECK_ARG(al16(qkv) && al16(cos_sin) && al16(q_norm_w) && al16(k_norm_w) && al16(q_out) && al16(k_cache) &&
                al16(v_cache));
   QB_CHECK_ARG(num_blocks <= (int64_t)INT32_MAX / KV8_PAGE);  // slots are int32
-  const int64_t kv = (T + ST_WIN - 1) / ST_WIN * hkv;
-  const int64_t q = (T * ((hq + ST_QH - 1) / ST_QH) + ST_HALVES - 1) / ST_HALVES;
-  QB_CHECK_ARG(T < INT32_MAX && kv + q <= INT32_MAX);
   StoreParams p{(const bf16*)qkv, T, ld_in, hq, hkv, positions, cos_sin, max_pos, (const bf16*)q_norm_w,
                 (const bf16*)k_norm_w, eps, (bf16*)q_out, {(uint8_t*)k_cache, (uint8_t*)v_cache},
-                {k_scale, v_scale}, slot_mapping, num_blocks * KV8_PAGE, (int)kv, err};
+                {k_scale, v_scale}, slot_mapping, num_blocks * KV8_PAGE, ST_GROUP, 1, 0, err};
+  if (T > ST_LONG_CALL) {
+    p.window = ST_LONG;
+    while (p.heads < hkv && T / KV8_BLOCK * hkv / (2 * p.heads) >= ST_ENOUGH) p.heads *= 2;
+  }
+  const int64_t kv = (T + p.window - 1) / p.window * ((hkv + p.heads - 1) / p.heads);
+  const int64_t q = (T * ((hq + ST_QH - 1) / ST_QH) + ST_HALVES - 1) / ST_HALVES;
+  QB_CHECK_ARG(T < INT32_MAX && kv + q <= INT32_MAX);
+  p.n_kv_ctas = kv;
   return qb_launch(kv_fp8_store_kernel, dim3((unsigned)(kv + q)), dim3(ST_THREADS), 0, (cudaStream_t)stream, 1, p);
 }
