@@ -14,7 +14,7 @@
 // Work split: a CTA per window of tokens and kv heads for K and V, further CTAs for q.  All tokens of the
 // call that fall into one block are handled by the CTA whose window holds the first of them, so a block's
 // scale has one writer; the CTA finds the others by scanning the slots (tokens whose left neighbour is in
-// the same block never scan).  A slot given twice takes the later token.  Windows are eight tokens in a
+// the same block never scan).  A slot given twice takes the later token.  Windows are 16 tokens in a
 // decode step, where each token is in a block of its own (a warp each), 64 in long calls, where most are
 // not, and as many heads share a scan as leave enough CTAs.
 #include <float.h>
@@ -23,10 +23,11 @@
 
 namespace {
 
-constexpr int ST_THREADS = 256, ST_WARPS = ST_THREADS / 32, ST_HALVES = ST_THREADS / 16;
-constexpr int ST_GROUP = ST_WARPS;             // blocks taken at a time: a warp each in a decode step
+constexpr int ST_THREADS = 512, ST_WARPS = ST_THREADS / 32, ST_HALVES = ST_THREADS / 16;
+constexpr int ST_GROUP = ST_WARPS;             // tokens of a window in a short call, a warp each; blocks looked for at a time
 constexpr int ST_LONG = 64;                    // tokens of a window in a long call ...
 constexpr int ST_LONG_CALL = 768;              // ... of more tokens than a decode step has
+constexpr int ST_ALONE_TRY = 8;                // more run heads than this in a window: look whether they are alone
 constexpr int ST_ENOUGH = 512;                 // working K/V CTAs that keep the GPU busy
 constexpr int ST_ROWS = KV8_BLOCK / ST_HALVES;  // rows of a block per half-warp
 constexpr int ST_QH = 4;                       // q heads per half-warp item (one rotation-table row for all)
@@ -103,15 +104,23 @@ QB_DEVICE void norm_rope(float (&v)[8], const float (&w)[8], const float (&c)[8]
     v[i] = l < 8 ? qk_rope_lo(x, partner, c[i], s[i]) : qk_rope_hi(x, partner, c[i], s[i]);
   }
 }
-// Largest finite magnitude of a lane's values (what is not finite is stored as NaN, whatever the scale).
-QB_DEVICE float finite_max(const float (&v)[8]) {
-  float m = 0.f;
+// Largest magnitude of a lane's values, as bits (they order as magnitudes do).  What is not finite is
+// stored as NaN, whatever the scale, and does not count: `odd` says that there is such a value.
+constexpr uint32_t FINITE = 0x7f7fffffu;
+QB_DEVICE float finite_max(const float (&v)[8], bool& odd) {
+  uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = fabsf(v[i]);
-    m = fmaxf(m, a <= FLT_MAX ? a : 0.f);
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  odd = m > FINITE;
+  if (odd) {
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
+      m = max(m, a <= FINITE ? a : 0u);
+    }
   }
-  return m;
+  return __uint_as_float(m);
 }
 // Smallest power of two (at least 2^-126) under which `top` is within 448 = 1.75 * 2^8.
 QB_DEVICE float scale_for(float top) {
@@ -119,18 +128,25 @@ QB_DEVICE float scale_for(float top) {
   const int e = (int)(b >> 23) - ((b & 0x7fffffu) <= 0x600000u ? 8 : 7);
   return __uint_as_float((uint32_t)max(e, 1) << 23);
 }
-QB_DEVICE float scaled(float x, float inv) { return fabsf(x) <= FLT_MAX ? x * inv : __int_as_float(0x7fffffff); }
-QB_DEVICE void st_codes(uint8_t* dst, const float (&v)[8], float inv) {
+QB_DEVICE void st_codes(uint8_t* dst, float (&v)[8], float inv, bool odd) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] *= inv;
+  if (odd) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if ((__float_as_uint(v[i]) & 0x7fffffffu) > FINITE) v[i] = __int_as_float(0x7fffffff);
+  }
   uint2 u;
-  u.x = float4_to_e4m3x4(scaled(v[0], inv), scaled(v[1], inv), scaled(v[2], inv), scaled(v[3], inv));
-  u.y = float4_to_e4m3x4(scaled(v[4], inv), scaled(v[5], inv), scaled(v[6], inv), scaled(v[7], inv));
+  u.x = float4_to_e4m3x4(v[0], v[1], v[2], v[3]);
+  u.y = float4_to_e4m3x4(v[4], v[5], v[6], v[7]);
   *reinterpret_cast<uint2*>(dst) = u;
 }
-// Rounds the block's rows that this call does not write again under a scale larger by 1 / ratio.
+// Rounds the block's rows that this call does not write (`kept`) again under a scale larger by 1 / ratio.
 // `n` threads take part, this one as number `i`.
-QB_DEVICE void round_again(uint8_t* block, const int* row_src, float ratio, int i, int n) {
+template <typename F>
+QB_DEVICE void round_again(uint8_t* block, F kept, float ratio, int i, int n) {
   for (int c = i; c < KV8_TILE / 16; c += n) {
-    if (row_src[c >> 3] >= 0) continue;
+    if (!kept(c >> 3)) continue;
     uint4* at = reinterpret_cast<uint4*>(block) + c;
     uint4 u = *at;
     uint32_t* w = reinterpret_cast<uint32_t*>(&u);
@@ -151,9 +167,8 @@ QB_DEVICE float joined_scale(float old, float top, bool anew) {
 
 QB_DEVICE void store_q(const StoreParams& p, int64_t cta) {
   const int l = threadIdx.x & 15;
-  const int per_token = (p.hq + ST_QH - 1) / ST_QH;
-  const int64_t item = cta * ST_HALVES + (threadIdx.x >> 4);
-  const bool live = item < p.T * per_token;
+  const unsigned per_token = (p.hq + ST_QH - 1) / ST_QH, item = (unsigned)(cta * ST_HALVES) + (threadIdx.x >> 4);
+  const bool live = item < (unsigned)p.T * per_token;
   const int64_t t = live ? item / per_token : 0;
   const int h0 = live ? (int)(item % per_token) * ST_QH : 0;
   Row8 raw[ST_QH];
@@ -182,47 +197,69 @@ struct Found {
   int block[ST_GROUP];               // -1: none, or its first token is elsewhere
   int head[ST_GROUP];                // the run head that brought it
   int first[ST_GROUP];               // the call's first token in the block
-  int rows[ST_GROUP];                // distinct rows written
   int row_src[ST_GROUP][KV8_BLOCK];  // the token that writes each row, -1: none
 };
 
+QB_DEVICE void note_match(Found& f, int i, int t, int slot) {
+  atomicMin(&f.first[i], t);
+  atomicMax(&f.row_src[i][slot & (KV8_BLOCK - 1)], t);
+}
+// Tokens of the call that fall into one of the n blocks.  A skipped slot (-1) matches no block.
 QB_DEVICE void note_token(Found& f, int n, int t, int slot) {
-  const int blk = slot >> 6;  // a skipped slot (-1) matches no block
-#pragma unroll
-  for (int i = 0; i < ST_GROUP; ++i)
-    if (i < n && blk == f.block[i]) {
-      atomicMin(&f.first[i], t);
-      if (atomicMax(&f.row_src[i][slot & (KV8_BLOCK - 1)], t) < 0) atomicAdd(&f.rows[i], 1);
+  for (int i = 0; i < n; ++i)
+    if (slot >> 6 == f.block[i]) note_match(f, i, t, slot);
+}
+QB_DEVICE void note_tokens(Found& f, int n, int t, const int4& s) {
+  for (int i = 0; i < n; ++i) {  // one block, in a prompt chunk: four comparisons for four tokens
+    const int blk = f.block[i];
+    const bool a = s.x >> 6 == blk, b = s.y >> 6 == blk, c = s.z >> 6 == blk, d = s.w >> 6 == blk;
+    if (a || b || c || d) {
+      if (a) note_match(f, i, t, s.x);
+      if (b) note_match(f, i, t + 1, s.y);
+      if (c) note_match(f, i, t + 2, s.z);
+      if (d) note_match(f, i, t + 3, s.w);
     }
+  }
 }
 
-// One token in each block (a decode step): a warp per block, its first half K, its second half V.
-QB_DEVICE void store_single(const StoreParams& p, const Found& f, int head, const float (&kw)[8]) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & 15, which = lane >> 4;
-  const int blk = f.block[warp];
-  if (blk < 0) return;  // uniform across the warp; no barrier follows in here
-  const int row = p.slots[f.head[warp]] & (KV8_BLOCK - 1);
-  const int64_t t = f.row_src[warp][row];  // the later one where a slot is given twice
+// A token that is alone in its block (a decode step): a warp, its first half K, its second half V.  The
+// token's row, rotation and scale are on their way while the warp looks through the call's slots.  False
+// where the block takes other tokens of the call, too: nothing is stored then.
+QB_DEVICE bool store_alone(const StoreParams& p, int64_t t, int slot, int head, const float (&kw)[8], bool aligned) {
+  const int lane = threadIdx.x & 31, l = lane & 15, which = lane >> 4, blk = slot >> 6, row = slot & (KV8_BLOCK - 1);
   const int64_t at = ((int64_t)(blk / KV8_SUBS) * p.hkv + head) * KV8_SUBS + blk % KV8_SUBS;
   float* scale = p.scales[which] + at;
   uint8_t* block = p.codes[which] + at * KV8_TILE;
+  const Row8 raw = ld_row(p.qkv + t * p.ld + (p.hq + (which ? p.hkv : 0) + head) * KV8_D + l * 8);
   const float old = *scale;
   float v[8], y[8], c[8], s[8];
-  unpack_row(ld_row(p.qkv + t * p.ld + (p.hq + (which ? p.hkv : 0) + head) * KV8_D + l * 8), v);
   ld_rotation(p, checked_pos(p, t, false), l, c, s);
+  bool alone = true;
+  const int quads = aligned ? (int)(p.T / 4) : 0;
+#pragma unroll 4
+  for (int i = lane; i < quads; i += 32) {
+    const int4 o = reinterpret_cast<const int4*>(p.slots)[i];
+    const int n = (o.x >> 6 == blk) + (o.y >> 6 == blk) + (o.z >> 6 == blk) + (o.w >> 6 == blk);
+    alone = alone && n == (t >> 2 == i ? 1 : 0);
+  }
+  for (int i = 4 * quads + lane; i < (int)p.T; i += 32) alone = alone && (p.slots[i] >> 6 != blk || i == (int)t);
+  if (!__all_sync(0xffffffffu, alone)) return false;
+  unpack_row(raw, v);
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] = v[i];
   norm_rope(y, kw, c, s, p.eps, l);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = which ? v[i] : y[i];
   const bool anew = row == 0;
-  const float now = joined_scale(old, half_max(finite_max(v)), anew);
-  st_codes(block + row * KV8_D + l * 8, v, 1.f / now);
+  bool odd;
+  const float now = joined_scale(old, half_max(finite_max(v, odd)), anew);
+  st_codes(block + row * KV8_D + l * 8, v, 1.f / now, odd);
   if (l == 0) *scale = now;
-  if (!anew && now > old) round_again(block, f.row_src[warp], old / now, l, 16);
+  if (!anew && now > old) round_again(block, [row](int r) { return r != row; }, old / now, l, 16);
+  return true;
 }
 
-// A block that takes several tokens (a prompt chunk): 16 half-warps on 64 rows.
+// A block that takes several tokens (a prompt chunk): 32 half-warps on 64 rows.
 QB_DEVICE void store_many(const StoreParams& p, const Found& f, int i, int head, const float (&kw)[8], unsigned* top) {
   const int tid = threadIdx.x, lane = tid & 31, l = tid & 15, blk = f.block[i];
   __syncthreads();  // `top` of the block before has been read
@@ -234,6 +271,7 @@ QB_DEVICE void store_many(const StoreParams& p, const Found& f, int i, int head,
   float k[ST_ROWS][8];
   Row8 v[ST_ROWS];
   float top_k = 0.f, top_v = 0.f;
+  bool odd_k[ST_ROWS], odd_v[ST_ROWS];
 #pragma unroll
   for (int r = 0; r < ST_ROWS; ++r) {
     const int64_t t = f.row_src[i][(tid >> 4) + r * ST_HALVES];
@@ -249,8 +287,8 @@ QB_DEVICE void store_many(const StoreParams& p, const Found& f, int i, int head,
     norm_rope(k[r], kw, c, s, p.eps, l);
     float x[8];
     unpack_row(v[r], x);
-    top_k = fmaxf(top_k, t >= 0 ? finite_max(k[r]) : 0.f);
-    top_v = fmaxf(top_v, finite_max(x));
+    top_k = fmaxf(top_k, finite_max(k[r], odd_k[r]));  // a row not written is zero
+    top_v = fmaxf(top_v, finite_max(x, odd_v[r]));
   }
   top_k = warp_max(top_k);
   top_v = warp_max(top_v);
@@ -270,18 +308,19 @@ QB_DEVICE void store_many(const StoreParams& p, const Found& f, int i, int head,
     if (f.row_src[i][row] < 0) continue;
     float x[8];
     unpack_row(v[r], x);
-    st_codes(kb + row * KV8_D + l * 8, k[r], 1.f / now_k);
-    st_codes(vb + row * KV8_D + l * 8, x, 1.f / now_v);
+    st_codes(kb + row * KV8_D + l * 8, k[r], 1.f / now_k, odd_k[r]);
+    st_codes(vb + row * KV8_D + l * 8, x, 1.f / now_v, odd_v[r]);
   }
-  if (!anew && now_k > old_k) round_again(kb, f.row_src[i], old_k / now_k, tid, ST_THREADS);
-  if (!anew && now_v > old_v) round_again(vb, f.row_src[i], old_v / now_v, tid, ST_THREADS);
+  const auto kept = [&f, i](int r) { return f.row_src[i][r] < 0; };
+  if (!anew && now_k > old_k) round_again(kb, kept, old_k / now_k, tid, ST_THREADS);
+  if (!anew && now_v > old_v) round_again(vb, kept, old_v / now_v, tid, ST_THREADS);
   if (tid == 0) {
     p.scales[0][at] = now_k;
     p.scales[1][at] = now_v;
   }
 }
 
-__global__ void __launch_bounds__(ST_THREADS)
+__global__ void __launch_bounds__(ST_THREADS, 2)
 kv_fp8_store_kernel(StoreParams p) {
   qb_pdl_trigger();
   qb_pdl_wait();
@@ -292,26 +331,50 @@ kv_fp8_store_kernel(StoreParams p) {
     store_q(p, (int64_t)blockIdx.x - p.n_kv_ctas);
     return;
   }
+  const unsigned kv = blockIdx.x;
   const int tid = threadIdx.x, head_groups = (p.hkv + p.heads - 1) / p.heads;
-  const int head0 = (int)(blockIdx.x % head_groups) * p.heads, head1 = min(p.hkv, head0 + p.heads);
-  const int64_t t0 = (int64_t)(blockIdx.x / head_groups) * p.window;
+  const int head0 = (int)(kv % head_groups) * p.heads, head1 = min(p.hkv, head0 + p.heads);
+  const int64_t t0 = (int64_t)(kv / head_groups) * p.window;
+  const bool aligned = (reinterpret_cast<uintptr_t>(p.slots) & 15) == 0;
+  float kw[8];
+  unpack_row(ld_row(p.kw + (tid & 15) * 8), kw);
   if (tid == 0) n_heads = 0;
   __syncthreads();
-  if (tid < p.window && t0 + tid < p.T) {
-    const int64_t t = t0 + tid, slot = p.slots[t];
-    if (slot >= 0 && slot < p.num_slots) {
-      const int before = t > 0 ? p.slots[t - 1] : -1;
-      if (before >> 6 != (int)slot >> 6) heads[atomicAdd(&n_heads, 1)] = (int)t;
-    } else if (slot != -1 && head0 == 0) {
-      qb_set_err(p.err, QB_DEVERR_SLOT);
+  {
+    // short calls: a warp per token of the window (one head); long ones: a thread per token
+    const bool by_warp = p.window == ST_GROUP;  // (then one kv head)
+    const int64_t t = t0 + (by_warp ? tid >> 5 : tid);
+    if ((by_warp || tid < p.window) && t < p.T) {
+      const int slot = p.slots[t], before = t > 0 ? p.slots[t - 1] : -1;
+      const bool mine = !by_warp || (tid & 31) == 0;
+      if (slot >= 0 && slot < p.num_slots) {
+        if (before >> 6 != slot >> 6 && !(by_warp && store_alone(p, t, slot, head0, kw, aligned)) && mine)
+          heads[atomicAdd(&n_heads, 1)] = (int)t;
+      } else if (slot != -1 && head0 == 0 && mine) {
+        qb_set_err(p.err, QB_DEVERR_SLOT);
+      }
     }
   }
   __syncthreads();
-  const int n = n_heads;
+  int n = n_heads;
+  if (n > ST_ALONE_TRY) {
+    // a long call whose tokens lie in blocks of their own (a large decode batch): a warp per token after all
+    for (int i = tid >> 5; i < n; i += ST_WARPS) {
+      const int t = heads[i];
+      bool alone = true;
+      for (int head = head0; alone && head < head1; ++head) alone = store_alone(p, t, p.slots[t], head, kw, aligned);
+      if (alone && (tid & 31) == 0) heads[i] = -1;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      n_heads = 0;
+      for (int i = 0; i < n; ++i)
+        if (heads[i] >= 0) heads[n_heads++] = heads[i];
+    }
+    __syncthreads();
+    n = n_heads;
+  }
   if (n == 0) return;
-  float kw[8];
-  unpack_row(ld_row(p.kw + (tid & 15) * 8), kw);
-  const bool aligned = (reinterpret_cast<uintptr_t>(p.slots) & 15) == 0;
   for (int g0 = 0; g0 < n; g0 += ST_GROUP) {
     const int m = min(ST_GROUP, n - g0);
     __syncthreads();  // the group before is done
@@ -319,36 +382,21 @@ kv_fp8_store_kernel(StoreParams p) {
       f.head[tid] = tid < m ? heads[g0 + tid] : -1;
       f.block[tid] = tid < m ? p.slots[f.head[tid]] >> 6 : -1;
       f.first[tid] = INT32_MAX;
-      f.rows[tid] = 0;
     }
     for (int i = tid; i < ST_GROUP * KV8_BLOCK; i += ST_THREADS) (&f.row_src[0][0])[i] = -1;
     __syncthreads();
     // every token of the call in one of those blocks
-    const int64_t quads = aligned ? p.T / 4 : 0;
+    const int quads = aligned ? (int)(p.T / 4) : 0;
 #pragma unroll 4
-    for (int64_t t = tid; t < quads; t += ST_THREADS) {
-      const int4 s = reinterpret_cast<const int4*>(p.slots)[t];
-      note_token(f, m, (int)(4 * t), s.x);
-      note_token(f, m, (int)(4 * t + 1), s.y);
-      note_token(f, m, (int)(4 * t + 2), s.z);
-      note_token(f, m, (int)(4 * t + 3), s.w);
-    }
-    for (int64_t t = 4 * quads + tid; t < p.T; t += ST_THREADS) note_token(f, m, (int)t, p.slots[t]);
+    for (int t = tid; t < quads; t += ST_THREADS)
+      note_tokens(f, m, 4 * t, reinterpret_cast<const int4*>(p.slots)[t]);
+    for (int t = 4 * quads + tid; t < (int)p.T; t += ST_THREADS) note_token(f, m, t, p.slots[t]);
     __syncthreads();
-    bool many = false;
-    if (tid < ST_GROUP) {
-      if (f.block[tid] >= 0 && f.first[tid] != f.head[tid]) f.block[tid] = -1;  // another run head came first
-      many = f.block[tid] >= 0 && f.rows[tid] > 1;
-    }
-    many = __syncthreads_or(many);
-    for (int head = head0; head < head1; ++head) {
-      if (!many) {
-        store_single(p, f, head, kw);
-        continue;
-      }
-      for (int i = 0; i < m; ++i)
-        if (f.block[i] >= 0) store_many(p, f, i, head, kw, top);  // uniform across the CTA
-    }
+    if (tid < ST_GROUP && f.block[tid] >= 0 && f.first[tid] != f.head[tid]) f.block[tid] = -1;  // another run head came first
+    __syncthreads();
+    for (int i = 0; i < m; ++i)
+      if (f.block[i] >= 0)  // uniform across the CTA
+        for (int head = head0; head < head1; ++head) store_many(p, f, i, head, kw, top);
   }
 }
 
@@ -379,7 +427,7 @@ extern "C" int qb_qk_norm_rope_store_fp8(const void* qkv, int64_t T, int64_t ld_
   }
   const int64_t kv = (T + p.window - 1) / p.window * ((hkv + p.heads - 1) / p.heads);
   const int64_t q = (T * ((hq + ST_QH - 1) / ST_QH) + ST_HALVES - 1) / ST_HALVES;
-  QB_CHECK_ARG(T < INT32_MAX && kv + q <= INT32_MAX);
+  QB_CHECK_ARG(T <= INT32_MAX / hq && kv + q <= INT32_MAX);
   p.n_kv_ctas = kv;
   return qb_launch(kv_fp8_store_kernel, dim3((unsigned)(kv + q)), dim3(ST_THREADS), 0, (cudaStream_t)stream, 1, p);
 }
