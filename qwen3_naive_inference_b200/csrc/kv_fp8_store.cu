@@ -81,7 +81,8 @@ QB_DEVICE int64_t checked_pos(const StoreParams& p, int64_t t, bool tell) {
   if (tell) qb_set_err(p.err, QB_DEVERR_SHAPE);
   return 0;
 }
-// cos and sin of the eight rotation-table columns of lane l (columns j and j + 64 turn together)
+// cos and sin of the eight rotation-table columns of lane l (columns j and j + 64 turn together: lo c - hi s
+// in the lanes of the lower half, where s is given negated, hi c + lo s in those of the upper)
 QB_DEVICE void ld_rotation(const StoreParams& p, int64_t pos, int l, float (&c)[8], float (&s)[8]) {
   const float* row = p.cos_sin + pos * KV8_D + (l & 7) * 8;
 #pragma unroll
@@ -91,17 +92,25 @@ QB_DEVICE void ld_rotation(const StoreParams& p, int64_t pos, int l, float (&c)[
     c[4 * i] = a.x; c[4 * i + 1] = a.y; c[4 * i + 2] = a.z; c[4 * i + 3] = a.w;
     s[4 * i] = b.x; s[4 * i + 1] = b.y; s[4 * i + 2] = b.z; s[4 * i + 3] = b.w;
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[i] = l < 8 ? -s[i] : s[i];
 }
 // QK-norm and rotation of a head row spread over a half-warp (lane l: elements 8l..8l+7).  Every
 // lane of the warp takes part in the shuffles.
-QB_DEVICE void norm_rope(float (&v)[8], const float (&w)[8], const float (&c)[8], const float (&s)[8], float eps,
-                         int l) {
-  const float rstd = qk_rstd(half_sum(qk_sumsq8(v)), eps);
+QB_DEVICE void norm_rope(float (&v)[8], const float (&w)[8], const float (&c)[8], const float (&s)[8], float eps) {
+  float2 sq = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float x = v[i] * rstd * w[i];
-    const float partner = __shfl_xor_sync(0xffffffffu, x, 8);
-    v[i] = l < 8 ? qk_rope_lo(x, partner, c[i], s[i]) : qk_rope_hi(x, partner, c[i], s[i]);
+  for (int i = 0; i < 4; ++i) sq = fma2(make_float2(v[2 * i], v[2 * i + 1]), make_float2(v[2 * i], v[2 * i + 1]), sq);
+  const float rstd = qk_rstd(half_sum(sq.x + sq.y), eps);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = mul2(mul2(make_float2(v[2 * i], v[2 * i + 1]), make_float2(rstd, rstd)), make_float2(w[2 * i], w[2 * i + 1]));
+    float2 partner;
+    partner.x = __shfl_xor_sync(0xffffffffu, x.x, 8);
+    partner.y = __shfl_xor_sync(0xffffffffu, x.y, 8);
+    const float2 y = fma2(x, make_float2(c[2 * i], c[2 * i + 1]), mul2(partner, make_float2(s[2 * i], s[2 * i + 1])));
+    v[2 * i] = y.x;
+    v[2 * i + 1] = y.y;
   }
 }
 // Largest magnitude of a lane's values, as bits (they order as magnitudes do).  What is not finite is
@@ -130,7 +139,11 @@ QB_DEVICE float scale_for(float top) {
 }
 QB_DEVICE void st_codes(uint8_t* dst, float (&v)[8], float inv, bool odd) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] *= inv;
+  for (int i = 0; i < 4; ++i) {
+    const float2 y = mul2(make_float2(v[2 * i], v[2 * i + 1]), make_float2(inv, inv));
+    v[2 * i] = y.x;
+    v[2 * i + 1] = y.y;
+  }
   if (odd) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -182,7 +195,7 @@ QB_DEVICE void store_q(const StoreParams& p, int64_t cta) {
   for (int k = 0; k < ST_QH; ++k) {
     float v[8];
     unpack_row(raw[k], v);
-    norm_rope(v, w, c, s, p.eps, l);
+    norm_rope(v, w, c, s, p.eps);
     if (live && h0 + k < p.hq) {
       Row8 o;
 #pragma unroll
@@ -247,7 +260,7 @@ QB_DEVICE bool store_alone(const StoreParams& p, int64_t t, int slot, int head, 
   unpack_row(raw, v);
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] = v[i];
-  norm_rope(y, kw, c, s, p.eps, l);
+  norm_rope(y, kw, c, s, p.eps);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = which ? v[i] : y[i];
   const bool anew = row == 0;
@@ -284,7 +297,7 @@ QB_DEVICE void store_many(const StoreParams& p, const Found& f, int i, int head,
     const int64_t t = f.row_src[i][(tid >> 4) + r * ST_HALVES];
     float c[8], s[8];
     ld_rotation(p, t >= 0 ? checked_pos(p, t, false) : 0, l, c, s);
-    norm_rope(k[r], kw, c, s, p.eps, l);
+    norm_rope(k[r], kw, c, s, p.eps);
     float x[8];
     unpack_row(v[r], x);
     top_k = fmaxf(top_k, finite_max(k[r], odd_k[r]));  // a row not written is zero
