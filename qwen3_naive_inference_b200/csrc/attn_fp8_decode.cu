@@ -68,7 +68,7 @@ struct DecodeP {
 
 // What a CTA works on: `rows` query rows over keys [begin, end) of table row `table`.
 struct Work {
-  int rows, table, begin, end, slot;
+  int rows, table, begin, end, slot;  // slot: of the workspace, -1: straight to the output
 };
 
 QB_DEVICE void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -245,6 +245,16 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
     const int live = page_of[i] < 0 ? 0 : w.end - w.begin - i * KV8_BLOCK;  // keys of the tile that count
     if (live > 16 * warp) {
       const uint32_t kt = base + s * DC_STAGE_BYTES, vt = kt + KV8_TILE;
+      // V^T, asked for first: lane (g, t) holds elements 16g .. 16g+15 of keys 2t, 2t+1, 2t+8, 2t+9
+      uint4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int row = 16 * warp + 2 * t + (k & 1) + 8 * (k >> 1);
+        v[k] = lds128(vt + row * KV8_D + ((uint32_t)(g ^ ((2 * t + (k & 1)) & 7)) << 4));
+        if (live < KV8_BLOCK && row >= live) v[k] = make_uint4(0, 0, 0, 0);
+      }
+      const uint32_t vw[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
+                                 {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
       float x[NT][4];
       {  // scores of keys 16 warp + g and + 8
         float part[NT][2][4];
@@ -265,8 +275,9 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
           const uint32_t u0[4] = {k0[c].x, k0[c].y, k0[c].z, k0[c].w}, u1[4] = {k1[c].x, k1[c].y, k1[c].z, k1[c].w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t a[4] = {e4m3x2_to_half2(u0[k] & 0xffffu), e4m3x2_to_half2(u1[k] & 0xffffu),
-                                   e4m3x2_to_half2(u0[k] >> 16), e4m3x2_to_half2(u1[k] >> 16)};
+            uint32_t a[4];
+            e4m3x4_to_half2x2(u0[k], a[0], a[2]);
+            e4m3x4_to_half2x2(u1[k], a[1], a[3]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_f16_16816(part[nt][c], a, qf[nt][4 * c + k][0], qf[nt][4 * c + k][1]);
           }
@@ -281,6 +292,17 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
           x[nt][3] = in1 ? (part[nt][0][3] + part[nt][1][3]) * (fac[nt][1] * ks) : -INFINITY;
         }
       }
+      // V's fragments do not wait for the scores: they are made while those are on their way
+      uint32_t va[8][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t lo = __byte_perm(vw[0][k], vw[1][k], half ? 0x7362 : 0x5140);
+          const uint32_t hi = __byte_perm(vw[2][k], vw[3][k], half ? 0x7362 : 0x5140);
+          e4m3x4_to_half2x2(lo, va[2 * k + half][0], va[2 * k + half][1]);
+          e4m3x4_to_half2x2(hi, va[2 * k + half][2], va[2 * k + half][3]);
+        }
       bool far = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -317,34 +339,16 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
         pb[nt][0] = movmatrix_trans(pack_half2(p0, p1));
         pb[nt][1] = movmatrix_trans(pack_half2(p2, p3));
       }
-      // V^T: lane (g, t) holds elements 16g .. 16g+15 of keys 2t, 2t+1, 2t+8, 2t+9
-      uint4 v[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int row = 16 * warp + 2 * t + (k & 1) + 8 * (k >> 1);
-        v[k] = lds128(vt + row * KV8_D + ((uint32_t)(g ^ ((2 * t + (k & 1)) & 7)) << 4));
-        if (live < KV8_BLOCK && row >= live) v[k] = make_uint4(0, 0, 0, 0);
-      }
       const float vs = vs_of[i];
-      const uint32_t vw[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
-                                 {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 8; ++k)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t lo = __byte_perm(vw[0][k], vw[1][k], half ? 0x7362 : 0x5140);
-          const uint32_t hi = __byte_perm(vw[2][k], vw[3][k], half ? 0x7362 : 0x5140);
-          const uint32_t a[4] = {e4m3x2_to_half2(lo & 0xffffu), e4m3x2_to_half2(lo >> 16),
-                                 e4m3x2_to_half2(hi & 0xffffu), e4m3x2_to_half2(hi >> 16)};
+        for (int nt = 0; nt < NT; ++nt) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_f16_16816(d, va[k], pb[nt][0], pb[nt][1]);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_f16_16816(d, a, pb[nt][0], pb[nt][1]);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[nt][2 * k + half][c] = fmaf(vs, d[c], o[nt][2 * k + half][c]);
-          }
+          for (int c = 0; c < 4; ++c) o[nt][k][c] = fmaf(vs, d[c], o[nt][k][c]);
         }
-      }
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(empty(s));
@@ -391,7 +395,7 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
     if (seq < 0) continue;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const int64_t row = (int64_t)seq * p.hq + kvh * group + r % group;
-    if (p.n_slots == 1) {
+    if (w.slot < 0) {
       uint2 u;
       u.x = pack_bf16x2(acc.x * inv, acc.y * inv);
       u.y = pack_bf16x2(acc.z * inv, acc.w * inv);
@@ -492,7 +496,8 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   w.table = b;
   w.begin = (int)min(begin, (int64_t)max(len, 0));
   w.end = (int)min((int64_t)max(len, 0), begin + p.own_tokens);
-  w.slot = (NTS > 0 ? p.shared_splits : 0) + split;
+  // a sequence whose keys are all here has nothing to join
+  w.slot = NTS == 0 && split == 0 && w.end == len ? -1 : (NTS > 0 ? p.shared_splits : 0) + split;
   if (w.begin >= w.end) {
     if (p.n_slots == 1)  // no keys at all
       for (int k = threadIdx.x; k < group * KV8_D / 4; k += DC_THREADS)
@@ -526,6 +531,7 @@ decode_fp8_join_kernel(DecodeP p) {
     }
   }
   const int own0 = p.members ? p.shared_splits : 0, n = member ? n_shared + own_live(p, b) : 0;
+  if (!p.members && n == 1) return;  // its only CTA has written the output
   const float* ws = p.ws + ((int64_t)b * p.hq + h) * p.n_slots * DC_WS_ROW;
   auto slot = [&](int s) { return ws + (int64_t)(s < n_shared ? s : own0 + s - n_shared) * DC_WS_ROW; };
   float m = -INFINITY;

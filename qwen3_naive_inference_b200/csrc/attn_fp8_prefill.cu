@@ -142,10 +142,7 @@ QB_DEVICE void put_codes(uint32_t tile, int r, int c, const uint4& u) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
   uint32_t h[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    h[2 * i] = e4m3x2_to_half2(w[i] & 0xffffu);
-    h[2 * i + 1] = e4m3x2_to_half2(w[i] >> 16);
-  }
+  for (int i = 0; i < 4; ++i) e4m3x4_to_half2x2(w[i], h[2 * i], h[2 * i + 1]);
   const uint32_t at = tile + operand_chunk(r, 2 * c, PF_KV_HALF);
   st_shared16(at, h[0], h[1], h[2], h[3]);
   st_shared16(at ^ 16u, h[4], h[5], h[6], h[7]);

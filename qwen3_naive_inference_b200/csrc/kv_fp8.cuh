@@ -18,15 +18,18 @@ constexpr int KV8_BLOCK = 64;   // tokens that share a scale
 constexpr int KV8_SUBS = KV8_PAGE / KV8_BLOCK;
 constexpr int KV8_TILE = KV8_BLOCK * KV8_D;  // bytes of one block's codes of one head
 
-// Two e4m3 codes (the low 16 bits) as two halves: exact, every code is a half value (NaN stays NaN).
-QB_DEVICE uint32_t e4m3x2_to_half2(uint32_t codes) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 lo;\n\tcvt.u16.u32 lo, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(codes));
-  return r;
+// Four e4m3 codes as halves, two to a word: exact, every code is a half value (NaN stays NaN).
+QB_DEVICE void e4m3x4_to_half2x2(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(codes));
 }
-QB_DEVICE float2 e4m3x2_to_float2(uint32_t codes) {
-  const uint32_t h = e4m3x2_to_half2(codes);
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+QB_DEVICE void e4m3x4_to_float4(uint32_t codes, float (&f)[4]) {
+  uint32_t lo, hi;
+  e4m3x4_to_half2x2(codes, lo, hi);
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
 }
 // Four values as e4m3 codes, round to nearest even; beyond +-448 saturates, NaN stays NaN.
 QB_DEVICE uint32_t float4_to_e4m3x4(float a, float b, float c, float d) {

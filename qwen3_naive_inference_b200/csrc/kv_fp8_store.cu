@@ -165,8 +165,9 @@ QB_DEVICE void round_again(uint8_t* block, F kept, float ratio, int i, int n) {
     uint32_t* w = reinterpret_cast<uint32_t*>(&u);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float2 a = e4m3x2_to_float2(w[k] & 0xffffu), b = e4m3x2_to_float2(w[k] >> 16);
-      w[k] = float4_to_e4m3x4(a.x * ratio, a.y * ratio, b.x * ratio, b.y * ratio);
+      float f[4];
+      e4m3x4_to_float4(w[k], f);
+      w[k] = float4_to_e4m3x4(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
     }
     *at = u;
   }
