@@ -9,7 +9,7 @@
 // R % group, so the group's heads share every key -- as two tiles of 128 rows, A and B, and walks the
 // keys a block of 64 at a time:
 //   warps 0-3, 4-7  softmax of tile A, of tile B: a thread per row
-//   warps 8-11      convert: codes come from global memory a block ahead, become halves (exactly) and go
+//   warps 8-11      convert: codes come from global memory two blocks ahead, become halves (exactly) and go
 //                   to shared memory in the swizzled layout of the MMA operands (rings of four blocks)
 //   warps 12, 13    issue S_A, S_B = Q_x K^T (both operands in shared memory)
 //   warps 14, 15    issue O_A, O_B += P_x V (P_x from TMEM, over the columns of its S_x); each of the four
@@ -157,21 +157,29 @@ QB_DEVICE void prefill_convert(const PrefillP& p, const PrefillSmem& sm, const P
   // one element half of two neighbouring keys
   const int chunk = (tid & 3) | ((tid >> 1) & 4), row0 = ((tid >> 4) << 1) | ((tid >> 2) & 1);
   const int first_masked = w.shift + w.q0 + 1;  // keys from here on are behind the first row's last one
-  // Codes of a key tile in registers (rows past the keys and tiles without a page: zero), and, in thread
-  // 0, its scales.
-  uint4 kr[4], vr[4];
-  float ks = -1.f, vs = 0.f, vref = 0.f;
-  int64_t at = -1;  // (page, head, block) of the tile that is loaded
-  auto find = [&](int j) {
-    const int key = w.begin + j * PF_KEYS, col = key / KV8_PAGE;
-    const int page = col < p.bt_width ? p.bt[(int64_t)w.b * p.bt_stride + col] : -1;
-    at = -1;
-    if (page >= 0 && page < p.num_blocks)
-      at = ((int64_t)page * p.hkv + w.kvh) * KV8_SUBS + key % KV8_PAGE / KV8_BLOCK;
-    else if (tid == 0)
-      qb_set_err(p.err, QB_DEVERR_PAGE);
+  float vref = 0.f;  // thread 0
+  // A key tile on its way: its codes in registers (rows past the keys and tiles without a page: zero) and, in
+  // thread 0, its scales.  Two tiles are, so that a tile's loads have the time of two to arrive; the page of
+  // the one after them is looked up meanwhile.
+  struct Coming {
+    uint4 k[4], v[4];
+    int64_t at;  // (page, head, block), -1: no page
+    float ks, vs;
   };
-  auto load = [&](const uint8_t* codes, uint4 (&r)[4], int j) {
+  auto page_of = [&](int j) {
+    const int col = (w.begin + j * PF_KEYS) / KV8_PAGE;
+    return j < n && col < p.bt_width ? p.bt[(int64_t)w.b * p.bt_stride + col] : -1;
+  };
+  auto find = [&](Coming& c, int j, int page) {
+    c.at = -1;
+    if (page >= 0 && page < p.num_blocks)
+      c.at = ((int64_t)page * p.hkv + w.kvh) * KV8_SUBS + (w.begin + j * PF_KEYS) % KV8_PAGE / KV8_BLOCK;
+    else if (j < n && tid == 0)
+      qb_set_err(p.err, QB_DEVERR_PAGE);
+    c.ks = tid == 0 && c.at >= 0 ? p.ks[c.at] : -1.f;
+    c.vs = tid == 0 && c.at >= 0 ? p.vs[c.at] : 0.f;
+  };
+  auto load = [&](const uint8_t* codes, uint4 (&r)[4], int64_t at, int j) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int key = row0 + 16 * i;
@@ -180,62 +188,67 @@ QB_DEVICE void prefill_convert(const PrefillP& p, const PrefillSmem& sm, const P
         r[i] = *reinterpret_cast<const uint4*>(codes + at * KV8_TILE + key * KV8_D + chunk * 16);
     }
   };
-  auto load_scales = [&]() {
-    if (tid != 0) return;
-    ks = at >= 0 ? p.ks[at] : -1.f;
-    vs = at >= 0 ? p.vs[at] : 0.f;
-  };
-  find(0);
-  load(p.k, kr, 0);
-  load_scales();
-  load(p.v, vr, 0);
-  for (int j = 0; j < n; ++j) {
-    if (j + 1 < n) find(j + 1);
-    if (!mbar_wait(sm.k_empty(j), sm.phase(j) ^ 1, sm.abort_flag(), p.err)) return;
+  int page = -1;  // of the tile after the two
+  auto take = [&](Coming& c, int j) {
+    const int later = page_of(j + 3);
+    if (!mbar_wait(sm.k_empty(j), sm.phase(j) ^ 1, sm.abort_flag(), p.err)) return false;
     if (tid == 0) {
       float* sc = sm.scales(j);
       sc[4] = 1.f;
-      if (vs > vref * PF_VSLACK) {
-        sc[4] = vref / vs;
-        vref = vs;
+      if (c.vs > vref * PF_VSLACK) {
+        sc[4] = vref / c.vs;
+        vref = c.vs;
       }
-      const float rv = vref > 0.f ? vs / vref : 0.f;
+      const float rv = vref > 0.f ? c.vs / vref : 0.f;
       const bool folded = rv >= PF_VLOW;
-      sc[0] = ks;
+      sc[0] = c.ks;
       sc[1] = folded ? log2f(rv) : 0.f;
       sc[2] = folded ? 1.f / rv : 1.f;
       sc[3] = folded ? 1.f : rv;
       sc[5] = vref;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) put_codes(sm.k(j), row0 + 16 * i, chunk, kr[i]);
-    if (j + 1 < n) {
-      load(p.k, kr, j + 1);
-      load_scales();
-    }
+    for (int i = 0; i < 4; ++i) put_codes(sm.k(j), row0 + 16 * i, chunk, c.k[i]);
     fence_async_shared();
     mbar_arrive(sm.k_full(j));
-    if (!mbar_wait(sm.v_empty(j), sm.phase(j) ^ 1, sm.abort_flag(), p.err)) return;
+    find(c, j + 2, page);
+    load(p.k, c.k, c.at, j + 2);
+    if (!mbar_wait(sm.v_empty(j), sm.phase(j) ^ 1, sm.abort_flag(), p.err)) return false;
     if (w.begin + (j + 1) * PF_KEYS > first_masked) {
       // some row sees this tile in part: no NaN may reach the product of a masked key
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t bad[4] = {nan_bytes(vr[i].x), nan_bytes(vr[i].y), nan_bytes(vr[i].z), nan_bytes(vr[i].w)};
+        const uint32_t bad[4] = {nan_bytes(c.v[i].x), nan_bytes(c.v[i].y), nan_bytes(c.v[i].z), nan_bytes(c.v[i].w)};
         if (bad[0] | bad[1] | bad[2] | bad[3]) {
-          vr[i].x &= ~((bad[0] >> 7) * 0xffu);
-          vr[i].y &= ~((bad[1] >> 7) * 0xffu);
-          vr[i].z &= ~((bad[2] >> 7) * 0xffu);
-          vr[i].w &= ~((bad[3] >> 7) * 0xffu);
+          c.v[i].x &= ~((bad[0] >> 7) * 0xffu);
+          c.v[i].y &= ~((bad[1] >> 7) * 0xffu);
+          c.v[i].z &= ~((bad[2] >> 7) * 0xffu);
+          c.v[i].w &= ~((bad[3] >> 7) * 0xffu);
           const int key = row0 + 16 * i;
           atomicOr(&sm.nan_keys(j)[key >> 5], 1u << (key & 31));
         }
       }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) put_codes(sm.v(j), row0 + 16 * i, chunk, vr[i]);
-    if (j + 1 < n) load(p.v, vr, j + 1);
+    for (int i = 0; i < 4; ++i) put_codes(sm.v(j), row0 + 16 * i, chunk, c.v[i]);
     fence_async_shared();
     mbar_arrive(sm.v_full(j));
+    load(p.v, c.v, c.at, j + 2);
+    page = later;
+    return true;
+  };
+  Coming a, b;
+  const int page0 = page_of(0), page1 = page_of(1);
+  page = page_of(2);
+  find(a, 0, page0);
+  load(p.k, a.k, a.at, 0);
+  find(b, 1, page1);
+  load(p.v, a.v, a.at, 0);
+  load(p.k, b.k, b.at, 1);
+  load(p.v, b.v, b.at, 1);
+  for (int j = 0; j < n; j += 2) {
+    if (!take(a, j)) return;
+    if (j + 1 < n && !take(b, j + 1)) return;
   }
 }
 
@@ -308,13 +321,19 @@ QB_DEVICE void prefill_issue(const PrefillP& p, const PrefillSmem& sm, const Pre
 // Query tile x into shared memory as halves: a half-warp per row, 16 rows each.
 QB_DEVICE void prefill_load_q(const PrefillP& p, const PrefillSmem& sm, const PrefillWork& w, int x) {
   const int tid = threadIdx.x & 127, l = tid & 15, group = p.hq / p.hkv;
-#pragma unroll 4
+  uint4 rows[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int R = x * PF_ROWS + (tid >> 4) + 8 * i;
+    rows[i] = make_uint4(0, 0, 0, 0);
+    if (R < w.rows)
+      rows[i] = *reinterpret_cast<const uint4*>(p.q + (w.row0 + w.q0 + R / group) * p.q_stride +
+                                                (w.kvh * group + R % group) * KV8_D + l * 8);
+  }
+#pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int r = (tid >> 4) + 8 * i, R = x * PF_ROWS + r;
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (R < w.rows)
-      u = *reinterpret_cast<const uint4*>(p.q + (w.row0 + w.q0 + R / group) * p.q_stride +
-                                          (w.kvh * group + R % group) * KV8_D + l * 8);
+    const uint4 u = rows[i];
     const uint32_t raw[4] = {u.x, u.y, u.z, u.w};
     float f[8], top = 0.f;
 #pragma unroll
@@ -485,10 +504,11 @@ prefill_fp8_kernel(PrefillP p) {
   extern __shared__ uint8_t smem_raw[];
   PrefillWork w;
   const int group = p.hq / p.hkv, subs = p.unit / p.pos_per_cta;
-  const int tile = blockIdx.x / subs, sub = blockIdx.x % subs, split = blockIdx.z;
+  // the last tiles of the sequences, which see the most keys, begin first
+  const int rank = gridDim.x - 1 - blockIdx.x, tile = rank / subs, sub = rank % subs, split = blockIdx.z;
   w.kvh = blockIdx.y;
-  w.b = p.tiles ? p.tiles[2 * tile] : tile / p.tiles_per_seq;
-  const int start = p.tiles ? p.tiles[2 * tile + 1] : tile % p.tiles_per_seq * p.unit;
+  w.b = p.tiles ? p.tiles[2 * tile] : tile % p.batch;
+  const int start = p.tiles ? p.tiles[2 * tile + 1] : tile / p.batch * p.unit;
   if (w.b < 0 || w.b >= p.batch || start < 0 || start % p.unit != 0) {
     // a 64-row tile whose rows belong to the CTA of an earlier one
     if ((w.b < 0 || w.b >= p.batch || start < 0) && threadIdx.x == 0) qb_set_err(p.err, QB_DEVERR_SHAPE);
