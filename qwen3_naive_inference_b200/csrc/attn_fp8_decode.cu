@@ -631,7 +631,10 @@ extern "C" int qb_paged_decode_attn_grouped_fp8(
   p.ws = workspace; p.out = (bf16*)out; p.err = err;
   p.members = group_members; p.shared_len = shared_len; p.kv_start = kv_start; p.n_groups = n_groups;
   p.shared_tokens = shared_tokens; p.shared_splits = shared_splits;
-  const int group = hq / hkv, row_tiles = group == 1 ? 1 : 2;
+  // Eight query rows a CTA where they are enough for a member: with 16, a group's shared keys were read
+  // once instead of twice (the second time from L2), but a CTA's registers spilled and its sixteen rows took
+  // longer to join (64 groups of 8: 102 us against 107, five small groups 11.6 against 16.3).
+  const int group = hq / hkv, row_tiles = group <= 8 ? 1 : 2;
   p.chunk = min(8, row_tiles * 8 / group);
   p.n_chunks = (8 + p.chunk - 1) / p.chunk;
   p.group_step = min(group_step, n_groups);
@@ -640,9 +643,7 @@ extern "C" int qb_paged_decode_attn_grouped_fp8(
   QB_CHECK_ARG(shared <= INT32_MAX);
   p.n_shared = (unsigned)shared;
   const cudaStream_t st = (cudaStream_t)stream;
-  if (group == 1) return launch_decode<1, 1>(tk, tv, p, st);
-  if (group <= 8) return launch_decode<2, 1>(tk, tv, p, st);
-  return launch_decode<2, 2>(tk, tv, p, st);
+  return row_tiles == 1 ? launch_decode<1, 1>(tk, tv, p, st) : launch_decode<2, 2>(tk, tv, p, st);
 }
 
 extern "C" size_t qb_paged_decode_fp8_workspace_bytes(int batch, int hq, int n_slots) {
