@@ -370,7 +370,16 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
   const uint32_t o_at = lanes + PF_COL_O + x * 128;
   const bool live = R < w.rows;
   const int pos = w.q0 + R / group;
-  const int last = live ? min(w.shift + pos, w.end - 1) : w.begin - 1;  // the row's last key here
+  // the row's last key here (rows behind the work's last do not hold the warp to the masked path)
+  const int last = live ? min(w.shift + pos, w.end - 1) : w.end - 1;
+  if (ok && __all_sync(0xffffffffu, !live)) {
+    // nothing to weigh: what stands in these lanes of TMEM meets their own rows of O only
+    for (int j = 0; ok && j < n; ++j) {
+      ok = __all_sync(0xffffffffu, mbar_wait(sm.s_full(x, j), sm.buffer_phase(j), ab, p.err)) != 0;
+      if (ok) mbar_arrive(sm.p_ready(x, j));
+    }
+    return;
+  }
   float ref = -INFINITY, l = 0.f, vref = 0.f;
   for (int j = 0; ok && j < n; ++j) {
     // tcgen05 loads and stores are warp-collective: every decision that leads to them is warp-uniform
