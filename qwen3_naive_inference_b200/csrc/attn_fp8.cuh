@@ -1,5 +1,7 @@
 // Host side shared by the attentions over the 8-bit paged KV cache: argument checks, tensor maps.
 #pragma once
+#include <atomic>
+
 #include "kv_fp8.cuh"
 #include "tma.cuh"
 
@@ -7,6 +9,19 @@ namespace {
 
 constexpr float KV8_LOG2E = 1.4426950408889634f;
 constexpr int KV8_MAX_GROUP = 16;  // query heads of a kv head
+
+// Lets kernel `fn` have `bytes` of dynamic shared memory on the current device; `done` holds a bit per
+// device that it was asked for on.
+int kv8_allow_smem(const void* fn, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return qb_launch_status();
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return QB_OK;
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return qb_launch_status();
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return QB_OK;
+}
 
 int kv8_check_cache(const void* q, int64_t q_stride, const void* k, const void* v, const float* ks, const float* vs,
                     int64_t num_blocks, const int32_t* bt, int64_t bt_stride, int bt_width, int hq, int hkv,

@@ -556,13 +556,9 @@ decode_fp8_join_kernel(DecodeP p) {
 
 template <int NTS, int NTO>
 int launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeP& p, cudaStream_t st) {
-  static bool attr = false;
-  if (!attr) {
-    if (cudaFuncSetAttribute(decode_fp8_kernel<NTS, NTO>, cudaFuncAttributeMaxDynamicSharedMemorySize, DC_SMEM) !=
-        cudaSuccess)
-      return qb_launch_status();
-    attr = true;
-  }
+  static std::atomic<uint64_t> allowed{0};
+  const int may = kv8_allow_smem(reinterpret_cast<const void*>(decode_fp8_kernel<NTS, NTO>), DC_SMEM, allowed);
+  if (may != QB_OK) return may;
   const int64_t ctas = p.n_shared + (int64_t)p.batch * p.hkv * p.own_splits, rows = (int64_t)p.batch * p.hq;
   if (ctas > INT32_MAX || rows > INT32_MAX) return QB_ERR_INVALID;
   const int rc = qb_launch_ex(decode_fp8_kernel<NTS, NTO>, dim3((unsigned)ctas), dim3(DC_THREADS), DC_SMEM, st, 1, true, tk,

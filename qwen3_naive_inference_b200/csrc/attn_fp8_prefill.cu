@@ -677,12 +677,9 @@ extern "C" int qb_attn_paged_prefill_fp8(const void* q, int64_t q_stride, const 
   const int64_t grid = (tile_info ? (int64_t)n_tiles : (int64_t)batch * p.tiles_per_seq) * (p.unit / p.pos_per_cta);
   QB_CHECK_ARG(grid <= INT32_MAX);
   if (grid == 0) return QB_OK;
-  static bool attr = false;
-  if (!attr) {
-    if (cudaFuncSetAttribute(prefill_fp8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PF_SMEM) != cudaSuccess)
-      return qb_launch_status();
-    attr = true;
-  }
+  static std::atomic<uint64_t> allowed{0};
+  const int may = kv8_allow_smem(reinterpret_cast<const void*>(prefill_fp8_kernel), PF_SMEM, allowed);
+  if (may != QB_OK) return may;
   const cudaStream_t st = (cudaStream_t)stream;
   const int rc = qb_launch_ex(prefill_fp8_kernel, dim3((unsigned)grid, (unsigned)hkv, (unsigned)n_splits), dim3(PF_THREADS),
                               PF_SMEM, st, 1, true, p);

@@ -651,6 +651,8 @@ class Qwen3ForCausalLM(nn.Module):
         [layers, num_blocks, kv_heads, 4] fp32."""
         a0 = self.model.layers[0].self_attn
         fp8 = self._kv_fp8()
+        if fp8 and a0.head_dim != 128:
+            raise ValueError(f"an 8-bit K/V cache needs heads of 128 elements, not {a0.head_dim}")
         if not self._num_blocks:
             self._num_blocks = self._compute_num_blocks()
         if fp8:

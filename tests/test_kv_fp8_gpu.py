@@ -226,6 +226,41 @@ def test_decode_large_queries(cuda):
             check_attention(pre[0, h:h + 1], *ref)
 
 
+@pytest.mark.parametrize("scale", [-0.07, 0.0])
+def test_scales_that_are_not_positive(cuda, scale):
+    """A negative softmax scale turns the order of the scores, a scale of zero gives the mean of V."""
+    g = gen(9)
+    k, v, ks, vs = random_cache(g, 2, 2)
+    table = torch.tensor([[1, 0]], dtype=torch.int32)
+    q = torch.randn(140, 8, D, generator=g).to(BF)
+    args = on(cuda, q, k, v, ks, vs, table)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    dec = ops.paged_decode_attention_fp8(args[0][:1], *args[1:], i32(449), scale)
+    pre = ops.attention_paged_prefill_fp8(*args[:5], i32(0, 140), i32(0, 500), 140, args[5], scale)
+    k64, v64 = values(k, ks), values(v, vs)
+    for h in range(8):
+        kv = [rows_of(c, table[0], 0, 500, h // 4) for c in (k64, v64)]
+        check_attention(pre[:, h], *attend(q[:, h], [kv], scale, 360))
+        check_attention(dec[:, h], *attend(q[:1, h], [[c[:450] for c in kv]], scale))
+
+
+def test_values_that_are_not_finite_in_queries(cuda):
+    """NaN and infinities in one row's queries stay in that row."""
+    g = gen(10)
+    k, v, ks, vs = random_cache(g, 2, 2)
+    table = torch.tensor([[1, 0]] * 3, dtype=torch.int32)
+    q = torch.randn(3, 4, D, generator=g).to(BF)
+    bad = q.clone()
+    bad[1, 2, 5], bad[1, 3, 0] = math.nan, math.inf
+    args = on(cuda, k, v, ks, vs, table, torch.tensor([300, 299, 100], dtype=torch.int32))
+    a, b = (ops.paged_decode_attention_fp8(x.to(cuda), *args, 0.1) for x in (q, bad))
+    assert bool(b[1, 2].isnan().all()) and torch.equal(a[[0, 2]], b[[0, 2]]) and torch.equal(a[1, :2], b[1, :2])
+    cu = torch.tensor([0, 3], dtype=torch.int32, device=cuda)
+    ck = torch.tensor([0, 400], dtype=torch.int32, device=cuda)
+    a, b = (ops.attention_paged_prefill_fp8(x.to(cuda), *args[:4], cu, ck, 3, args[4][:1].contiguous(), 0.1) for x in (q, bad))
+    assert bool(b[1, 2].isnan().all()) and torch.equal(a[[0, 2]], b[[0, 2]]) and torch.equal(a[1, :2], b[1, :2])
+
+
 # ------------------------------------------------------------------------------------------ grouped
 GROUPED = [
     # hq, hkv, per group: shared keys, own keys of each member
@@ -753,6 +788,11 @@ def test_refusals(cuda):
         with pytest.raises(ops.NativeError):
             f()
             pytest.fail(f"call {i} was taken")
+    # tensors of another device than the current one (as seen where the current one is asked for)
+    with pytest.MonkeyPatch.context() as mp:
+        mp.setattr(torch.cuda, "current_device", lambda: 1)
+        with pytest.raises(ops.NativeError, match="current CUDA device"):
+            dec(q, k, v, ks, vs, t, n, 0.1)
     # nothing to do is taken: no rows, no tokens
     e = torch.empty(0, 4, D, dtype=BF, device=cuda)
     assert dec(e, k, v, ks, vs, t[:0], n[:0], 0.1, max_ctx=1).shape == (0, 4, D)
