@@ -496,8 +496,8 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   w.table = b;
   w.begin = (int)min(begin, (int64_t)max(len, 0));
   w.end = (int)min((int64_t)max(len, 0), begin + p.own_tokens);
-  // a sequence whose keys are all here has nothing to join
-  w.slot = NTS == 0 && split == 0 && w.end == len ? -1 : (NTS > 0 ? p.shared_splits : 0) + split;
+  // a sequence whose keys are all here has nothing to join; with one slot there is no workspace
+  w.slot = NTS == 0 && (p.n_slots == 1 || (split == 0 && w.end == len)) ? -1 : (NTS > 0 ? p.shared_splits : 0) + split;
   if (w.begin >= w.end) {
     if (p.n_slots == 1)  // no keys at all
       for (int k = threadIdx.x; k < group * KV8_D / 4; k += DC_THREADS)

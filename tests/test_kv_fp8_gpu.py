@@ -177,6 +177,27 @@ def test_decode_bad_pages_are_reported(cuda):
     ops.check_device_errors()
 
 
+@pytest.mark.parametrize("keys,max_ctx", [(1000, 512), (3000, 2000)])
+def test_decode_keys_beyond_max_ctx_are_reported(cuda, keys, max_ctx):
+    """A sequence longer than max_ctx, in one split (which has no workspace) and in several: reported, the
+    output that of the keys the plan covers; its neighbours are not touched by it."""
+    g = gen(11)
+    k, v, ks, vs = random_cache(g, 14, 2)
+    table = paged(g, [keys, 70], 14)
+    q = torch.randn(2, 4, D, generator=g).to(BF)
+    split, n = ops.decode_split_plan_fp8(2, 2, max_ctx)
+    assert (n == 1) == (max_ctx <= 768) and split * n < keys
+    args = on(cuda, q, k, v, ks, vs, table, torch.tensor([keys, 70], dtype=torch.int32))
+    out = ops.paged_decode_attention_fp8(*args, 0.1, seqlen_add=0, max_ctx=max_ctx)
+    with pytest.raises(ops.NativeError, match="inconsistent"):
+        ops.check_device_errors()
+    k64, v64 = values(k, ks), values(v, vs)
+    for b, seen in enumerate((split * n, 70)):
+        for h in range(4):
+            kv = [rows_of(c, table[b], 0, seen, h // 2) for c in (k64, v64)]
+            check_attention(out[b, h:h + 1], *attend(q[b, h:h + 1], [kv], 0.1), f"row {b} head {h}")
+
+
 def test_decode_scales_far_apart(cuda):
     """Blocks whose scales differ by 2^60, and whose values are zero under the smallest scale: each block's
     share counts whatever its neighbours hold."""
