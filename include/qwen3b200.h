@@ -235,8 +235,8 @@ int qb_paged_decode_attn_fp8(const void* q, int64_t q_stride, const void* k_cach
  * seqlens[b] + seqlen_add - kv_start[b].  Sequences in no group get zeros; kv_start is a multiple of 64;
  * entries of group_members that name no sequence set QB_DEVERR_SHAPE.  The CTAs of the shared keys take
  * groups g, g + group_step, ... one after another: the number of live groups expected (a table captured
- * for any grouping may have many empty entries behind them, which then cost no CTAs), or n_groups.  A sequence is in one group at
- * most.  workspace: qb_paged_decode_grouped_fp8_workspace_bytes(batch, hq, shared_splits + own_splits),
+ * for any grouping may have many empty entries behind them, which then cost no CTAs), or n_groups.  A sequence
+ * is in one group at most.  With n_groups = 0 nothing is written.  workspace: qb_paged_decode_grouped_fp8_workspace_bytes(batch, hq, shared_splits + own_splits),
  * any contents. */
 int qb_paged_decode_attn_grouped_fp8(const void* q, int64_t q_stride, const void* k_cache,
                                      const void* v_cache, const float* k_scale, const float* v_scale,
@@ -252,7 +252,8 @@ size_t qb_paged_decode_grouped_fp8_workspace_bytes(int batch, int hq, int n_slot
 /* Causal attention of the query rows cu_seqlens_q over the first cu_seqlens_k keys of each sequence in
  * that cache; arguments as the paged form of qb_attn_varlen_fwd.  q and out rows q_stride / o_stride
  * elements apart (multiples of 8).  hq / hkv <= 16.  Rows in no sequence are left as they were.
- * tile_info has to hold every 64-row tile of a sequence.  With n_splits > 1 the keys are split over
+ * tile_info has to hold every 64-row tile of a sequence; without it tiles_per_seq * 64 >= every Lq (rows
+ * beyond are left as they were and set QB_DEVERR_SHAPE).  With n_splits > 1 the keys are split over
  * CTAs, split_keys (a multiple of 128) each, and joined by a second kernel; split_keys * n_splits >=
  * every Lk (keys beyond are left out and set QB_DEVERR_SHAPE); workspace:
  * qb_attn_paged_prefill_fp8_workspace_bytes(total_q, hq, n_splits), any contents. */

@@ -30,6 +30,8 @@
 // Every wait is bounded (~2 s): on timeout QB_DEVERR_TIMEOUT is raised, all roles leave, TMEM is freed.
 #include <float.h>
 
+#include <algorithm>
+
 #include "attn_fp8.cuh"
 #include "tcgen05.cuh"
 
@@ -66,6 +68,7 @@ struct PrefillP {
   const int32_t* bt;
   int64_t bt_stride;
   int bt_width;
+  int table_keys;        // that a row of the table can name
   const int32_t* cu_q;
   const int32_t* cu_k;
   int batch;
@@ -528,6 +531,8 @@ prefill_fp8_kernel(PrefillP p) {
   const int lk = p.cu_k[w.b + 1] - p.cu_k[w.b];
   w.q0 = start + sub * p.pos_per_cta;
   if (w.q0 >= w.lq) return;
+  if (!p.tiles && w.q0 == 0 && w.lq / p.unit > p.tiles_per_seq - (w.lq % p.unit != 0) && threadIdx.x == 0)
+    qb_set_err(p.err, QB_DEVERR_SHAPE);  // queries past the last tile
   if (lk < w.lq || w.row0 < 0 || w.row0 + w.lq > p.total_q) {
     if (threadIdx.x == 0) qb_set_err(p.err, QB_DEVERR_SHAPE);
     return;
@@ -539,6 +544,10 @@ prefill_fp8_kernel(PrefillP p) {
   w.end = min(w.shift + w.q0 + positions, p.n_splits > 1 ? w.begin + p.split_keys : INT32_MAX);
   if (p.n_splits > 1 && split == p.n_splits - 1 && w.end < w.shift + w.q0 + positions && threadIdx.x == 0)
     qb_set_err(p.err, QB_DEVERR_SHAPE);  // keys past the last split
+  if (w.end > p.table_keys) {  // such keys are left out
+    if (threadIdx.x == 0) qb_set_err(p.err, QB_DEVERR_PAGE);
+    w.end = p.table_keys;
+  }
   if (w.begin >= w.end) return;  // uniform across the CTA, before any barrier or TMEM exists
   const int rows_a = min(w.rows, PF_ROWS);
   const int end_a = min(w.end, w.shift + w.q0 + (rows_a - 1) / group + 1);  // tile A's last row's keys
@@ -616,8 +625,8 @@ prefill_fp8_join_kernel(PrefillP p) {
     else hi = mid;
   }
   const int lq = p.cu_q[lo + 1] - p.cu_q[lo], lk = p.cu_k[lo + 1] - p.cu_k[lo], i = (int)row - p.cu_q[lo];
-  if (i < 0 || i >= lq || lk < lq || p.cu_q[lo + 1] > p.total_q) return;
-  const int n = min(p.n_splits, (lk - lq + i) / p.split_keys + 1);
+  if (i < 0 || i >= lq || lk < lq || p.cu_q[lo + 1] > p.total_q || p.table_keys == 0) return;
+  const int n = min(p.n_splits, min(lk - lq + i, p.table_keys - 1) / p.split_keys + 1);
   const float* ws = p.ws + (row * p.hq + head) * p.n_splits * PF_WS_ROW;
   float m = -INFINITY;
   for (int s = lane; s < n; s += 32) m = fmaxf(m, ws[(int64_t)s * PF_WS_ROW + KV8_D]);
@@ -665,7 +674,7 @@ extern "C" int qb_attn_paged_prefill_fp8(const void* q, int64_t q_stride, const 
   PrefillP p{};
   p.q = (const bf16*)q; p.q_stride = q_stride; p.k = (const uint8_t*)k_cache; p.v = (const uint8_t*)v_cache;
   p.ks = k_scale; p.vs = v_scale; p.num_blocks = num_blocks; p.bt = block_tables; p.bt_stride = bt_stride;
-  p.bt_width = bt_width; p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k; p.batch = batch; p.tiles = tile_info;
+  p.bt_width = bt_width; p.table_keys = (int)std::min<int64_t>((int64_t)bt_width * KV8_PAGE, INT32_MAX); p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k; p.batch = batch; p.tiles = tile_info;
   p.hq = hq; p.hkv = hkv;
   p.pos_per_cta = 16;
   while (p.pos_per_cta * 2 * (hq / hkv) <= 2 * PF_ROWS) p.pos_per_cta *= 2;

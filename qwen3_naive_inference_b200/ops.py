@@ -578,7 +578,7 @@ def _fp8_rows(what, q, hkv):
 
 def _fp8_ints(what, *ts):
     for t in ts:
-        if t.dtype != torch.int32 or t.stride(-1) != 1:
+        if t.dtype != torch.int32 or (t.stride(-1) != 1 and t.shape[-1] > 1 and t.numel()):
             raise NativeError(f"{what} needs int32 index tensors with unit stride")
 
 
@@ -655,7 +655,7 @@ def grouped_decode_plan_fp8(batch, n_groups, hq, hkv, max_shared, max_own, slots
     :func:`paged_decode_attention_grouped_fp8`; ``n_groups``: the live groups expected."""
     own, own_splits = decode_split_plan_fp8(batch, hkv, max(1, max_own), slots)
     shared, shared_splits = decode_split_plan_fp8(n_groups, hkv, max(1, max_shared), slots)
-    return n_groups, shared, shared_splits, own, own_splits
+    return max(1, n_groups), shared, shared_splits, own, own_splits
 
 
 def workspace_fp8(batch, hq, n_slots, device, grouped=False):
@@ -691,6 +691,8 @@ def paged_decode_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_tabl
     if block_tables.dim() != 2 or seqlens.dim() != 1 or block_tables.shape[0] != B or seqlens.shape[0] != B:
         raise NativeError(f"{what} needs block_tables [batch, width] and seqlens [batch]")
     width = block_tables.shape[1]
+    if (split_tokens is None) != (max_splits is None):
+        raise NativeError(f"{what} needs both split_tokens and max_splits, or neither")
     if split_tokens is None:
         split_tokens, max_splits = decode_split_plan_fp8(B, hkv, width * KV_FP8_PAGE if max_ctx is None else max_ctx)
     out = _fp8_out(what, out, q)
@@ -721,6 +723,8 @@ def paged_decode_attention_grouped_fp8(q, k_cache, v_cache, k_scale, v_scale, bl
                           "[groups, 8] and shared_len [groups]")
     group_step, shared_tokens, shared_splits, own_tokens, own_splits = plan
     out = _fp8_out(what, out, q)
+    if n_groups == 0:
+        return out.zero_()
     ws, ws_ptr = _fp8_workspace(what, workspace, q, B, hq, shared_splits + own_splits, grouped=True)
     err, stream = _launch_ptrs(dev)
     check(lib().qb_paged_decode_attn_grouped_fp8(
@@ -739,6 +743,7 @@ def prefill_split_plan_fp8(batch, total_q, max_q, max_k, hq, hkv, sm_count=148):
     while positions * 2 * (hq // hkv) <= 256:
         positions *= 2
     tiles = min(batch * math.ceil(max_q / positions), batch + total_q // positions)  # ragged: close above the count
+    tiles = max(tiles, total_q // positions)  # rows in no sequence are joined with the others
     want = min(sm_count // max(1, tiles * hkv), math.ceil(max_k / 512))
     if want <= 1:
         return 0, 1

@@ -485,6 +485,35 @@ def test_prefill_nan_in_later_keys(cuda):
         assert bool(torch.isfinite(dec).all())
 
 
+@pytest.mark.parametrize("past,width", [(400, 1), (3000, 8)])
+def test_prefill_keys_beyond_the_table_are_reported(cuda, past, width):
+    """More keys than the table can name, in one split and in several: reported, and left out."""
+    g = gen(33)
+    k, v, ks, vs = random_cache(g, 9, 2)
+    q = torch.randn(20, 4, D, generator=g).to(BF)
+    table = torch.arange(1, width + 1, dtype=torch.int32)[None]
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    args = on(cuda, q, k, v, ks, vs, i32(0, 20), i32(0, 20 + past))
+    n = ops.prefill_split_plan_fp8(1, 20, 20, 20 + past, 4, 2)[1]
+    assert (n == 1) == (past == 400)
+    out = ops.attention_paged_prefill_fp8(*args, 20, table.to(cuda), 0.1, max_seqlen_k=20 + past)
+    with pytest.raises(ops.NativeError, match="page id"):
+        ops.check_device_errors()
+    k64, v64 = values(k, ks), values(v, vs)
+    for h in range(4):
+        kv = [rows_of(c, table[0], 0, width * PAGE, h // 2) for c in (k64, v64)]
+        check_attention(out[:, h], *attend(q[:, h], [kv], 0.1, past))
+    # a sequence of more queries than max_seqlen_q: the rows beyond are left, and reported
+    q = torch.randn(300, 4, D, generator=g).to(BF)
+    out = torch.full((300, 4, D), 2.0, dtype=BF, device=cuda)
+    args = on(cuda, q, k, v, ks, vs, i32(0, 300), i32(0, 300))
+    ops.attention_paged_prefill_fp8(*args, 100, torch.tensor([[1, 2]], dtype=torch.int32, device=cuda), 0.1, out=out)
+    with pytest.raises(ops.NativeError, match="inconsistent"):
+        ops.check_device_errors()
+    assert bool((out[128:] == 2.0).all()) and not bool((out[:128] == 2.0).all())
+    ops.check_device_errors()
+
+
 def test_prefill_shapes_reported(cuda):
     """Fewer keys than queries, and a page outside the pool."""
     g = gen(32)
@@ -796,6 +825,7 @@ def test_refusals(cuda):
         lambda: dec(q, k, v, ks, vs, t, n.long(), 0.1),
         lambda: dec(q, k, v, ks, vs, t, i32(5, 6), 0.1),
         lambda: dec(q, k, v, ks, vs, t, n, 0.1, split_tokens=100, max_splits=3),
+        lambda: dec(q, k, v, ks, vs, t, n, 0.1, split_tokens=128),
         lambda: dec(q, k, v, ks, vs, t, n, 0.1, split_tokens=16384, max_splits=1),
         lambda: dec(q, k, v, ks, vs, t, n, 0.1, split_tokens=64, max_splits=4, workspace=torch.zeros(8, device=cuda)),
         lambda: dec(q, k, v, ks, vs, t, n.cpu(), 0.1),
@@ -809,6 +839,10 @@ def test_refusals(cuda):
         with pytest.raises(ops.NativeError):
             f()
             pytest.fail(f"call {i} was taken")
+    # no groups: no sequence is in one
+    z = ops.paged_decode_attention_grouped_fp8(q, k, v, ks, vs, t, n, 0.1, t[:0, :1].expand(0, 8).contiguous(), n[:0], n,
+                                               ops.grouped_decode_plan_fp8(q.shape[0], 0, 4, 2, 0, 64))
+    assert z.shape == q.shape and not bool(z.any())
     # tensors of another device than the current one (as seen where the current one is asked for)
     with pytest.MonkeyPatch.context() as mp:
         mp.setattr(torch.cuda, "current_device", lambda: 1)
