@@ -88,6 +88,11 @@ QB_DEVICE uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+QB_DEVICE float max3(float a, float b, float c) {  // NaN only if all are
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 QB_DEVICE void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 QB_DEVICE void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -409,13 +414,16 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
       for (int i = 0; i < 64; ++i)
         if (i >= seen) v[i] = __float_as_uint(-INFINITY);
     }
-    float top[8];
+    float top[4];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) top[c] = __uint_as_float(v[c]);
+    for (int c = 0; c < 4; ++c) top[c] = max3(__uint_as_float(v[c]), __uint_as_float(v[c + 4]), __uint_as_float(v[c + 8]));
 #pragma unroll
-    for (int i = 8; i < 64; ++i) top[i & 7] = fmaxf(top[i & 7], __uint_as_float(v[i]));
-    const float mt = f * fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])),
-                               fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])));
+    for (int i = 12; i < 60; i += 8)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) top[c] = max3(top[c], __uint_as_float(v[i + c]), __uint_as_float(v[i + 4 + c]));
+#pragma unroll
+    for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(v[60 + c]));
+    const float mt = f * fmaxf(max3(top[0], top[1], top[2]), top[3]);
     const bool need = mt > ref + PF_SLACK;
     if (__any_sync(0xffffffffu, need) || vfac != 1.f) {
       float a = vfac;
@@ -447,19 +455,25 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
 #pragma unroll
     for (int c = 0; c < 4; ++c) sum[c] = make_float2(0.f, 0.f);
     uint32_t pk[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      float2 y = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ff, ss);
-      y.x = fast_exp2(y.x);
-      y.y = fast_exp2(y.y);
-      sum[i & 3] = add2(sum[i & 3], y);
-      pk[i] = pack_half2(y.x, y.y);
-    }
-    if (after != 1.f) {  // (the same for every thread of the CTA) weigh in fp32, from the probabilities again
+    // `after` is the same for every thread of the CTA.  Two loops, so that a score is not needed again once
+    // it is a probability: its register is free for the ones that follow.
+    if (after == 1.f) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        const float2 y = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ff, ss);
-        pk[i] = pack_half2(fast_exp2(y.x) * after, fast_exp2(y.y) * after);
+        float2 y = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ff, ss);
+        y.x = fast_exp2(y.x);
+        y.y = fast_exp2(y.y);
+        sum[i & 3] = add2(sum[i & 3], y);
+        pk[i] = pack_half2(y.x, y.y);
+      }
+    } else {  // weigh in fp32, after the sum
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        float2 y = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ff, ss);
+        y.x = fast_exp2(y.x);
+        y.y = fast_exp2(y.y);
+        sum[i & 3] = add2(sum[i & 3], y);
+        pk[i] = pack_half2(y.x * after, y.y * after);
       }
     }
     tmem_st32(s_at, pk);
