@@ -236,7 +236,9 @@ int qb_paged_decode_attn_fp8(const void* q, int64_t q_stride, const void* k_cach
  * entries of group_members that name no sequence set QB_DEVERR_SHAPE.  The CTAs of the shared keys take
  * groups g, g + group_step, ... one after another: the number of live groups expected (a table captured
  * for any grouping may have many empty entries behind them, which then cost no CTAs), or n_groups.  A sequence
- * is in one group at most.  With n_groups = 0 nothing is written.  workspace: qb_paged_decode_grouped_fp8_workspace_bytes(batch, hq, shared_splits + own_splits),
+ * is in one group at most.  With n_groups = 0 nothing is written.  Where
+ * qb_paged_decode_grouped_fp8_whole(hq, hkv, min(group_step, n_groups), ...) says so -- many groups, keys in
+ * one split each -- a CTA takes members through all their keys and the workspace is not needed.  workspace: qb_paged_decode_grouped_fp8_workspace_bytes(batch, hq, shared_splits + own_splits),
  * any contents. */
 int qb_paged_decode_attn_grouped_fp8(const void* q, int64_t q_stride, const void* k_cache,
                                      const void* v_cache, const float* k_scale, const float* v_scale,
@@ -248,6 +250,8 @@ int qb_paged_decode_attn_grouped_fp8(const void* q, int64_t q_stride, const void
                                      int shared_tokens, int shared_splits, int own_tokens, int own_splits,
                                      float* workspace, void* out, int* err, qb_stream_t stream);
 size_t qb_paged_decode_fp8_workspace_bytes(int batch, int hq, int n_slots);
+int qb_paged_decode_grouped_fp8_whole(int hq, int hkv, int group_step, int shared_tokens, int shared_splits,
+                                      int own_tokens, int own_splits);
 size_t qb_paged_decode_grouped_fp8_workspace_bytes(int batch, int hq, int n_slots);
 /* Causal attention of the query rows cu_seqlens_q over the first cu_seqlens_k keys of each sequence in
  * that cache; arguments as the paged form of qb_attn_varlen_fwd.  q and out rows q_stride / o_stride

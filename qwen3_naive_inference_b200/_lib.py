@@ -70,6 +70,7 @@ SIGNATURES: dict[str, tuple] = {
     "qb_paged_decode_attn_grouped_fp8": (I, [P, L, P, P, P, P, L, I, P, L, I, P, I, I, I, I, I, F, P, P, I, P, I, I,
                                              I, I, I, P, P, P, P]),
     "qb_paged_decode_fp8_workspace_bytes": (c_size_t, [I, I, I]),
+    "qb_paged_decode_grouped_fp8_whole": (I, [I, I, I, I, I, I, I]),
     "qb_paged_decode_grouped_fp8_workspace_bytes": (c_size_t, [I, I, I]),
     "qb_attn_paged_prefill_fp8": (I, [P, L, P, P, P, P, L, I, P, L, I, P, P, I, P, I, I, I, I, I, F, I, I, P, P, L, L, P,
                                       P]),

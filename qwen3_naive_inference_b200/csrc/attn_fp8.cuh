@@ -35,14 +35,14 @@ int kv8_check_cache(const void* q, int64_t q_stride, const void* k, const void* 
   return QB_OK;
 }
 
-// The cache as [num_blocks * hkv * 256, 128] bytes, read a block of 64 rows at a time; the 16-byte
+// The cache as [num_blocks * hkv * 256, 128] bytes, read `rows` rows of a block of 64 at a time; the 16-byte
 // chunks of a row are XORed with (row & 7), so that eight rows' chunks lie in different banks.
-bool kv8_tmap(CUtensorMap* map, const void* codes, int64_t num_blocks, int hkv) {
+bool kv8_tmap(CUtensorMap* map, const void* codes, int64_t num_blocks, int hkv, int rows) {
   auto fn = encode_fn();
   if (!fn) return false;
   cuuint64_t dims[2] = {(cuuint64_t)KV8_D, (cuuint64_t)num_blocks * hkv * KV8_PAGE};
   cuuint64_t strides[1] = {(cuuint64_t)KV8_D};
-  cuuint32_t box[2] = {(cuuint32_t)KV8_D, (cuuint32_t)KV8_BLOCK};
+  cuuint32_t box[2] = {(cuuint32_t)KV8_D, (cuuint32_t)rows};
   cuuint32_t estr[2] = {1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

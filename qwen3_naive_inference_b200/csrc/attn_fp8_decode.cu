@@ -33,9 +33,10 @@ constexpr int DC_STAGE_BYTES = 2 * KV8_TILE;       // K then V
 constexpr int DC_MAX_TILES = 128;                  // of one CTA's range (8192 keys)
 constexpr int DC_WS_ROW = KV8_D + 4;               // workspace row: O / l, then ref + log2 l
 constexpr int DC_O_ROW = KV8_D + 4;                // shared-memory row of a warp's output (padded)
-constexpr int DC_META = DC_MAX_TILES * 12 + (2 * DC_STAGES + 1) * 8 + 8 + 2 * DC_WARPS * 16 * 4;
+constexpr int DC_META = DC_MAX_TILES * 16 + (2 * DC_STAGES + 1) * 8 + 8 + 2 * DC_WARPS * 16 * 4;
 constexpr int DC_SMEM = DC_STAGES * DC_STAGE_BYTES + DC_META + 1024 /*align*/;
 static_assert(DC_WARPS * 16 * DC_O_ROW * 4 <= DC_STAGES * DC_STAGE_BYTES, "the join reuses the stages");
+constexpr int DC_WHOLE_CTAS = 400;
 constexpr float DC_HEAD = 7.f, DC_SLACK = 15.f;    // ref = max - 7; moves when a score is above ref + 15
 
 struct DecodeP {
@@ -65,6 +66,15 @@ struct DecodeP {
   unsigned n_shared;          // shared CTAs; the own CTAs follow
   int* entry_of;              // [batch] in the workspace: where a sequence stands in `members`
 };
+
+// The cache's tensor maps: whole blocks, and 16 rows for the blocks that a range ends in.
+struct DecodeMaps {
+  CUtensorMap k, v, k16, v16;
+};
+bool decode_maps(DecodeMaps* m, const void* k, const void* v, int64_t num_blocks, int hkv) {
+  return kv8_tmap(&m->k, k, num_blocks, hkv, KV8_BLOCK) && kv8_tmap(&m->v, v, num_blocks, hkv, KV8_BLOCK) &&
+         kv8_tmap(&m->k16, k, num_blocks, hkv, 16) && kv8_tmap(&m->v16, v, num_blocks, hkv, 16);
+}
 
 // What a CTA works on: `rows` query rows over keys [begin, end) of table row `table`.
 struct Work {
@@ -105,13 +115,31 @@ QB_DEVICE int row_sequence(const DecodeP& p, const int32_t* members, int b, int 
   return m >= 0 && m < p.batch ? m : -1;
 }
 
+// A sequence's own keys are [first, len); first is a block's start (-1: it is not).
+QB_DEVICE int own_first(const DecodeP& p, int b) {
+  const int first = p.kv_start ? p.kv_start[b] : 0;
+  return first >= 0 && first % KV8_BLOCK == 0 ? first : -1;
+}
+// The producer's lanes look up the pages of tiles lane, lane + 32, ... of `tiles` from key `begin` (-1: none).
+// No length is needed for it, so it goes ahead while those are on their way.
+constexpr int DC_LANE_TILES = DC_MAX_TILES / 32;
+QB_DEVICE void find_pages(const DecodeP& p, int table, int64_t begin, int tiles, int (&pages)[DC_LANE_TILES]) {
+  if (threadIdx.x < DC_WARPS * 32) return;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < DC_LANE_TILES; ++j) {
+    const int64_t col = (begin / KV8_BLOCK + lane + 32 * j) / KV8_SUBS;
+    pages[j] = lane + 32 * j < tiles && col < p.bt_width ? p.bt[(int64_t)table * p.bt_stride + col] : -1;
+  }
+}
+
 // One CTA: the work `w` of kv head `kvh`; NT tiles of eight query rows.  `members`: the chunk's member
 // list (shared work), `b`: the sequence (own work).  `u0` tiles and `item` works came before in this CTA.
-template <int NT, bool SHARED>
-QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtensorMap& tv, uint8_t* smem, uint32_t base,
-                           const Work& w, int kvh, const int32_t* members, int b, int u0, int item) {
+template <int NT, bool SHARED, bool WHOLE>
+QB_DEVICE void decode_work(const DecodeP& p, const DecodeMaps& maps, const int (&pages)[DC_LANE_TILES], uint8_t* smem,
+                           uint32_t base, const Work& w, int kvh, const int32_t* members, int b, int u0, int item) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int n = (w.end - w.begin + KV8_BLOCK - 1) / KV8_BLOCK;
+  int n = (w.end - w.begin + KV8_BLOCK - 1) / KV8_BLOCK;
   const int group = p.hq / p.hkv;
   uint8_t* meta = smem + DC_STAGES * DC_STAGE_BYTES;
   const uint32_t bar = base + DC_STAGES * DC_STAGE_BYTES;  // full[S], empty[S], meta
@@ -119,43 +147,92 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
   auto empty = [&](int s) { return bar + 8 * (DC_STAGES + s); };
   const uint32_t ready = bar + 8 * (2 * DC_STAGES);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(meta + 8 * (2 * DC_STAGES + 1));
-  int* page_of = reinterpret_cast<int*>(meta + 8 * (2 * DC_STAGES + 2));
-  float* ks_of = reinterpret_cast<float*>(page_of + DC_MAX_TILES);
+  int* n_of = reinterpret_cast<int*>(meta + 8 * (2 * DC_STAGES + 1) + 4);  // WHOLE: tiles
+  int* block_of = reinterpret_cast<int*>(meta + 8 * (2 * DC_STAGES + 2));  // of a tile: (page, head, block), -1: no page
+  int* part_of = block_of + DC_MAX_TILES;  // WHOLE: its keys, first row << 8, one past its last row << 16
+  float* ks_of = reinterpret_cast<float*>(part_of + DC_MAX_TILES);
   float* vs_of = ks_of + DC_MAX_TILES;
   float* join = vs_of + DC_MAX_TILES;  // [warp][16] ref, [warp][16] l
 
   if (warp == DC_WARPS) {
     // ------------------------------------------------------------ producer
-    float ks[DC_MAX_TILES / 32], vs[DC_MAX_TILES / 32];
-#pragma unroll
-    for (int j = 0; j < DC_MAX_TILES / 32; ++j) {
-      const int i = lane + 32 * j;
-      ks[j] = vs[j] = 0.f;
-      if (i >= n) continue;
-      const int blk = w.begin / KV8_BLOCK + i, col = blk / KV8_SUBS;
-      int page = col < p.bt_width ? p.bt[(int64_t)w.table * p.bt_stride + col] : -1;
+    float ks[DC_LANE_TILES], vs[DC_LANE_TILES];
+    auto found = [&](int j, int page, int blk) {  // tile lane + 32 j is block `blk` of a sequence, in `page`
+      int at = -1;
       if (page < 0 || page >= p.num_blocks) {
         qb_set_err(p.err, QB_DEVERR_PAGE);
-        page = -1;
       } else {
-        const int64_t at = ((int64_t)page * p.hkv + kvh) * KV8_SUBS + blk % KV8_SUBS;
+        at = (page * p.hkv + kvh) * KV8_SUBS + blk % KV8_SUBS;
         ks[j] = p.ks[at];
         vs[j] = p.vs[at];
       }
-      page_of[i] = page;
+      block_of[lane + 32 * j] = at;
+    };
+    if (WHOLE) {
+      // the group's shared keys, [0, w.end) of table row w.table, then each member's own, which lane m looks up
+      int seq = -1, first = 0, keys = 0;
+      if (lane < w.rows / group) {
+        seq = members[lane];
+        if (seq < 0 || seq >= p.batch) {
+          seq = -1;
+        } else {
+          first = own_first(p, seq);
+          keys = p.seqlens[seq] + p.seqlen_add - first;
+          if (first < 0 || keys > p.own_tokens) qb_set_err(p.err, QB_DEVERR_SHAPE);
+          keys = first < 0 ? 0 : max(0, min(keys, p.own_tokens));
+        }
+      }
+      int last = (keys + KV8_BLOCK - 1) / KV8_BLOCK;  // tile after the member's last, counted from the first own one
+      for (int o = 1; o < 8; o *= 2) {
+        const int before = __shfl_up_sync(0xffffffffu, last, o);
+        if (lane >= o && lane < 8) last += before;
+      }
+      const int shared = n;
+      n += __shfl_sync(0xffffffffu, last, 7);
+#pragma unroll
+      for (int j = 0; j < DC_LANE_TILES; ++j) {
+        const int i = lane + 32 * j, own = i - shared;
+        int m = 0;
+        for (int k = 0; k < 7; ++k) m += own >= __shfl_sync(0xffffffffu, last, k);
+        const int from = __shfl_sync(0xffffffffu, first, m), mine = __shfl_sync(0xffffffffu, keys, m);
+        const int to = __shfl_sync(0xffffffffu, last, m), table = __shfl_sync(0xffffffffu, seq, m);
+        ks[j] = vs[j] = 0.f;
+        if (i >= n) continue;
+        const int nth = own - (to - (mine + KV8_BLOCK - 1) / KV8_BLOCK);  // the tile among the member's
+        const int blk = own < 0 ? i : from / KV8_BLOCK + nth, row = own < 0 ? w.table : table;
+        const int live = own < 0 ? w.end - i * KV8_BLOCK : mine - nth * KV8_BLOCK, col = blk / KV8_SUBS;
+        part_of[i] = min(live, KV8_BLOCK) | (own < 0 ? w.rows << 16 : (m * group) << 8 | ((m + 1) * group) << 16);
+        found(j, col < p.bt_width ? p.bt[(int64_t)row * p.bt_stride + col] : -1, blk);
+      }
+      if (lane == 0) *n_of = n;
+    } else {
+#pragma unroll
+      for (int j = 0; j < DC_LANE_TILES; ++j) {
+        ks[j] = vs[j] = 0.f;
+        if (lane + 32 * j < n) found(j, pages[j], w.begin / KV8_BLOCK + lane + 32 * j);
+      }
     }
     __syncwarp();
     auto issue = [&](int i) {
-      const int s = (u0 + i) % DC_STAGES, page = page_of[i];
-      if (page < 0) {
+      const int s = (u0 + i) % DC_STAGES, block = block_of[i];
+      if (block < 0) {
         mbar_arrive(full(s));
         return;
       }
-      const int row = ((page * p.hkv + kvh) * KV8_SUBS + (w.begin / KV8_BLOCK + i) % KV8_SUBS) * KV8_BLOCK;
+      const int row = block * KV8_BLOCK;
       const uint32_t at = base + s * DC_STAGE_BYTES;
-      mbar_expect_tx(full(s), DC_STAGE_BYTES);
-      tma_load_2d(at, &tk, 0, row, full(s));
-      tma_load_2d(at + KV8_TILE, &tv, 0, row, full(s));
+      const int keys = WHOLE ? part_of[i] & 255 : w.end - w.begin - i * KV8_BLOCK;
+      const int parts = (min(keys, KV8_BLOCK) + 15) / 16;  // of 16 keys, the last ones ragged
+      mbar_expect_tx(full(s), parts * 2 * 16 * KV8_D);
+      if (parts == KV8_BLOCK / 16) {
+        tma_load_2d(at, &maps.k, 0, row, full(s));
+        tma_load_2d(at + KV8_TILE, &maps.v, 0, row, full(s));
+      } else {
+        for (int k = 0; k < parts; ++k) {
+          tma_load_2d(at + k * 16 * KV8_D, &maps.k16, 0, row + 16 * k, full(s));
+          tma_load_2d(at + KV8_TILE + k * 16 * KV8_D, &maps.v16, 0, row + 16 * k, full(s));
+        }
+      }
     };
     int issued = 0;
     auto issue_to = [&](int last) {
@@ -167,7 +244,7 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
     };
     if (lane == 0) issue_to(min(n, DC_STAGES));
 #pragma unroll
-    for (int j = 0; j < DC_MAX_TILES / 32; ++j)
+    for (int j = 0; j < DC_LANE_TILES; ++j)
       if (lane + 32 * j < n) {
         ks_of[lane + 32 * j] = ks[j];
         vs_of[lane + 32 * j] = vs[j];
@@ -195,7 +272,7 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
     const int r = nt * 8 + g;
     const int s = r < w.rows ? row_sequence<SHARED>(p, members, b, r) : -1;
     uint4 raw[4];
-    float top = 0.f;
+    __nv_bfloat162 most = __float2bfloat162_rn(0.f);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       raw[i] = make_uint4(0, 0, 0, 0);
@@ -204,11 +281,9 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
                                                 32 * t)[i];
       const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 f = unpack_bf16x2(u[k]);
-        top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-      }
+      for (int k = 0; k < 4; ++k) most = __hmax2(most, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u[k])));
     }
+    float top = fmaxf(__low2float(most), __high2float(most));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     // the row's largest value goes to [2^9, 2^10): a bf16 value is a half down to 2^-23 of it
@@ -222,8 +297,8 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
       const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float2 f = unpack_bf16x2(u[k]);
-        qf[nt][2 * i + k / 2][k & 1] = pack_half2(f.x * mul, f.y * mul);
+        const float2 f = mul2(unpack_bf16x2(u[k]), make_float2(mul, mul));
+        qf[nt][2 * i + k / 2][k & 1] = pack_half2(f.x, f.y);
       }
     }
   }
@@ -236,13 +311,23 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
     for (int i = 0; i < 8; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
   }
   bool ok = __all_sync(0xffffffffu, mbar_wait(ready, (uint32_t)item & 1u, abort_flag, p.err));
+  if (WHOLE) n = *n_of;
   for (int i = 0; ok && i < n; ++i) {
     const int s = (u0 + i) % DC_STAGES;
     if (!__all_sync(0xffffffffu, mbar_wait(full(s), (uint32_t)((u0 + i) / DC_STAGES) & 1u, abort_flag, p.err))) {
       ok = false;
       break;
     }
-    const int live = page_of[i] < 0 ? 0 : w.end - w.begin - i * KV8_BLOCK;  // keys of the tile that count
+    // keys of the tile that count, and for which of the rows
+    const int part = WHOLE ? part_of[i] : 0, live = block_of[i] < 0 ? 0 : WHOLE ? part & 255 : w.end - w.begin - i * KV8_BLOCK;
+    bool counts[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int r = 8 * nt + 2 * t + c;
+        counts[nt][c] = !WHOLE || (r >= ((part >> 8) & 255) && r < part >> 16);
+      }
     if (live > 16 * warp) {
       const uint32_t kt = base + s * DC_STAGE_BYTES, vt = kt + KV8_TILE;
       // V^T, asked for first: lane (g, t) holds elements 16g .. 16g+15 of keys 2t, 2t+1, 2t+8, 2t+9
@@ -286,10 +371,10 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
         const bool in0 = 16 * warp + g < live, in1 = 16 * warp + g + 8 < live;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          x[nt][0] = in0 ? (part[nt][0][0] + part[nt][1][0]) * (fac[nt][0] * ks) : -INFINITY;
-          x[nt][1] = in0 ? (part[nt][0][1] + part[nt][1][1]) * (fac[nt][1] * ks) : -INFINITY;
-          x[nt][2] = in1 ? (part[nt][0][2] + part[nt][1][2]) * (fac[nt][0] * ks) : -INFINITY;
-          x[nt][3] = in1 ? (part[nt][0][3] + part[nt][1][3]) * (fac[nt][1] * ks) : -INFINITY;
+          x[nt][0] = in0 && counts[nt][0] ? (part[nt][0][0] + part[nt][1][0]) * (fac[nt][0] * ks) : -INFINITY;
+          x[nt][1] = in0 && counts[nt][1] ? (part[nt][0][1] + part[nt][1][1]) * (fac[nt][1] * ks) : -INFINITY;
+          x[nt][2] = in1 && counts[nt][0] ? (part[nt][0][2] + part[nt][1][2]) * (fac[nt][0] * ks) : -INFINITY;
+          x[nt][3] = in1 && counts[nt][1] ? (part[nt][0][3] + part[nt][1][3]) * (fac[nt][1] * ks) : -INFINITY;
         }
       }
       // V's fragments do not wait for the scores: they are made while those are on their way
@@ -347,7 +432,8 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
           float d[4] = {0.f, 0.f, 0.f, 0.f};
           mma_f16_16816(d, va[k], pb[nt][0], pb[nt][1]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) o[nt][k][c] = fmaf(vs, d[c], o[nt][k][c]);
+          for (int c = 0; c < 4; ++c)
+            if (counts[nt][c & 1]) o[nt][k][c] = fmaf(vs, d[c], o[nt][k][c]);  // (else V may be NaN, and P 0)
         }
     }
     __syncwarp();
@@ -408,25 +494,14 @@ QB_DEVICE void decode_work(const DecodeP& p, const CUtensorMap& tk, const CUtens
   }
 }
 
-// A sequence's own keys: [first, len), and the splits of them that hold any.  first is a block's start
-// (-1: it is not).
-QB_DEVICE int own_first(const DecodeP& p, int b) {
-  const int first = p.kv_start ? p.kv_start[b] : 0;
-  return first >= 0 && first % KV8_BLOCK == 0 ? first : -1;
-}
+// The splits of a sequence's own keys that hold any.
 QB_DEVICE int own_live(const DecodeP& p, int b) {
   const int first = own_first(p, b), keys = p.seqlens[b] + p.seqlen_add - first;
   return first < 0 || keys <= 0 ? 0 : min(p.own_splits, (keys + p.own_tokens - 1) / p.own_tokens);
 }
 
-// NTS, NTO: row tiles of a shared and of an own CTA (NTS = 0: no groups).
-template <int NTS, int NTO>
-__global__ void __launch_bounds__(DC_THREADS, 3)
-decode_fp8_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, DecodeP p) {
-  extern __shared__ uint8_t smem_raw[];
-  qb_pdl_trigger();
-  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023) & ~1023u;
-  uint8_t* smem = smem_raw + (base - raw);
+// The CTA's barriers.
+QB_DEVICE void decode_barriers(const DecodeMaps& maps, uint8_t* smem, uint32_t base) {
   if (threadIdx.x == 0) {
     const uint32_t bar = base + DC_STAGES * DC_STAGE_BYTES;
     for (int s = 0; s < DC_STAGES; ++s) {
@@ -436,13 +511,32 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     mbar_init(bar + 16 * DC_STAGES, 1);
     *reinterpret_cast<volatile int*>(smem + DC_STAGES * DC_STAGE_BYTES + 8 * (2 * DC_STAGES + 1)) = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tk)) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tv)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.k)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.v)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.k16)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.v16)) : "memory");
   }
   __syncthreads();
+}
+// The stages, which a join wrote to, go back to the copies.
+QB_DEVICE void stages_back() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
+}
+
+// NTS, NTO: row tiles of a shared and of an own CTA (NTS = 0: no groups).
+template <int NTS, int NTO>
+__global__ void __launch_bounds__(DC_THREADS, 3)
+decode_fp8_kernel(const __grid_constant__ DecodeMaps maps, DecodeP p) {
+  extern __shared__ uint8_t smem_raw[];
+  qb_pdl_trigger();
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  decode_barriers(maps, smem, base);
   qb_pdl_wait();
   unsigned i = blockIdx.x;
   const int group = p.hq / p.hkv;
+  int pages[DC_LANE_TILES];
   if (NTS > 0 && i < p.n_shared) {
     const int split = i % p.shared_splits;
     i /= p.shared_splits;
@@ -453,6 +547,7 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     for (int grp = first; grp < p.n_groups; grp += p.group_step) {
       const int32_t* members = p.members + grp * 8 + c * p.chunk;
       const int donor = p.members[grp * 8], keys = p.shared_len[grp];
+      if (donor >= 0 && donor < p.batch) find_pages(p, donor, split * p.shared_tokens, p.shared_tokens / KV8_BLOCK, pages);
       Work w;
       const int n_members = min(p.chunk, 8 - c * p.chunk);
       w.rows = n_members * group;
@@ -471,11 +566,8 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       }
       if (split == p.shared_splits - 1 && w.end < keys && threadIdx.x == 0) qb_set_err(p.err, QB_DEVERR_SHAPE);
       if (!any || w.begin >= w.end || donor < 0 || donor >= p.batch) continue;
-      if (item > 0) {  // the stages, which the join wrote to, go back to the copies
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncthreads();
-      }
-      decode_work<NTS == 0 ? 1 : NTS, true>(p, tk, tv, smem, base, w, kvh, members, 0, u0, item);
+      if (item > 0) stages_back();
+      decode_work<NTS == 0 ? 1 : NTS, true, false>(p, maps, pages, smem, base, w, kvh, members, 0, u0, item);
       u0 += (w.end - w.begin + KV8_BLOCK - 1) / KV8_BLOCK;
       ++item;
     }
@@ -488,6 +580,7 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   const int b = i / p.hkv;
   const int len = p.seqlens[b] + p.seqlen_add, first = own_first(p, b);
   const int64_t begin = (int64_t)first + (int64_t)split * p.own_tokens;
+  find_pages(p, b, max(begin, (int64_t)0), p.own_tokens / KV8_BLOCK, pages);
   if ((first < 0 || (split == p.own_splits - 1 && begin + p.own_tokens < len)) && threadIdx.x == 0)
     qb_set_err(p.err, QB_DEVERR_SHAPE);
   if (first < 0) return;
@@ -504,7 +597,60 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         reinterpret_cast<uint2*>(p.out + ((int64_t)b * p.hq + kvh * group) * KV8_D)[k] = make_uint2(0, 0);
     return;
   }
-  decode_work<NTO, false>(p, tk, tv, smem, base, w, kvh, nullptr, b, 0, 0);
+  decode_work<NTO, false, false>(p, maps, pages, smem, base, w, kvh, nullptr, b, 0, 0);
+}
+
+// Many groups: a CTA takes up to eight query rows of a group -- four members, where two query heads share a
+// kv head -- through the shared keys and then through each member's own, one after another in the same ring
+// and the same running sums; own tiles count for their member's rows only.  Nothing is left to join, and what a
+// CTA needs to begin and to end (as long as four tiles of keys take) is paid once for four members.
+template <int NT>
+__global__ void __launch_bounds__(DC_THREADS, 3)
+decode_whole_fp8_kernel(const __grid_constant__ DecodeMaps maps, DecodeP p) {
+  extern __shared__ uint8_t smem_raw[];
+  qb_pdl_trigger();
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  decode_barriers(maps, smem, base);
+  qb_pdl_wait();
+  unsigned i = blockIdx.x;
+  const int group = p.hq / p.hkv;
+  if (i >= p.n_shared) {  // a warp per sequence: zeros for those in no group
+    const int64_t b = (int64_t)(i - p.n_shared) * (DC_THREADS / 32) + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (b >= p.batch) return;
+    bool member = false;
+    for (int k = lane; k < p.n_groups * 8; k += 32) member |= p.members[k] == (int)b;
+    if (__any_sync(0xffffffffu, member)) return;
+    for (int k = lane; k < p.hq * KV8_D / 8; k += 32)
+      reinterpret_cast<uint4*>(p.out + b * p.hq * KV8_D)[k] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const int kvh = i % p.hkv;
+  i /= p.hkv;
+  const int c = i % p.n_chunks, n_members = min(p.chunk, 8 - c * p.chunk);
+  int u0 = 0, item = 0, pages[DC_LANE_TILES];
+  for (int grp = i / p.n_chunks; grp < p.n_groups; grp += p.group_step) {
+    const int32_t* members = p.members + grp * 8 + c * p.chunk;
+    const int donor = p.members[grp * 8], keys = p.shared_len[grp];
+    bool any = false, wrong = false;
+    for (int m = 0; m < n_members; ++m) {
+      any |= members[m] >= 0 && members[m] < p.batch;
+      wrong |= members[m] >= p.batch;
+    }
+    if ((wrong || keys > p.shared_tokens) && threadIdx.x == 0) qb_set_err(p.err, QB_DEVERR_SHAPE);
+    if (!any) continue;
+    Work w;
+    w.rows = n_members * group;
+    w.table = donor;
+    w.begin = 0;
+    w.end = donor >= 0 && donor < p.batch ? max(0, min(keys, p.shared_tokens)) : 0;
+    w.slot = -1;
+    if (item > 0) stages_back();
+    decode_work<NT, true, true>(p, maps, pages, smem, base, w, kvh, members, 0, u0, item);
+    u0 += *reinterpret_cast<const int*>(smem + DC_STAGES * DC_STAGE_BYTES + 8 * (2 * DC_STAGES + 1) + 4);
+    ++item;
+  }
 }
 
 // Joins the splits of a (sequence, head): a warp each, weights 2^(lse - largest lse).  Only the splits
@@ -555,20 +701,32 @@ decode_fp8_join_kernel(DecodeP p) {
 }
 
 template <int NTS, int NTO>
-int launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeP& p, cudaStream_t st) {
+int launch_decode(const DecodeMaps& maps, const DecodeP& p, cudaStream_t st) {
   static std::atomic<uint64_t> allowed{0};
   const int may = kv8_allow_smem(reinterpret_cast<const void*>(decode_fp8_kernel<NTS, NTO>), DC_SMEM, allowed);
   if (may != QB_OK) return may;
   const int64_t ctas = p.n_shared + (int64_t)p.batch * p.hkv * p.own_splits, rows = (int64_t)p.batch * p.hq;
   if (ctas > INT32_MAX || rows > INT32_MAX) return QB_ERR_INVALID;
-  const int rc = qb_launch_ex(decode_fp8_kernel<NTS, NTO>, dim3((unsigned)ctas), dim3(DC_THREADS), DC_SMEM, st, 1, true, tk,
-                              tv, p);
+  const int rc = qb_launch_ex(decode_fp8_kernel<NTS, NTO>, dim3((unsigned)ctas), dim3(DC_THREADS), DC_SMEM, st, 1, true,
+                              maps, p);
   if (rc != QB_OK || p.n_slots == 1) return rc;
   return qb_launch_ex(decode_fp8_join_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, 1, true, p);
 }
 
+template <int NT>
+int launch_whole(const DecodeMaps& maps, const DecodeP& p, cudaStream_t st) {
+  static std::atomic<uint64_t> allowed{0};
+  const int may = kv8_allow_smem(reinterpret_cast<const void*>(decode_whole_fp8_kernel<NT>), DC_SMEM, allowed);
+  if (may != QB_OK) return may;
+  const int64_t ctas = p.n_shared + ((int64_t)p.batch + DC_THREADS / 32 - 1) / (DC_THREADS / 32);
+  if (ctas > INT32_MAX) return QB_ERR_INVALID;
+  return qb_launch_ex(decode_whole_fp8_kernel<NT>, dim3((unsigned)ctas), dim3(DC_THREADS), DC_SMEM, st, 1, true, maps, p);
+}
+
 // floats of the splits' partial outputs
 size_t decode_partials(int batch, int hq, int n_slots) { return (size_t)batch * hq * n_slots * DC_WS_ROW; }
+
+int members_per_cta(int group) { return min(8, (group <= 8 ? 8 : 16) / group); }
 
 bool split_ok(int tokens, int splits) {
   return tokens > 0 && tokens % KV8_BLOCK == 0 && tokens <= DC_MAX_TILES * KV8_BLOCK && splits >= 1 &&
@@ -590,8 +748,8 @@ extern "C" int qb_paged_decode_attn_fp8(const void* q, int64_t q_stride, const v
                                  bt_width, hq, hkv, out);
   if (ok != QB_OK) return ok;
   QB_CHECK_ARG(seqlens && (max_splits == 1 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0)));
-  CUtensorMap tk, tv;
-  if (!kv8_tmap(&tk, k_cache, num_blocks, hkv) || !kv8_tmap(&tv, v_cache, num_blocks, hkv)) return QB_ERR_INVALID;
+  DecodeMaps maps;
+  if (!decode_maps(&maps, k_cache, v_cache, num_blocks, hkv)) return QB_ERR_INVALID;
   DecodeP p{};
   p.q = (const bf16*)q; p.q_stride = q_stride; p.ks = k_scale; p.vs = v_scale; p.num_blocks = num_blocks;
   p.bt = block_tables; p.bt_stride = bt_stride; p.bt_width = bt_width; p.seqlens = seqlens; p.seqlen_add = seqlen_add;
@@ -599,7 +757,15 @@ extern "C" int qb_paged_decode_attn_fp8(const void* q, int64_t q_stride, const v
   p.own_tokens = split_tokens; p.own_splits = max_splits; p.n_slots = max_splits;
   p.ws = workspace; p.out = (bf16*)out; p.err = err;
   const cudaStream_t st = (cudaStream_t)stream;
-  return hq / hkv <= 8 ? launch_decode<0, 1>(tk, tv, p, st) : launch_decode<0, 2>(tk, tv, p, st);
+  return hq / hkv <= 8 ? launch_decode<0, 1>(maps, p, st) : launch_decode<0, 2>(maps, p, st);
+}
+
+extern "C" int qb_paged_decode_grouped_fp8_whole(int hq, int hkv, int group_step, int shared_tokens, int shared_splits,
+                                                 int own_tokens, int own_splits) {
+  if (shared_splits != 1 || own_splits != 1 || hkv < 1 || hq / hkv < 1 || hq / hkv > KV8_MAX_GROUP) return 0;
+  const int chunk = members_per_cta(hq / hkv);
+  return (int64_t)group_step * ((8 + chunk - 1) / chunk) * hkv >= DC_WHOLE_CTAS &&
+         shared_tokens + (int64_t)chunk * own_tokens <= DC_MAX_TILES * KV8_BLOCK;
 }
 
 extern "C" int qb_paged_decode_attn_grouped_fp8(
@@ -615,10 +781,12 @@ extern "C" int qb_paged_decode_attn_grouped_fp8(
   const int ok = kv8_check_cache(q, q_stride, k_cache, v_cache, k_scale, v_scale, num_blocks, block_tables, bt_stride,
                                  bt_width, hq, hkv, out);
   if (ok != QB_OK) return ok;
-  QB_CHECK_ARG(seqlens && group_members && shared_len && kv_start && workspace &&
-               (reinterpret_cast<uintptr_t>(workspace) & 15) == 0);
-  CUtensorMap tk, tv;
-  if (!kv8_tmap(&tk, k_cache, num_blocks, hkv) || !kv8_tmap(&tv, v_cache, num_blocks, hkv)) return QB_ERR_INVALID;
+  const bool whole =
+      qb_paged_decode_grouped_fp8_whole(hq, hkv, min(group_step, n_groups), shared_tokens, shared_splits, own_tokens, own_splits);
+  QB_CHECK_ARG(seqlens && group_members && shared_len && kv_start &&
+               (whole || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0)));
+  DecodeMaps maps;
+  if (!decode_maps(&maps, k_cache, v_cache, num_blocks, hkv)) return QB_ERR_INVALID;
   DecodeP p{};
   p.q = (const bf16*)q; p.q_stride = q_stride; p.ks = k_scale; p.vs = v_scale; p.num_blocks = num_blocks;
   p.bt = block_tables; p.bt_stride = bt_stride; p.bt_width = bt_width; p.seqlens = seqlens; p.seqlen_add = seqlen_add;
@@ -630,16 +798,18 @@ extern "C" int qb_paged_decode_attn_grouped_fp8(
   // Eight query rows a CTA where they are enough for a member: with 16, a group's shared keys were read
   // once instead of twice (the second time from L2), but a CTA's registers spilled and its sixteen rows took
   // longer to join (64 groups of 8: 102 us against 107, five small groups 11.6 against 16.3).
-  const int group = hq / hkv, row_tiles = group <= 8 ? 1 : 2;
-  p.chunk = min(8, row_tiles * 8 / group);
+  const int row_tiles = hq / hkv <= 8 ? 1 : 2;
+  p.chunk = members_per_cta(hq / hkv);
   p.n_chunks = (8 + p.chunk - 1) / p.chunk;
   p.group_step = min(group_step, n_groups);
-  p.entry_of = reinterpret_cast<int*>(workspace + decode_partials(batch, hq, p.n_slots));
+  p.entry_of = whole ? nullptr : reinterpret_cast<int*>(workspace + decode_partials(batch, hq, p.n_slots));
   const int64_t shared = (int64_t)p.group_step * p.n_chunks * hkv * shared_splits;
   QB_CHECK_ARG(shared <= INT32_MAX);
   p.n_shared = (unsigned)shared;
   const cudaStream_t st = (cudaStream_t)stream;
-  return row_tiles == 1 ? launch_decode<1, 1>(tk, tv, p, st) : launch_decode<2, 2>(tk, tv, p, st);
+  if (whole)
+    return row_tiles == 1 ? launch_whole<1>(maps, p, st) : launch_whole<2>(maps, p, st);
+  return row_tiles == 1 ? launch_decode<1, 1>(maps, p, st) : launch_decode<2, 2>(maps, p, st);
 }
 
 extern "C" size_t qb_paged_decode_fp8_workspace_bytes(int batch, int hq, int n_slots) {

@@ -11,6 +11,7 @@ embedding).  Dense projections go through :func:`linear`.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import numpy as np
@@ -655,7 +656,17 @@ def grouped_decode_plan_fp8(batch, n_groups, hq, hkv, max_shared, max_own, slots
     :func:`paged_decode_attention_grouped_fp8`; ``n_groups``: the live groups expected."""
     own, own_splits = decode_split_plan_fp8(batch, hkv, max(1, max_own), slots)
     shared, shared_splits = decode_split_plan_fp8(n_groups, hkv, max(1, max_shared), slots)
+    up = lambda n: math.ceil(max(1, n) / 64) * 64  # noqa: E731
+    if own_splits == 1:  # no more than there can be: a CTA then takes whole groups where there are many
+        own = up(max_own)
+    if shared_splits == 1:
+        shared = up(max_shared)
     return max(1, n_groups), shared, shared_splits, own, own_splits
+
+
+@functools.lru_cache(maxsize=256)
+def _grouped_whole(*sizes):
+    return bool(lib().qb_paged_decode_grouped_fp8_whole(*sizes))
 
 
 def workspace_fp8(batch, hq, n_slots, device, grouped=False):
@@ -725,14 +736,15 @@ def paged_decode_attention_grouped_fp8(q, k_cache, v_cache, k_scale, v_scale, bl
     out = _fp8_out(what, out, q)
     if n_groups == 0:
         return out.zero_()
-    ws, ws_ptr = _fp8_workspace(what, workspace, q, B, hq, shared_splits + own_splits, grouped=True)
+    whole = _grouped_whole(hq, hkv, min(group_step, n_groups), *plan[1:])  # many groups: one kernel, no partial outputs
+    ws, ws_ptr = (None, 0) if whole else _fp8_workspace(what, workspace, q, B, hq, shared_splits + own_splits, grouped=True)
     err, stream = _launch_ptrs(dev)
     check(lib().qb_paged_decode_attn_grouped_fp8(
         q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
         num_blocks, KV_FP8_PAGE, block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1],
         seqlens.data_ptr(), seqlen_add, B, hq, hkv, 128, scale, group_members.data_ptr(), shared_len.data_ptr(), n_groups,
         kv_start.data_ptr(), group_step, shared_tokens, shared_splits, own_tokens, own_splits, ws_ptr, out.data_ptr(),
-        err, stream), what, kernels=2)
+        err, stream), what, kernels=1 if whole else 2)
     return out
 
 

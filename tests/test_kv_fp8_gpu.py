@@ -370,6 +370,72 @@ def test_grouped(cuda, hq, hkv, groups, plan):
     ops.check_device_errors()
 
 
+def many_groups(g, n, top_shared, top_own):
+    pick = lambda lo, hi: int(torch.randint(lo, hi + 1, (1,), generator=g))  # noqa: E731
+    return [(pick(1, top_shared), [pick(1, top_own) for _ in range(1 + i % 8)]) for i in range(n)]
+
+
+@pytest.mark.parametrize("hq,hkv,n", [(16, 8, 50), (8, 8, 64), (40, 8, 8), (24, 8, 16), (96, 8, 8), (64, 8, 9)])
+def test_grouped_many(cuda, hq, hkv, n):
+    """Enough groups for a CTA to take members through all their keys: against the formula, and with a table
+    that has more entries than there are groups, walked in steps."""
+    g = gen(60 + hq)
+    groups = many_groups(g, n, 150, 140)
+    groups[0] = (130, [1, 64, 65, 63, 128, 2, 129, 140])
+    groups[1] = (64, [64] * 8)
+    groups[2] = (1, [1])
+    q, k, v, ks, vs, parts, args, grp = grouped_inputs(g, hq, hkv, groups, cuda)
+    plan = ops.grouped_decode_plan_fp8(q.shape[0], n, hq, hkv, 150, 140)
+    assert ops._grouped_whole(hq, hkv, n, *plan[1:]) and plan[1:] == (192, 1, 192, 1)
+    out = ops.paged_decode_attention_grouped_fp8(*args, 0.1, *grp, plan, out=torch.full_like(args[0], 3.0))
+    k64, v64 = values(k, ks), values(v, vs)
+    for row, head, s, pages, st, end in parts:
+        for h in (row % hq, hq - 1 - row % hq):
+            kv = [[torch.cat([rows_of(c, head, 0, s, h // (hq // hkv)), rows_of(c, pages, st, end, h // (hq // hkv))])
+                   for c in (k64, v64)]]
+            check_attention(out[row, h:h + 1], *attend(q[row, h:h + 1], kv, 0.1), f"row {row} head {h}")
+    big = 2 * n + 3
+    members = torch.full((big, 8), -1, dtype=torch.int32, device=cuda)
+    shared = torch.zeros(big, dtype=torch.int32, device=cuda)
+    at = torch.randperm(big, generator=g)[:n].to(cuda)
+    members[at], shared[at] = grp[0], grp[1]
+    again = ops.paged_decode_attention_grouped_fp8(*args, 0.1, members, shared, grp[2], plan)
+    assert torch.equal(again, out)
+    # the same keys split and joined
+    split = ops.paged_decode_attention_grouped_fp8(*args, 0.1, *grp, (n, 64, 3, 64, 3))
+    assert torch.allclose(split.float(), out.float(), rtol=2.0 ** -6, atol=1e-2)
+    ops.check_device_errors()
+    # a sequence in no group gets zeros, its neighbours what they had; ids outside the batch are reported
+    lone = int(members[at[0], 3])
+    members[at[0], 3] = -1
+    keep = [i for i in range(q.shape[0]) if i != lone]
+    out2 = ops.paged_decode_attention_grouped_fp8(*args, 0.1, members, shared, grp[2], plan, out=torch.full_like(out, 3.0))
+    assert torch.equal(out2[keep], out[keep]) and not bool(out2[lone].any())
+    ops.check_device_errors()
+    members[at[0], 3] = q.shape[0]
+    out2 = ops.paged_decode_attention_grouped_fp8(*args, 0.1, members, shared, grp[2], plan, out=torch.full_like(out, 3.0))
+    with pytest.raises(ops.NativeError, match="inconsistent"):
+        ops.check_device_errors()
+    assert torch.equal(out2[keep], out[keep]) and not bool(out2[lone].any())
+    # keys beyond the plan are left out and reported
+    ops.paged_decode_attention_grouped_fp8(*args, 0.1, *grp, (n, 64, 1, 192, 1))
+    with pytest.raises(ops.NativeError, match="inconsistent"):
+        ops.check_device_errors()
+    ops.paged_decode_attention_grouped_fp8(*args, 0.1, *grp, (n, 192, 1, 64, 1))
+    with pytest.raises(ops.NativeError, match="inconsistent"):
+        ops.check_device_errors()
+    # NaN in a member's own keys and values stays in that member's rows
+    row, head, s, pages, st, end = parts[1]
+    for cache in (1, 2):
+        bad = [a.clone() if i == cache else a for i, a in enumerate(args)]
+        bad[cache].view(torch.uint8)[pages[-1], hkv - 1, 5, 7] = 0x7F
+        out3 = ops.paged_decode_attention_grouped_fp8(*bad, 0.1, *grp, plan)
+        keep = [i for i in range(q.shape[0]) if i != row]
+        assert torch.equal(out3[keep], out[keep]) and torch.equal(out3[row, :-(hq // hkv)], out[row, :-(hq // hkv)])
+        assert bool(out3[row, -1].isnan().any())
+    ops.check_device_errors()
+
+
 def test_grouped_equals_plain_decode_where_nothing_is_skipped(cuda):
     """Prompts of whole pages: the shared and the unshared kernels attend the same keys; a sequence in no
     group gets zeros whatever the workspace holds, a member id outside the batch is reported."""
