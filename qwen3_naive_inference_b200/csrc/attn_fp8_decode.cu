@@ -36,7 +36,6 @@ constexpr int DC_O_ROW = KV8_D + 4;                // shared-memory row of a war
 constexpr int DC_META = DC_MAX_TILES * 16 + (2 * DC_STAGES + 1) * 8 + 8 + 2 * DC_WARPS * 16 * 4;
 constexpr int DC_SMEM = DC_STAGES * DC_STAGE_BYTES + DC_META + 1024 /*align*/;
 static_assert(DC_WARPS * 16 * DC_O_ROW * 4 <= DC_STAGES * DC_STAGE_BYTES, "the join reuses the stages");
-constexpr int DC_WHOLE_CTAS = 400;
 constexpr float DC_HEAD = 7.f, DC_SLACK = 15.f;    // ref = max - 7; moves when a score is above ref + 15
 
 struct DecodeP {
@@ -600,6 +599,11 @@ decode_fp8_kernel(const __grid_constant__ DecodeMaps maps, DecodeP p) {
   decode_work<NTO, false, false>(p, maps, pages, smem, base, w, kvh, nullptr, b, 0, 0);
 }
 
+// From this many CTAs on (24 groups of eight heads) whole groups are faster than splits that are joined: us per
+// call, whole / split, of 24, 48 and 64 groups of eight with 64 to 512 shared keys: 20 / 32, 33 / 55, 41 / 72 with up
+// to 100 own keys a member, 46 / 54, 80 / 91, 103 / 119 with up to 700.  Below, the longest CTA decides: 8 groups
+// 14 / 15 and 34 / 27.
+constexpr int DC_WHOLE_CTAS = 384;
 // Many groups: a CTA takes up to eight query rows of a group -- four members, where two query heads share a
 // kv head -- through the shared keys and then through each member's own, one after another in the same ring
 // and the same running sums; own tiles count for their member's rows only.  Nothing is left to join, and what a
