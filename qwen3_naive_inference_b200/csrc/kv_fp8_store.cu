@@ -155,21 +155,29 @@ QB_DEVICE void st_codes(uint8_t* dst, float (&v)[8], float inv, bool odd) {
   *reinterpret_cast<uint2*>(dst) = u;
 }
 // Rounds the block's rows that this call does not write (`kept`) again under a scale larger by 1 / ratio.
-// `n` threads take part, this one as number `i`.
-template <typename F>
-QB_DEVICE void round_again(uint8_t* block, F kept, float ratio, int i, int n) {
-  for (int c = i; c < KV8_TILE / 16; c += n) {
-    if (!kept(c >> 3)) continue;
-    uint4* at = reinterpret_cast<uint4*>(block) + c;
-    uint4 u = *at;
-    uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+// N threads take part, this one as number `i`.  Up to eight loads of a thread are on their way at once: in a decode
+// step some block of the call nearly always needs it, and the step waits for that block's warp (with one load
+// after another a step of 512 sequences took 23 us where rows arrive for the first time, 6 us without this).
+template <int N, typename F>
+QB_DEVICE void round_again(uint8_t* block, F kept, float ratio, int i) {
+  constexpr int EACH = KV8_TILE / 16 / N, AHEAD = EACH < 8 ? EACH : 8;
+  uint4* at = reinterpret_cast<uint4*>(block) + i;
+#pragma unroll 1
+  for (int c = 0; c < EACH; c += AHEAD) {
+    uint4 u[AHEAD];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float f[4];
-      e4m3x4_to_float4(w[k], f);
-      w[k] = float4_to_e4m3x4(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+    for (int k = 0; k < AHEAD; ++k) u[k] = at[(c + k) * N];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      uint32_t w[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float f[4];
+        e4m3x4_to_float4(w[j], f);
+        w[j] = float4_to_e4m3x4(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+      }
+      if (kept((i + (c + k) * N) >> 3)) at[(c + k) * N] = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    *at = u;
   }
 }
 // The block's scale after values up to `top` joined it: the old one unless the block begins anew or
@@ -269,7 +277,13 @@ QB_DEVICE bool store_alone(const StoreParams& p, int64_t t, int slot, int head, 
   const float now = joined_scale(old, half_max(finite_max(v, odd)), anew);
   st_codes(block + row * KV8_D + l * 8, v, 1.f / now, odd);
   if (l == 0) *scale = now;
-  if (!anew && now > old) round_again(block, [row](int r) { return r != row; }, old / now, l, 16);
+  const unsigned raised = __ballot_sync(0xffffffffu, !anew && now > old);
+#pragma unroll
+  for (int side = 0; side < 2; ++side)
+    if (raised >> (16 * side) & 1) {  // the whole warp, K's block, then V's
+      const float ratio = __shfl_sync(0xffffffffu, old / now, 16 * side);
+      round_again<32>(p.codes[side] + at * KV8_TILE, [row](int r) { return r != row; }, ratio, lane);
+    }
   return true;
 }
 
@@ -326,8 +340,8 @@ QB_DEVICE void store_many(const StoreParams& p, const Found& f, int i, int head,
     st_codes(vb + row * KV8_D + l * 8, x, 1.f / now_v, odd_v[r]);
   }
   const auto kept = [&f, i](int r) { return f.row_src[i][r] < 0; };
-  if (!anew && now_k > old_k) round_again(kb, kept, old_k / now_k, tid, ST_THREADS);
-  if (!anew && now_v > old_v) round_again(vb, kept, old_v / now_v, tid, ST_THREADS);
+  if (!anew && now_k > old_k) round_again<ST_THREADS>(kb, kept, old_k / now_k, tid);
+  if (!anew && now_v > old_v) round_again<ST_THREADS>(vb, kept, old_v / now_v, tid);
   if (tid == 0) {
     p.scales[0][at] = now_k;
     p.scales[1][at] = now_v;
