@@ -651,22 +651,22 @@ def decode_split_plan_fp8(batch: int, hkv: int, max_ctx: int, slots: int = 444) 
     return split, math.ceil(max_ctx / split)
 
 
-def grouped_decode_plan_fp8(batch, n_groups, hq, hkv, max_shared, max_own, slots=444):
-    """(group_step, shared_tokens, shared_splits, own_tokens, own_splits) of
-    :func:`paged_decode_attention_grouped_fp8`; ``n_groups``: the live groups expected."""
-    own, own_splits = decode_split_plan_fp8(batch, hkv, max(1, max_own), slots)
-    shared, shared_splits = decode_split_plan_fp8(n_groups, hkv, max(1, max_shared), slots)
-    up = lambda n: math.ceil(max(1, n) / 64) * 64  # noqa: E731
-    if own_splits == 1:  # no more than there can be: a CTA then takes whole groups where there are many
-        own = up(max_own)
-    if shared_splits == 1:
-        shared = up(max_shared)
-    return max(1, n_groups), shared, shared_splits, own, own_splits
-
-
 @functools.lru_cache(maxsize=256)
 def _grouped_whole(*sizes):
     return bool(lib().qb_paged_decode_grouped_fp8_whole(*sizes))
+
+
+def grouped_decode_plan_fp8(batch, n_groups, hq, hkv, max_shared, max_own, slots=444):
+    """(group_step, shared_tokens, shared_splits, own_tokens, own_splits) of
+    :func:`paged_decode_attention_grouped_fp8`; ``n_groups``: the live groups expected.  One split of each where
+    there are groups enough for a CTA to take members through all their keys."""
+    up = lambda n: math.ceil(max(1, n) / 64) * 64  # noqa: E731
+    whole = max(1, n_groups), up(max_shared), 1, up(max_own), 1
+    if _grouped_whole(hq, hkv, *whole):
+        return whole
+    own, own_splits = decode_split_plan_fp8(batch, hkv, max(1, max_own), slots)
+    shared, shared_splits = decode_split_plan_fp8(n_groups, hkv, max(1, max_shared), slots)
+    return max(1, n_groups), shared, shared_splits, own, own_splits
 
 
 def workspace_fp8(batch, hq, n_slots, device, grouped=False):
