@@ -549,7 +549,7 @@ def _kv_fp8(what, k_cache, v_cache, k_scale, v_scale, others):
         raise NativeError(f"{what}: the tensors must be on the current CUDA device")
     shape = k_cache.shape
     if k_cache.dtype != FP8 or v_cache.dtype != FP8 or v_cache.shape != shape or len(shape) != 4 \
-            or shape[2] != KV_FP8_PAGE or shape[3] != 128:
+            or shape[1] < 1 or shape[2] != KV_FP8_PAGE or shape[3] != 128:
         raise NativeError(f"{what} needs float8_e4m3fn caches [num_blocks, kv_heads, {KV_FP8_PAGE}, 128]")
     if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or k_scale.shape != v_scale.shape \
             or k_scale.shape != (shape[0], shape[1], KV_FP8_PAGE // KV_FP8_BLOCK):

@@ -436,6 +436,37 @@ def test_grouped_many(cuda, hq, hkv, n):
     ops.check_device_errors()
 
 
+def test_grouped_many_in_a_graph(cuda):
+    """A captured call follows the group table, the lengths and the cache as they are when it is replayed, on a
+    stream of its own."""
+    g = gen(77)
+    groups = many_groups(g, 40, 90, 100)
+    q, k, v, ks, vs, parts, args, grp = grouped_inputs(g, 16, 8, groups, cuda)
+    n = q.shape[0]
+    plan = ops.grouped_decode_plan_fp8(n, 40, 16, 8, 128, 128)
+    assert ops._grouped_whole(16, 8, 40, *plan[1:])
+    live = [t.clone() for t in args]
+    members, shared, start = grp[0].clone(), grp[1].clone(), grp[2].clone()
+    out = torch.empty_like(args[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.paged_decode_attention_grouped_fp8(*live, 0.1, members, shared, start, plan, out=out)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            ops.paged_decode_attention_grouped_fp8(*live, 0.1, members, shared, start, plan, out=out)
+        for shift in (0, 1, 7):  # groups elsewhere in the table, answers that have grown, other queries
+            members.copy_(grp[0].roll(shift, 0))
+            shared.copy_(grp[1].roll(shift, 0))
+            live[6].copy_(torch.maximum(args[6] - shift, grp[2] - 1))
+            live[0].copy_(args[0].roll(shift, 2))
+            graph.replay()
+            want = ops.paged_decode_attention_grouped_fp8(*live, 0.1, members, shared, start, plan)
+            assert torch.equal(out, want)
+    torch.cuda.current_stream().wait_stream(side)
+    ops.check_device_errors()
+
+
 def test_grouped_equals_plain_decode_where_nothing_is_skipped(cuda):
     """Prompts of whole pages: the shared and the unshared kernels attend the same keys; a sequence in no
     group gets zeros whatever the workspace holds, a member id outside the batch is reported."""
