@@ -237,8 +237,9 @@ int qb_paged_decode_attn_fp8(const void* q, int64_t q_stride, const void* k_cach
  * groups g, g + group_step, ... one after another: the number of live groups expected (a table captured
  * for any grouping may have many empty entries behind them, which then cost no CTAs), or n_groups.  A sequence
  * is in one group at most.  With n_groups = 0 nothing is written.  Where
- * qb_paged_decode_grouped_fp8_whole(hq, hkv, min(group_step, n_groups), ...) says so -- many groups, keys in
- * one split each -- a CTA takes members through all their keys and the workspace is not needed.  workspace: qb_paged_decode_grouped_fp8_workspace_bytes(batch, hq, shared_splits + own_splits),
+ * qb_paged_decode_grouped_fp8_whole(hq, hkv, min(group_step, n_groups), ...) says so -- keys in one split
+ * each, few for the number of groups -- a CTA takes members through all their keys and the workspace is
+ * not needed.  workspace: qb_paged_decode_grouped_fp8_workspace_bytes(batch, hq, shared_splits + own_splits),
  * any contents. */
 int qb_paged_decode_attn_grouped_fp8(const void* q, int64_t q_stride, const void* k_cache,
                                      const void* v_cache, const float* k_scale, const float* v_scale,

@@ -612,12 +612,15 @@ decode_fp8_kernel(const __grid_constant__ DecodeMaps maps, DecodeP p) {
   decode_work<NTO, false, false>(p, maps, pages, smem, base, w, kvh, nullptr, b, 0, 0);
 }
 
-// From this many CTAs on (24 groups of eight heads) whole groups are faster than splits that are joined: us per
-// call, whole / split, of 24, 48 and 64 groups of eight with 64 to 512 shared keys: 20 / 32, 33 / 55, 41 / 72 with up
-// to 100 own keys a member, 46 / 54, 80 / 91, 103 / 119 with up to 700.  Below, the longest CTA decides: 8 groups
-// 14 / 15 and 34 / 27.
-constexpr int DC_WHOLE_CTAS = 384;
-// Many groups: a CTA takes up to eight query rows of a group -- four members, where two query heads share a
+// Whole groups are taken where the longest CTA's keys are no more than this for the number of CTAs: with few CTAs
+// its length is the call's, with many its fewer beginnings and ends count.  Measured (us per call, whole / split;
+// eight heads, so 16 CTAs a group of eight; the keys a CTA has at most):
+//    2 groups, 768 keys 11.3 / 12.7, 1280 keys 13.4 / 13.0, 1792 keys 16.5 / 13.1
+//    8 groups, 832 keys 12.9 / 14.6, 1344 keys 18.6 / 18.2, 3328 keys 34 / 27
+//   16 groups, 1344 keys 21.9 / 27.6, 1792 keys 25.2 / 29.7, 3328 keys 43 / 39
+//   24 groups, 1024 keys 20 / 32, 3328 keys 46 / 54;   64 groups, 1024 keys 41 / 72, 3328 keys 103 / 119
+constexpr int DC_WHOLE_KEYS = 512, DC_WHOLE_KEYS_PER_CTA = 8;
+// Whole groups: a CTA takes up to eight query rows of a group -- four members, where two query heads share a
 // kv head -- through the shared keys and then through each member's own, one after another in the same ring
 // and the same running sums; own tiles count for their member's rows only.  Nothing is left to join, and what a
 // CTA needs to begin and to end (as long as four tiles of keys take) is paid once for four members.
@@ -781,8 +784,9 @@ extern "C" int qb_paged_decode_grouped_fp8_whole(int hq, int hkv, int group_step
                                                  int own_tokens, int own_splits) {
   if (shared_splits != 1 || own_splits != 1 || hkv < 1 || hq / hkv < 1 || hq / hkv > KV8_MAX_GROUP) return 0;
   const int chunk = members_per_cta(hq / hkv);
-  return (int64_t)group_step * ((8 + chunk - 1) / chunk) * hkv >= DC_WHOLE_CTAS &&
-         shared_tokens + (int64_t)chunk * own_tokens <= DC_MAX_TILES * KV8_BLOCK;
+  const int64_t ctas = (int64_t)group_step * ((8 + chunk - 1) / chunk) * hkv;
+  const int64_t keys = shared_tokens + (int64_t)chunk * own_tokens;
+  return ctas > 0 && keys <= DC_MAX_TILES * KV8_BLOCK && keys <= DC_WHOLE_KEYS + DC_WHOLE_KEYS_PER_CTA * ctas;
 }
 
 extern "C" int qb_paged_decode_attn_grouped_fp8(

@@ -625,7 +625,7 @@ def qk_norm_rope_store_fp8(qkv, positions, cos_sin, q_norm_w, k_norm_w, eps, hq,
     if unit != 1 or ld < width or ld % 8 or qkv.data_ptr() % 16:
         qkv, ld = qkv.contiguous(), width
     positions, q_norm_w, k_norm_w = positions.contiguous(), q_norm_w.contiguous(), k_norm_w.contiguous()
-    q = qkv.new_empty((T, hq, 128))
+    q = qkv.new_empty(T, hq, 128)
     err, stream = _launch_ptrs(dev)
     check(lib().qb_qk_norm_rope_store_fp8(
         qkv.data_ptr(), T, ld, hq, hkv, 128, positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0],
@@ -659,7 +659,7 @@ def _grouped_whole(*sizes):
 def grouped_decode_plan_fp8(batch, n_groups, hq, hkv, max_shared, max_own, slots=444):
     """(group_step, shared_tokens, shared_splits, own_tokens, own_splits) of
     :func:`paged_decode_attention_grouped_fp8`; ``n_groups``: the live groups expected.  One split of each where
-    there are groups enough for a CTA to take members through all their keys."""
+    a CTA takes members through all their keys."""
     up = lambda n: math.ceil(max(1, n) / 64) * 64  # noqa: E731
     whole = max(1, n_groups), up(max_shared), 1, up(max_own), 1
     if _grouped_whole(hq, hkv, *whole):
@@ -683,7 +683,7 @@ def _fp8_workspace(what, workspace, q, batch, hq, n_slots, grouped=False):
     f = lib().qb_paged_decode_grouped_fp8_workspace_bytes if grouped else lib().qb_paged_decode_fp8_workspace_bytes
     nbytes = f(batch, hq, n_slots)
     if workspace is None:
-        workspace = q.new_empty((nbytes // 2,))
+        workspace = q.new_empty(nbytes // 2)
     elif workspace.numel() * workspace.element_size() < nbytes or workspace.data_ptr() % 16 \
             or not workspace.is_contiguous():
         raise NativeError(f"{what}: the workspace is too small for {n_slots} splits, or not aligned")
@@ -736,7 +736,7 @@ def paged_decode_attention_grouped_fp8(q, k_cache, v_cache, k_scale, v_scale, bl
     out = _fp8_out(what, out, q)
     if n_groups == 0:
         return out.zero_()
-    whole = _grouped_whole(hq, hkv, min(group_step, n_groups), *plan[1:])  # many groups: one kernel, no partial outputs
+    whole = _grouped_whole(hq, hkv, min(group_step, n_groups), *plan[1:])  # one kernel, no partial outputs
     ws, ws_ptr = (None, 0) if whole else _fp8_workspace(what, workspace, q, B, hq, shared_splits + own_splits, grouped=True)
     err, stream = _launch_ptrs(dev)
     check(lib().qb_paged_decode_attn_grouped_fp8(
