@@ -6,7 +6,8 @@
 // key's 256 bytes of codes are read once and meet hq / hkv query rows (a group's members times that),
 // so the bound is HBM: 2 * (128 + 1/16) bytes a key and kv head.
 //
-// A CTA takes one kv head of one sequence (or of a group's shared prefix) and a range of its keys.  A
+// A CTA takes one kv head of one sequence (or of a group's shared prefix) and a range of its keys; where there
+// are groups enough, one of several members and all their keys (decode_whole_fp8_kernel).  A
 // producer warp brings 64-key tiles (8 KB of K, 8 KB of V: one block's codes lie in a row) by TMA into a
 // ring of stages; four warps take 16 keys of every tile each and never wait for one another: each keeps
 // its own running reference, sum and output, joined once at the end.
@@ -28,7 +29,7 @@
 //   512 sequences of 64 to 1024 keys      97.3 us, 556 MB: 5.7 TB/s
 //   16 sequences of 2048 to 32768 keys      88 us, 458 MB: 5.2 TB/s (ragged lengths: CTAs end at different times);
 //                                         as many bytes in equal lengths: 6.5 TB/s and more
-//   one sequence of 700 keys              8.3 us: the chain of lookups (length, page, scale), copy and join
+//   one sequence of 700 keys              8.4 us: the chain of lookups (length, page, scale), copy and join
 //   64 groups of 8, 64 to 512 shared and 170 to 512 own keys   82 us, 404 MB: 4.9 TB/s
 // What a CTA needs before its first and after its last tile is as long as two to four tiles, and three CTAs of an
 // SM hide it only in part: 4096 CTAs of one key each take 21 us.  Longer work a CTA (decode_whole_fp8_kernel) pays

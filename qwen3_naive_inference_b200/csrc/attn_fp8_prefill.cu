@@ -699,7 +699,8 @@ extern "C" int qb_attn_paged_prefill_fp8(const void* q, int64_t q_stride, const 
   PrefillP p{};
   p.q = (const bf16*)q; p.q_stride = q_stride; p.k = (const uint8_t*)k_cache; p.v = (const uint8_t*)v_cache;
   p.ks = k_scale; p.vs = v_scale; p.num_blocks = num_blocks; p.bt = block_tables; p.bt_stride = bt_stride;
-  p.bt_width = bt_width; p.table_keys = (int)std::min<int64_t>((int64_t)bt_width * KV8_PAGE, INT32_MAX); p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k; p.batch = batch; p.tiles = tile_info;
+  p.bt_width = bt_width; p.table_keys = (int)std::min<int64_t>((int64_t)bt_width * KV8_PAGE, INT32_MAX);
+  p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k; p.batch = batch; p.tiles = tile_info;
   p.hq = hq; p.hkv = hkv;
   p.pos_per_cta = 16;
   while (p.pos_per_cta * 2 * (hq / hkv) <= 2 * PF_ROWS) p.pos_per_cta *= 2;
