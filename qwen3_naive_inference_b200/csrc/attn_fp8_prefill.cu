@@ -17,11 +17,13 @@
 // S_x has two buffers in TMEM, so the scores of block j + 1 are ready when the softmax is done with block
 // j: the softmax warps never wait for the tensor pipe.  TMEM: four S buffers of 64 columns, O_A, O_B of 128.
 // Q enters as halves scaled by a power of two per row (its largest value in [2^9, 2^10): bf16 values stay
-// exact down to 2^-23 of it); ks and the softmax scale meet the fp32 scores.  P = 2^(x - ref) is rounded
-// to halves: ref is set 4 below the largest score and moved when a score passes it by 12.  vs joins P
-// relative to a reference of its own, which follows the blocks' scales (moved when one is over 8 times it),
-// so O counts in units of that reference; a block whose scale is 2^-10 of it or less is weighed after the
-// sum l has taken its probabilities.
+// exact down to 2^-23 of it); ks and the softmax scale meet the fp32 scores.  What meets V is the
+// probability weighed by its block's scale, P = vs 2^(x - ref) = 2^(x + log2 vs - ref), rounded to halves:
+// a row's ref is set 7 below the largest x + log2 vs and moved when one passes it by 15, so P stays below 2^15
+// and loses nothing above 2^-31 of the largest share, however far apart the blocks' scales are.  The sum l
+// has a reference of its own, moved by the same rule on x alone; a tile joins it as sum(P) 2^(ref - log2 vs - lref).
+// A tile whose shares are all below 2^-100 of the reference (a block of zeros under the smallest scale, say) may
+// still hold probability: it gives P = 0 and its sum is taken from 2^(x - lref).
 // Keys behind a row's last one take a score of -inf; their V must not count either, so codes past the
 // sequence are zeroed and, in tiles that some row sees in part, NaN codes of V are zeroed too and their
 // keys noted: a row that does attend such a key becomes NaN.
@@ -56,12 +58,13 @@ constexpr int PF_KV_HALF = PF_KEYS * 64 * 2, PF_KV_TILE = 2 * PF_KV_HALF;
 constexpr int PF_STAGES = 4;
 constexpr int PF_Q = 0, PF_K = 2 * PF_Q_TILE, PF_V = PF_K + PF_STAGES * PF_KV_TILE;
 constexpr int PF_META = PF_V + PF_STAGES * PF_KV_TILE;
-constexpr int PF_SLOTS = 8, PF_SLOT = 8;           // tiles whose scales are held, words of one
+constexpr int PF_SLOTS = 8, PF_SLOT = 4;           // tiles whose scales are held, words of one
 constexpr int PF_BARS = 4 * PF_STAGES + 20;
 // barriers; TMEM slot, abort flag; row factors; per slot the tile's scales and NaN keys
 constexpr int PF_SMEM = PF_META + PF_BARS * 8 + 8 + 2 * PF_ROWS * 4 + PF_SLOTS * PF_SLOT * 4 + 1024 /*align*/;
 constexpr uint32_t PF_COL_S = 0, PF_COL_O = 256;   // S: + 128 * query tile + 64 * buffer; O: + 128 * query tile
-constexpr float PF_HEAD = 4.f, PF_SLACK = 12.f, PF_VSLACK = 8.f, PF_VLOW = 1.f / 1024;
+constexpr float PF_HEAD = 7.f, PF_SLACK = 15.f;    // ref = largest - 7; moves when one is above ref + 15
+constexpr float PF_APART = -100.f;                 // log2 of a share of O below which P is taken as zero
 constexpr int PF_WS_ROW = KV8_D + 4;
 
 // kind::f16, D fp32, A and B f16, M = 128; S: N = 64, both K-major; O: N = 128, B (V) MN-major.
@@ -140,12 +143,10 @@ struct PrefillSmem {
   QB_DEVICE uint32_t* tmem_slot() const { return reinterpret_cast<uint32_t*>(ptr + PF_META + 8 * PF_BARS); }
   QB_DEVICE volatile int* abort_flag() const { return reinterpret_cast<volatile int*>(tmem_slot() + 1); }
   QB_DEVICE float* row_fac() const { return reinterpret_cast<float*>(tmem_slot() + 2); }
-  // slot of key tile j: [0] ks (negative: no such page), [1] the exponent that weighs P by vs / vref (0: it
-  // is not weighed there), [2] the factor that takes this out of the sum, [3] the factor of P after it,
-  // [4] what O is multiplied by before the tile (vref has moved), [5] vref; [6], [7] bits of NaN keys.
+  // slot of key tile j: [0] ks (negative: no such page), [1] log2 vs; [2], [3] bits of NaN keys.
   // Eight slots: a slot is written for tile j + 8 when S of j + 4 is done, so the softmax is past j + 2.
   QB_DEVICE float* scales(int j) const { return row_fac() + 2 * PF_ROWS + j % PF_SLOTS * PF_SLOT; }
-  QB_DEVICE uint32_t* nan_keys(int j) const { return reinterpret_cast<uint32_t*>(scales(j) + 6); }
+  QB_DEVICE uint32_t* nan_keys(int j) const { return reinterpret_cast<uint32_t*>(scales(j) + 2); }
 };
 
 // What a CTA works on.
@@ -176,7 +177,6 @@ QB_DEVICE void prefill_convert(const PrefillP& p, const PrefillSmem& sm, const P
   // one element half of two neighbouring keys
   const int chunk = (tid & 3) | ((tid >> 1) & 4), row0 = ((tid >> 4) << 1) | ((tid >> 2) & 1);
   const int first_masked = w.shift + w.q0 + 1;  // keys from here on are behind the first row's last one
-  float vref = 0.f;  // thread 0
   // A key tile on its way: its codes in registers (rows past the keys and tiles without a page: zero) and, in
   // thread 0, its scales.  Two tiles are, so that a tile's loads have the time of two to arrive; the page of
   // the one after them is looked up meanwhile.
@@ -213,18 +213,8 @@ QB_DEVICE void prefill_convert(const PrefillP& p, const PrefillSmem& sm, const P
     if (!mbar_wait(sm.k_empty(j), sm.phase(j) ^ 1, sm.abort_flag(), p.err)) return false;
     if (tid == 0) {
       float* sc = sm.scales(j);
-      sc[4] = 1.f;
-      if (c.vs > vref * PF_VSLACK) {
-        sc[4] = vref / c.vs;
-        vref = c.vs;
-      }
-      const float rv = vref > 0.f ? c.vs / vref : 0.f;
-      const bool folded = rv >= PF_VLOW;
       sc[0] = c.ks;
-      sc[1] = folded ? log2f(rv) : 0.f;
-      sc[2] = folded ? 1.f / rv : 1.f;
-      sc[3] = folded ? 1.f : rv;
-      sc[5] = vref;
+      sc[1] = log2f(c.vs);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) put_codes(sm.k(j), row0 + 16 * i, chunk, c.k[i]);
@@ -399,7 +389,8 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
     }
     return;
   }
-  float ref = -INFINITY, l = 0.f, vref = 0.f;
+  // O counts in units of 2^ref, l in units of 2^lref
+  float ref = -INFINITY, lref = -INFINITY, l = 0.f;
   for (int j = 0; ok && j < n; ++j) {
     // tcgen05 loads and stores are warp-collective: every decision that leads to them is warp-uniform
     if (!__all_sync(0xffffffffu, mbar_wait(sm.s_full(x, j), sm.buffer_phase(j), ab, p.err))) {
@@ -412,8 +403,7 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
     tmem_ld32_nowait(s_at, v);
     tmem_ld32_nowait(s_at + 32, v + 32);
     const float* sc = sm.scales(j);
-    const float ks = sc[0], weight = sc[1], unweigh = sc[2], after = sc[3], vfac = sc[4];
-    vref = sc[5];
+    const float ks = sc[0], lvs = sc[1];
     const int seen = ks < 0.f ? 0 : last - (w.begin + j * PF_KEYS) + 1;  // keys of the tile that the row sees
     const float f = fmaxf(fac * ks, FLT_MIN);  // not zero: -inf (a key not seen) has to stay -inf
     const bool whole = __all_sync(0xffffffffu, seen >= PF_KEYS);
@@ -434,15 +424,14 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
       for (int c = 0; c < 4; ++c) top[c] = max3(top[c], __uint_as_float(v[i + c]), __uint_as_float(v[i + 4 + c]));
 #pragma unroll
     for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(v[60 + c]));
-    const float mt = f * fmaxf(max3(top[0], top[1], top[2]), top[3]);
-    const bool need = mt > ref + PF_SLACK;
-    if (__any_sync(0xffffffffu, need) || vfac != 1.f) {
-      float a = vfac;
+    const float mt = f * fmaxf(max3(top[0], top[1], top[2]), top[3]), mw = mt + lvs;  // largest score, plain and weighed
+    const bool need = mw > ref + PF_SLACK;
+    if (__any_sync(0xffffffffu, need)) {
+      float a = 1.f;
       if (need) {
-        const float to = mt - PF_HEAD, alpha = ref == -INFINITY ? 0.f : fast_exp2(ref - to);
+        const float to = mw - PF_HEAD;
+        a = ref == -INFINITY ? 0.f : fast_exp2(ref - to);
         ref = to;
-        l *= alpha;
-        a *= alpha;
       }
       if (j > 0) {  // O holds the tiles before: wait for the last of them, weigh them anew
         if (!__all_sync(0xffffffffu, mbar_wait(sm.pv_done(x, j - 1), sm.buffer_phase(j - 1), ab, p.err))) {
@@ -460,15 +449,24 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
         }
       }
     }
-    const float shift = weight - (ref == -INFINITY ? 0.f : ref);
+    if (mt > lref + PF_SLACK) {
+      const float to = mt - PF_HEAD;
+      l *= lref == -INFINITY ? 0.f : fast_exp2(lref - to);
+      lref = to;
+    }
+    // does the row see keys here whose shares of O are all next to nothing?  (ref is -inf while every vs was zero)
+    const bool apart = mt > -INFINITY && !(mw - ref >= PF_APART);
+    const float shift = apart ? -lref : lvs - (ref == -INFINITY ? 0.f : ref);
+    // takes a tile's sum to units of 2^lref; at most 2^115 where the tile is not `apart`
+    const float to_l = apart ? 1.f : mt == -INFINITY ? 0.f : fast_exp2(ref - lvs - lref);
     const float2 ff = make_float2(f, f), ss = make_float2(shift, shift);
     float2 sum[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) sum[c] = make_float2(0.f, 0.f);
     uint32_t pk[32];
-    // `after` is the same for every thread of the CTA.  Two loops, so that a score is not needed again once
-    // it is a probability: its register is free for the ones that follow.
-    if (after == 1.f) {
+    // Two loops, so that a score is not needed again once it is a probability: its register is free for the
+    // ones that follow.
+    if (!__any_sync(0xffffffffu, apart)) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         float2 y = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ff, ss);
@@ -477,26 +475,29 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
         sum[i & 3] = add2(sum[i & 3], y);
         pk[i] = pack_half2(y.x, y.y);
       }
-    } else {  // weigh in fp32, after the sum
+    } else {  // some rows' probabilities go to the sum only
+      const float keep = apart ? 0.f : 1.f;
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         float2 y = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ff, ss);
         y.x = fast_exp2(y.x);
         y.y = fast_exp2(y.y);
         sum[i & 3] = add2(sum[i & 3], y);
-        pk[i] = pack_half2(y.x * after, y.y * after);
+        pk[i] = pack_half2(y.x * keep, y.y * keep);
       }
     }
     tmem_st32(s_at, pk);
     const float2 s2 = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
-    l = fmaf(s2.x + s2.y, unweigh, l);
+    l = fmaf(s2.x + s2.y, to_l, l);
     tmem_st_wait();
     tc_fence_before();
     mbar_arrive(sm.p_ready(x, j));
   }
   if (!ok || !__all_sync(0xffffffffu, mbar_wait(sm.o_last(x), 0, ab, p.err))) return;
   tc_fence_after();
-  float inv = l == 0.f ? 0.f : vref / l;
+  // 2^(ref - lref) / l in two factors: value scales reach both ends of the exponent range
+  const float units = ref == -INFINITY ? 0.f : ref - lref, half = rintf(0.5f * units), back = exp2f(half);
+  float inv = l == 0.f ? 0.f : exp2f(units - half) / l;
   // NaN values that the converters took out of the tiles some row sees in part (every V has been read)
   for (int j = max(0, w.shift + w.q0 + 1 - w.begin) / PF_KEYS; j < n; ++j)
 #pragma unroll
@@ -518,21 +519,21 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         reinterpret_cast<float4*>(ws + c)[i] =
-            make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
-                        __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
+            make_float4(__uint_as_float(o[4 * i]) * inv * back, __uint_as_float(o[4 * i + 1]) * inv * back,
+                        __uint_as_float(o[4 * i + 2]) * inv * back, __uint_as_float(o[4 * i + 3]) * inv * back);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint4 u;
-        u.x = pack_bf16x2(__uint_as_float(o[8 * i + 0]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
-        u.y = pack_bf16x2(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
-        u.z = pack_bf16x2(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
-        u.w = pack_bf16x2(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
+        u.x = pack_bf16x2(__uint_as_float(o[8 * i + 0]) * inv * back, __uint_as_float(o[8 * i + 1]) * inv * back);
+        u.y = pack_bf16x2(__uint_as_float(o[8 * i + 2]) * inv * back, __uint_as_float(o[8 * i + 3]) * inv * back);
+        u.z = pack_bf16x2(__uint_as_float(o[8 * i + 4]) * inv * back, __uint_as_float(o[8 * i + 5]) * inv * back);
+        u.w = pack_bf16x2(__uint_as_float(o[8 * i + 6]) * inv * back, __uint_as_float(o[8 * i + 7]) * inv * back);
         reinterpret_cast<uint4*>(out + c)[i] = u;
       }
     }
   }
-  if (live && p.n_splits > 1) ws[KV8_D] = l == 0.f ? -INFINITY : ref + log2f(l);
+  if (live && p.n_splits > 1) ws[KV8_D] = l == 0.f ? -INFINITY : lref + log2f(l);
 }
 
 __global__ void __launch_bounds__(PF_THREADS, 1)

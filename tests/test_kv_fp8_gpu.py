@@ -633,6 +633,86 @@ def test_prefill_shapes_reported(cuda):
         check_attention(out[:, h], *attend(q[:, h], [kv], 0.1))
 
 
+# ------------------------------------------------------------------------------------------ value scales
+def leaning_cache(g, num_blocks, hkv, table, blocks, value_scale):
+    """random_cache whose keys in the token blocks `blocks` of the sequence `table` score high where element 0
+    of a query is positive and all others low; `value_scale`: of the blocks' values, by token block."""
+    k, v, ks, vs = random_cache(g, num_blocks, hkv)
+    ks[:] = 2.0 ** -6
+    k[..., 0] = torch.tensor(-448.0).to(F8)
+    for i in range(4 * len(table)):
+        page, sub = int(table[i // 4]), i % 4
+        vs[page, :, sub] = value_scale(i)
+        if i in blocks:
+            k[page, :, sub * BLOCK:(sub + 1) * BLOCK, 0] = torch.tensor(448.0).to(F8)
+    return k, v, ks, vs
+
+
+# The keys' lead is 2 * 0.1 * 7 * q0 (natural units): 2.02 bits of probability for each unit of q0.
+VALUE_SCALES = [
+    # blocks that lead, their lead in bits, exponents of the value scale of those blocks and of the others
+    ([5], 161, -20, 0), ([5], 161, -24, 0), ([5], 161, -30, 0), ([5], 161, -60, 0), ([5], 161, -90, 0),
+    ([0], 161, -30, 0), ([1, 3, 5, 7, 9], 161, -30, 0), ([1, 3, 5, 7, 9], 161, -60, 30), ([9], 60, -20, -4),
+    # probabilities of 2^-30 and less that outweigh the others by their values
+    ([0, 1, 2, 3, 4, 6, 7, 8, 9, 10, 11], 30, -30, 30), ([0, 2, 4, 6, 8, 10], 40, 0, 60), ([2], 40, 0, 40),
+    ([4], 30, -126, 4), ([4], 100, -126, 100),
+    # values near the end of the type's range
+    ([3], 20, 119, 119), ([3], 20, -120, -120), ([3], 20, -60, 115),
+]
+
+
+def value_scale_case(lead, bits, small, other, rows=40, n=700):
+    """(q, cache, table, per head the 64-bit keys and values) of one sequence whose last rows are queries."""
+    g = gen(700 + bits + len(lead))
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32)
+    cache = leaning_cache(g, 4, 2, table[0], lead, lambda i: 2.0 ** (small if i in lead else other))
+    q = torch.randn(rows, 4, D, generator=g)
+    q[:, :, 0] = bits / 2.02
+    kv = [[rows_of(values(cache[i], cache[i + 2]), table[0], 0, n, h // 2) for i in (0, 1)] for h in range(4)]
+    return q.to(BF), cache, table, kv
+
+
+def zero_block_cases():
+    """Blocks whose values are all zero, under the smallest scale and under a scale of zero."""
+    for zero in (2.0 ** -126, 0.0):
+        for blocks, big in (([0, 1, 6], 0), ([1, 3, 5, 7, 9], 110), (list(range(10)), -20)):
+            q, (k, v, ks, vs), table, _ = value_scale_case(blocks, 0, 0, big)
+            for i in blocks:
+                v.view(torch.uint8)[int(table[0, i // 4]), :, i % 4 * 64:i % 4 * 64 + 64] = 0
+                vs[int(table[0, i // 4]), :, i % 4] = zero
+            kv = [[rows_of(values(*c), table[0], 0, 700, h // 2) for c in ((k, ks), (v, vs))] for h in range(4)]
+            yield q, (k, v, ks, vs), table, kv, f"zeros under {zero} in {blocks}:"
+
+
+def check_prefill_values(dev, q, cache, table, kv, msg=""):
+    """A sequence whose last rows are queries: many copies side by side take one split, one with room for
+    more keys in its table takes several."""
+    rows, n = q.shape[0], kv[0][0].shape[0]
+    args = on(dev, *cache)
+    for copies, width in ((64, 3), (1, 24)):
+        assert (ops.prefill_split_plan_fp8(copies, copies * rows, rows, width * PAGE, 4, 2)[1] > 1) == (copies == 1)
+        cu_q, cu_k = (torch.arange(copies + 1, dtype=torch.int32, device=dev) * i for i in (rows, n))
+        t = torch.cat([table, torch.full((1, width - 3), -1, dtype=torch.int32)], 1).to(dev).repeat(copies, 1)
+        out = ops.attention_paged_prefill_fp8(q.to(dev).repeat(copies, 1, 1), *args, cu_q, cu_k, rows, t, 0.1)
+        assert torch.equal(out[:rows], out[-rows:])
+        for h in range(4):
+            check_attention(out[:rows, h], *attend(q[:, h], [kv[h]], 0.1, n - rows), f"{msg} {copies} copies, head {h}")
+    ops.check_device_errors()
+
+
+@pytest.mark.parametrize("lead,bits,small,other", VALUE_SCALES)
+def test_prefill_weighs_value_scales_with_the_probabilities(cuda, lead, bits, small, other):
+    """Blocks of values whose scales are far apart, where the probabilities and not the scales alone say which
+    of them an output is made of.  What is rounded to halves is a probability weighed by its block's scale
+    against a reference that follows the largest of those, so the bound is that of any other call."""
+    check_prefill_values(cuda, *value_scale_case(lead, bits, small, other))
+
+
+def test_prefill_value_blocks_of_zeros_take_their_probability(cuda):
+    for q, cache, table, kv, msg in zero_block_cases():
+        check_prefill_values(cuda, q, cache, table, kv, msg)
+
+
 # ------------------------------------------------------------------------------------------ store
 def scale_for(top):
     if top == 0:
