@@ -18,7 +18,14 @@
 //                  a score passes it by 15: P stays below 2^15 and loses nothing above 2^-31 of the largest.
 //   O^T += vs V^T P^T   the 128 head elements are the M rows (8 tiles), the warp's 16 keys the K dimension,
 //                  so a tile's product is one mma per 16 elements: vs, one number a tile, joins with the
-//                  fp32 accumulator, whatever the scales of other tiles are.
+//                  fp32 accumulator.
+// Where a CTA's tiles have scales more than 2^8 apart, a probability that is nothing beside the largest may still
+// make the output (and near the ends of the exponent range vs P V leaves it).  The producer, which has the scales in
+// hand, sees it; the CTA then writes nothing and takes a second pass, which weighs before it rounds:
+// P = 2^(x + log2 vs - oref), where oref follows the largest x + log2 vs as ref does x, O counts in units of 2^oref,
+// and the sum takes sum(P) 2^(oref - log2 vs - ref).  That form for all CTAs cost 10% (512 sequences of up to 1024
+// keys 98 -> 109 us), a choice between the two inside the loop 3%; the second pass costs calls that do not take it
+// 0.2% (plain) and 2% (64 groups 83.0 -> 84.6, five small groups 12.2 -> 12.5).
 // The order of head elements and keys inside a product is free, so every operand comes straight from
 // 16-byte shared-memory reads (conflict-free under the TMA swizzle) without a transpose but for the
 // byte pairs of V (prmt) and P (movmatrix).
@@ -47,10 +54,20 @@ constexpr int DC_STAGE_BYTES = 2 * KV8_TILE;       // K then V
 constexpr int DC_MAX_TILES = 128;                  // of one CTA's range (8192 keys)
 constexpr int DC_WS_ROW = KV8_D + 4;               // workspace row: O / l, then ref + log2 l
 constexpr int DC_O_ROW = KV8_D + 4;                // shared-memory row of a warp's output (padded)
-constexpr int DC_META = DC_MAX_TILES * 16 + (2 * DC_STAGES + 1) * 8 + 8 + 2 * DC_WARPS * 16 * 4;
+constexpr int DC_META = DC_MAX_TILES * 16 + (2 * DC_STAGES + 1) * 8 + 8 + (3 * DC_WARPS * 16 + 2) * 4;
+constexpr int DC_MOST = (2 * DC_STAGES + 2) * 8 + DC_MAX_TILES * 16 + 3 * DC_WARPS * 16 * 4;  // where `most_of` lies in it
+constexpr int DC_LEFT = DC_MOST + 4;  // set where a work's scales were far apart
 constexpr int DC_SMEM = DC_STAGES * DC_STAGE_BYTES + DC_META + 1024 /*align*/;
 static_assert(DC_WARPS * 16 * DC_O_ROW * 4 <= DC_STAGES * DC_STAGE_BYTES, "the join reuses the stages");
 constexpr float DC_HEAD = 7.f, DC_SLACK = 15.f;    // ref = max - 7; moves when a score is above ref + 15
+// Largest ratio of a CTA's scales, and the range of their largest, without weighing before rounding: a P that is lost
+// (2^-32 of the largest) is then at most 2^-24 of the output's largest share, and |O| below 2^15 * 448 * 8192 vs.
+constexpr float DC_NEAR = 256.f, DC_VS_LEAST = 0x1p-100f, DC_VS_MOST = 0x1p60f;
+// Weighed, a tile whose scale is less than 2^-50 of the largest (a block of zeros under the smallest scale, say) may
+// hold probability although its P, as small as 2^-126, does not: its sum is taken from 2^(x - ref).  Within 2^50
+// a P below 2^-100 has x - ref below -42: with x', vs' of the key that set oref, oref is at most x' + log2 vs' - 7,
+// and x' at most ref + 15.
+constexpr float DC_APART = 0x1p-50f;
 
 struct DecodeP {
   const bf16* q;
@@ -146,10 +163,111 @@ QB_DEVICE void find_pages(const DecodeP& p, int table, int64_t begin, int tiles,
   }
 }
 
+// The scores x of a tile into P (pb, B fragments), with the running references, sums and outputs moved along.
+template <int NT>
+QB_DEVICE void plain_tile(const float (&x)[NT][4], float (&ref)[NT][2], float (&l)[NT][2], float (&o)[NT][8][4],
+                          uint32_t (&pb)[NT][2]) {
+  bool far = false;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+    far |= fmaxf(x[nt][0], x[nt][2]) > ref[nt][0] + DC_SLACK || fmaxf(x[nt][1], x[nt][3]) > ref[nt][1] + DC_SLACK;
+  if (__any_sync(0xffffffffu, far)) {  // the first tile, then rarely: move the reference, scale what is there
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float m = fmaxf(x[nt][c], x[nt][c + 2]);
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        if (m > ref[nt][c] + DC_SLACK) {
+          const float now = m - DC_HEAD, alpha = dc_exp2(ref[nt][c] - now);
+          ref[nt][c] = now;
+          l[nt][c] *= alpha;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            o[nt][k][c] *= alpha;
+            o[nt][k][c + 2] *= alpha;
+          }
+        }
+      }
+  }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const float r0 = ref[nt][0] == -INFINITY ? 0.f : ref[nt][0], r1 = ref[nt][1] == -INFINITY ? 0.f : ref[nt][1];
+    const float p0 = dc_exp2(x[nt][0] - r0), p1 = dc_exp2(x[nt][1] - r1);
+    const float p2 = dc_exp2(x[nt][2] - r0), p3 = dc_exp2(x[nt][3] - r1);
+    l[nt][0] += p0 + p2;
+    l[nt][1] += p1 + p3;
+    pb[nt][0] = movmatrix_trans(pack_half2(p0, p1));
+    pb[nt][1] = movmatrix_trans(pack_half2(p2, p3));
+  }
+}
+// The same with P weighed by the tile's scale before it is rounded; `orefs`: the warp's references of O, by row.
+template <int NT>
+QB_DEVICE void weigh_tile(const float (&x)[NT][4], float vs, float most, float* orefs, float (&ref)[NT][2],
+                          float (&l)[NT][2], float (&o)[NT][8][4], uint32_t (&pb)[NT][2]) {
+  const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+  const float lvs = log2f(vs);
+  const bool apart = vs < most * DC_APART || vs == 0.f;  // the same for the whole warp
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float y[4];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float m = fmaxf(x[nt][c], x[nt][c + 2]), at = orefs[8 * nt + 2 * t + c];
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+      if (m > ref[nt][c] + DC_SLACK) {
+        l[nt][c] *= dc_exp2(ref[nt][c] - (m - DC_HEAD));
+        ref[nt][c] = m - DC_HEAD;
+      }
+      if (m + lvs > at + DC_SLACK) {
+        const float now = m + lvs - DC_HEAD, alpha = dc_exp2(at - now);
+        at = now;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          o[nt][k][c] *= alpha;
+          o[nt][k][c + 2] *= alpha;
+        }
+      }
+      __syncwarp();
+      if (g == 0) orefs[8 * nt + 2 * t + c] = at;
+      // (`at` is -inf where no score, or none with a scale, has come: P is zero all the same)
+      const float r = (at == -INFINITY ? 0.f : at) - lvs, lr = ref[nt][c] == -INFINITY ? 0.f : ref[nt][c];
+      y[c] = dc_exp2(x[nt][c] - r);
+      y[c + 2] = dc_exp2(x[nt][c + 2] - r);
+      if (apart) l[nt][c] += dc_exp2(x[nt][c] - lr) + dc_exp2(x[nt][c + 2] - lr);
+      else l[nt][c] = fmaf(y[c] + y[c + 2], at == -INFINITY ? 0.f : dc_exp2(r - lr), l[nt][c]);
+    }
+    pb[nt][0] = movmatrix_trans(pack_half2(y[0], y[1]));
+    pb[nt][1] = movmatrix_trans(pack_half2(y[2], y[3]));
+  }
+  __syncwarp();
+}
+
+// Four elements of a row from the warps' outputs `so`, in units of 2^oref, and the row's sum in units of 2^m.
+QB_DEVICE float4 join_weighed(const float* so, const float* orefs, float m, float sum) {
+  float top = -INFINITY;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < DC_WARPS; ++k) top = fmaxf(top, orefs[k * 16]);
+  for (int k = 0; k < DC_WARPS; ++k) {
+    const float at = orefs[k * 16], f = at == -INFINITY ? 0.f : exp2f(at - top);
+    const float4 x = *reinterpret_cast<const float4*>(so + k * 16 * DC_O_ROW);
+    acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+  }
+  // 2^(top - m) / sum in two factors: value scales reach both ends of the exponent range
+  const float units = top == -INFINITY ? 0.f : top - m, half = rintf(0.5f * units), back = exp2f(half);
+  const float inv = sum == 0.f ? 0.f : exp2f(units - half) / sum;
+  return make_float4(acc.x * inv * back, acc.y * inv * back, acc.z * inv * back, acc.w * inv * back);
+}
+
 // One CTA: the work `w` of kv head `kvh`; NT tiles of eight query rows.  `members`: the chunk's member
 // list (shared work), `b`: the sequence (own work).  `u0` tiles and `item` works came before in this CTA.
-template <int NT, bool SHARED, bool WHOLE>
-QB_DEVICE void decode_work(const DecodeP& p, const DecodeMaps& maps, const int (&pages)[DC_LANE_TILES], uint8_t* smem,
+// Nothing is written of work whose scales are far apart (for WEIGH: are not), which `*most_of` says.  Returns the tiles.
+template <int NT, bool SHARED, bool WHOLE, bool WEIGH>
+QB_DEVICE int decode_work(const DecodeP& p, const DecodeMaps& maps, const int (&pages)[DC_LANE_TILES], uint8_t* smem,
                            uint32_t base, const Work& w, int kvh, const int32_t* members, int b, int u0, int item) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   int n = (w.end - w.begin + KV8_BLOCK - 1) / KV8_BLOCK;
@@ -166,6 +284,9 @@ QB_DEVICE void decode_work(const DecodeP& p, const DecodeMaps& maps, const int (
   float* ks_of = reinterpret_cast<float*>(part_of + DC_MAX_TILES);
   float* vs_of = ks_of + DC_MAX_TILES;
   float* join = vs_of + DC_MAX_TILES;  // [warp][16] ref, [warp][16] l
+  float* oref = join + 2 * DC_WARPS * 16;   // [warp][16], where P is weighed
+  float* most_of = oref + DC_WARPS * 16;    // the largest scale where P is weighed, else 0
+  int* left_of = reinterpret_cast<int*>(most_of + 1);
 
   if (warp == DC_WARPS) {
     // ------------------------------------------------------------ producer
@@ -263,8 +384,23 @@ QB_DEVICE void decode_work(const DecodeP& p, const DecodeMaps& maps, const int (
         vs_of[lane + 32 * j] = vs[j];
       }
     __syncwarp();
+    auto look = [&] {  // are the scales far apart?  (They are not negative: their bits order as they do.)
+      uint32_t least = ~0u, most = 0;
+#pragma unroll
+      for (int j = 0; j < DC_LANE_TILES; ++j)
+        if (lane + 32 * j < n) {  // (a tile without a page counts as a scale of zero)
+          least = min(least, __float_as_uint(vs[j]));
+          most = max(most, __float_as_uint(vs[j]));
+        }
+      const float lo = __uint_as_float(__reduce_min_sync(0xffffffffu, least)), hi = __uint_as_float(__reduce_max_sync(0xffffffffu, most));
+      const bool apart = hi > 0.f && (hi > DC_NEAR * lo || hi < DC_VS_LEAST || hi > DC_VS_MOST);
+      if (lane == 0) *most_of = apart ? hi : 0.f;
+      if (lane == 0 && apart) *left_of = 1;
+    };
+    if (WEIGH) look();
+    if (lane == 0) mbar_arrive(ready);
+    if (!WEIGH) look();  // off the way to the first tile
     if (lane == 0) {
-      mbar_arrive(ready);
       issue_to(n);
       // never leave with a copy in flight into this CTA's shared memory
       for (int i = max(0, issued - DC_STAGES); i < issued; ++i)
@@ -273,7 +409,7 @@ QB_DEVICE void decode_work(const DecodeP& p, const DecodeMaps& maps, const int (
     __syncwarp();
     __syncthreads();
     __syncthreads();
-    return;
+    return n;
   }
   // -------------------------------------------------------------- consumers
   // Q as B fragments: column g of tile nt is row nt * 8 + g; lane t holds elements 32t .. 32t+31, the two
@@ -325,6 +461,10 @@ QB_DEVICE void decode_work(const DecodeP& p, const DecodeMaps& maps, const int (
   }
   bool ok = __all_sync(0xffffffffu, mbar_wait(ready, (uint32_t)item & 1u, abort_flag, p.err));
   if (WHOLE) n = *n_of;
+  if (WEIGH) {
+    if (lane < 16) oref[warp * 16 + lane] = -INFINITY;
+    __syncwarp();
+  }
   for (int i = 0; ok && i < n; ++i) {
     const int s = (u0 + i) % DC_STAGES;
     if (!__all_sync(0xffffffffu, mbar_wait(full(s), (uint32_t)((u0 + i) / DC_STAGES) & 1u, abort_flag, p.err))) {
@@ -401,43 +541,12 @@ QB_DEVICE void decode_work(const DecodeP& p, const DecodeMaps& maps, const int (
           e4m3x4_to_half2x2(lo, va[2 * k + half][0], va[2 * k + half][1]);
           e4m3x4_to_half2x2(hi, va[2 * k + half][2], va[2 * k + half][3]);
         }
-      bool far = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        far |= fmaxf(x[nt][0], x[nt][2]) > ref[nt][0] + DC_SLACK || fmaxf(x[nt][1], x[nt][3]) > ref[nt][1] + DC_SLACK;
-      if (__any_sync(0xffffffffu, far)) {  // the first tile, then rarely: move the reference, scale what is there
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float m = fmaxf(x[nt][c], x[nt][c + 2]);
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-            if (m > ref[nt][c] + DC_SLACK) {
-              const float now = m - DC_HEAD, alpha = dc_exp2(ref[nt][c] - now);
-              ref[nt][c] = now;
-              l[nt][c] *= alpha;
-#pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                o[nt][k][c] *= alpha;
-                o[nt][k][c + 2] *= alpha;
-              }
-            }
-          }
-      }
       uint32_t pb[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float r0 = ref[nt][0] == -INFINITY ? 0.f : ref[nt][0], r1 = ref[nt][1] == -INFINITY ? 0.f : ref[nt][1];
-        const float p0 = dc_exp2(x[nt][0] - r0), p1 = dc_exp2(x[nt][1] - r1);
-        const float p2 = dc_exp2(x[nt][2] - r0), p3 = dc_exp2(x[nt][3] - r1);
-        l[nt][0] += p0 + p2;
-        l[nt][1] += p1 + p3;
-        pb[nt][0] = movmatrix_trans(pack_half2(p0, p1));
-        pb[nt][1] = movmatrix_trans(pack_half2(p2, p3));
-      }
-      const float vs = vs_of[i];
+      if (WEIGH)
+        weigh_tile<NT>(x, vs_of[i], *most_of, oref + warp * 16, ref, l, o, pb);
+      else
+        plain_tile<NT>(x, ref, l, o, pb);
+      const float vs = WEIGH ? 1.f : vs_of[i];
 #pragma unroll
       for (int k = 0; k < 8; ++k)
 #pragma unroll
@@ -475,7 +584,7 @@ QB_DEVICE void decode_work(const DecodeP& p, const DecodeMaps& maps, const int (
         dst[k] = make_float4(o[nt][2 * k][c], o[nt][2 * k][c + 2], o[nt][2 * k + 1][c], o[nt][2 * k + 1][c + 2]);
     }
   __syncthreads();
-  if (*abort_flag) return;
+  if (*abort_flag || (*most_of > 0.f) != WEIGH) return n;
   for (int i = tid; i < w.rows * 32; i += DC_WARPS * 32) {
     const int r = i >> 5, d = (i & 31) * 4;
     const int seq = row_sequence<SHARED>(p, members, b, r);
@@ -492,19 +601,25 @@ QB_DEVICE void decode_work(const DecodeP& p, const DecodeMaps& maps, const int (
       acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
     }
     if (seq < 0) continue;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (WEIGH) {
+      acc = join_weighed(so + r * DC_O_ROW + d, oref + r, m, sum);
+    } else {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
+    }
     const int64_t row = (int64_t)seq * p.hq + kvh * group + r % group;
     if (w.slot < 0) {
       uint2 u;
-      u.x = pack_bf16x2(acc.x * inv, acc.y * inv);
-      u.y = pack_bf16x2(acc.z * inv, acc.w * inv);
+      u.x = pack_bf16x2(acc.x, acc.y);
+      u.y = pack_bf16x2(acc.z, acc.w);
       *reinterpret_cast<uint2*>(p.out + row * KV8_D + d) = u;
     } else {
       float* ws = p.ws + (row * p.n_slots + w.slot) * DC_WS_ROW;
-      *reinterpret_cast<float4*>(ws + d) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      *reinterpret_cast<float4*>(ws + d) = acc;
       if (d == 0) ws[KV8_D] = sum == 0.f ? -INFINITY : m + log2f(sum);
     }
   }
+  return n;
 }
 
 // The splits of a sequence's own keys that hold any.
@@ -523,6 +638,7 @@ QB_DEVICE void decode_barriers(const DecodeMaps& maps, uint8_t* smem, uint32_t b
     }
     mbar_init(bar + 16 * DC_STAGES, 1);
     *reinterpret_cast<volatile int*>(smem + DC_STAGES * DC_STAGE_BYTES + 8 * (2 * DC_STAGES + 1)) = 0;
+    *reinterpret_cast<int*>(smem + DC_STAGES * DC_STAGE_BYTES + DC_LEFT) = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.k)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.v)) : "memory");
@@ -531,22 +647,31 @@ QB_DEVICE void decode_barriers(const DecodeMaps& maps, uint8_t* smem, uint32_t b
   }
   __syncthreads();
 }
+// The barriers of a pass that is done may be made anew.
+QB_DEVICE void barriers_back(uint8_t* smem, uint32_t base) {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0)
+    for (int i = 0; i < 2 * DC_STAGES + 1; ++i)
+      asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(base + DC_STAGES * DC_STAGE_BYTES + 8 * i) : "memory");
+}
 // The stages, which a join wrote to, go back to the copies.
 QB_DEVICE void stages_back() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncthreads();
 }
 
-// NTS, NTO: row tiles of a shared and of an own CTA (NTS = 0: no groups).
-template <int NTS, int NTO>
-__global__ void __launch_bounds__(DC_THREADS, 3)
-decode_fp8_kernel(const __grid_constant__ DecodeMaps maps, DecodeP p) {
-  extern __shared__ uint8_t smem_raw[];
-  qb_pdl_trigger();
-  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023) & ~1023u;
-  uint8_t* smem = smem_raw + (base - raw);
-  decode_barriers(maps, smem, base);
-  qb_pdl_wait();
+// Did the pass leave work to the one that weighs?
+QB_DEVICE bool left_to_weigh(const uint8_t* smem) {
+  const uint8_t* meta = smem + DC_STAGES * DC_STAGE_BYTES;
+  const bool aborted = *reinterpret_cast<const volatile int*>(meta + 8 * (2 * DC_STAGES + 1)) != 0;
+  return !aborted && *reinterpret_cast<const int*>(meta + DC_LEFT) != 0;
+}
+
+// The CTA's work, or (WEIGH) what the pass before left of it; true if some was left.  NTS, NTO: row tiles of a shared
+// and of an own CTA (NTS = 0: no groups).
+template <int NTS, int NTO, bool WEIGH>
+QB_DEVICE bool decode_pass(const DecodeMaps& maps, const DecodeP& p, uint8_t* smem, uint32_t base) {
   unsigned i = blockIdx.x;
   const int group = p.hq / p.hkv;
   int pages[DC_LANE_TILES];
@@ -580,11 +705,10 @@ decode_fp8_kernel(const __grid_constant__ DecodeMaps maps, DecodeP p) {
       if (split == p.shared_splits - 1 && w.end < keys && threadIdx.x == 0) qb_set_err(p.err, QB_DEVERR_SHAPE);
       if (!any || w.begin >= w.end || donor < 0 || donor >= p.batch) continue;
       if (item > 0) stages_back();
-      decode_work<NTS == 0 ? 1 : NTS, true, false>(p, maps, pages, smem, base, w, kvh, members, 0, u0, item);
-      u0 += (w.end - w.begin + KV8_BLOCK - 1) / KV8_BLOCK;
+      u0 += decode_work<NTS == 0 ? 1 : NTS, true, false, WEIGH>(p, maps, pages, smem, base, w, kvh, members, 0, u0, item);
       ++item;
     }
-    return;
+    return left_to_weigh(smem);
   }
   i -= p.n_shared;
   const int split = i % p.own_splits;
@@ -596,7 +720,7 @@ decode_fp8_kernel(const __grid_constant__ DecodeMaps maps, DecodeP p) {
   find_pages(p, b, max(begin, (int64_t)0), p.own_tokens / KV8_BLOCK, pages);
   if ((first < 0 || (split == p.own_splits - 1 && begin + p.own_tokens < len)) && threadIdx.x == 0)
     qb_set_err(p.err, QB_DEVERR_SHAPE);
-  if (first < 0) return;
+  if (first < 0) return false;
   Work w;
   w.rows = group;
   w.table = b;
@@ -608,9 +732,28 @@ decode_fp8_kernel(const __grid_constant__ DecodeMaps maps, DecodeP p) {
     if (p.n_slots == 1)  // no keys at all
       for (int k = threadIdx.x; k < group * KV8_D / 4; k += DC_THREADS)
         reinterpret_cast<uint2*>(p.out + ((int64_t)b * p.hq + kvh * group) * KV8_D)[k] = make_uint2(0, 0);
-    return;
+    return false;
   }
-  decode_work<NTO, false, false>(p, maps, pages, smem, base, w, kvh, nullptr, b, 0, 0);
+  decode_work<NTO, false, false, WEIGH>(p, maps, pages, smem, base, w, kvh, nullptr, b, 0, 0);
+  return left_to_weigh(smem);
+}
+template <int NTS, int NTO>
+QB_DEVICE void decode_weigh(const DecodeMaps& maps, const DecodeP& p, uint8_t* smem, uint32_t base) {
+  barriers_back(smem, base);
+  decode_barriers(maps, smem, base);
+  decode_pass<NTS, NTO, true>(maps, p, smem, base);
+}
+
+template <int NTS, int NTO>
+__global__ void __launch_bounds__(DC_THREADS, 3)
+decode_fp8_kernel(const __grid_constant__ DecodeMaps maps, const __grid_constant__ DecodeP p) {
+  extern __shared__ uint8_t smem_raw[];
+  qb_pdl_trigger();
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  decode_barriers(maps, smem, base);
+  qb_pdl_wait();
+  if (decode_pass<NTS, NTO, false>(maps, p, smem, base)) decode_weigh<NTS, NTO>(maps, p, smem, base);
 }
 
 // Whole groups are taken where the longest CTA's keys are no more than this for the number of CTAs: with few CTAs
@@ -625,27 +768,20 @@ constexpr int DC_WHOLE_KEYS = 512, DC_WHOLE_KEYS_PER_CTA = 8;
 // kv head -- through the shared keys and then through each member's own, one after another in the same ring
 // and the same running sums; own tiles count for their member's rows only.  Nothing is left to join, and what a
 // CTA needs to begin and to end (as long as four tiles of keys take) is paid once for four members.
-template <int NT>
-__global__ void __launch_bounds__(DC_THREADS, 3)
-decode_whole_fp8_kernel(const __grid_constant__ DecodeMaps maps, DecodeP p) {
-  extern __shared__ uint8_t smem_raw[];
-  qb_pdl_trigger();
-  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023) & ~1023u;
-  uint8_t* smem = smem_raw + (base - raw);
-  decode_barriers(maps, smem, base);
-  qb_pdl_wait();
+template <int NT, bool WEIGH>
+QB_DEVICE bool decode_whole_pass(const DecodeMaps& maps, const DecodeP& p, uint8_t* smem, uint32_t base) {
   unsigned i = blockIdx.x;
   const int group = p.hq / p.hkv;
   if (i >= p.n_shared) {  // a warp per sequence: zeros for those in no group
     const int64_t b = (int64_t)(i - p.n_shared) * (DC_THREADS / 32) + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
-    if (b >= p.batch) return;
+    if (b >= p.batch) return false;
     bool member = false;
     for (int k = lane; k < p.n_groups * 8; k += 32) member |= p.members[k] == (int)b;
-    if (__any_sync(0xffffffffu, member)) return;
+    if (__any_sync(0xffffffffu, member)) return false;
     for (int k = lane; k < p.hq * KV8_D / 8; k += 32)
       reinterpret_cast<uint4*>(p.out + b * p.hq * KV8_D)[k] = make_uint4(0, 0, 0, 0);
-    return;
+    return false;
   }
   const int kvh = i % p.hkv;
   i /= p.hkv;
@@ -668,10 +804,28 @@ decode_whole_fp8_kernel(const __grid_constant__ DecodeMaps maps, DecodeP p) {
     w.end = donor >= 0 && donor < p.batch ? max(0, min(keys, p.shared_tokens)) : 0;
     w.slot = -1;
     if (item > 0) stages_back();
-    decode_work<NT, true, true>(p, maps, pages, smem, base, w, kvh, members, 0, u0, item);
-    u0 += *reinterpret_cast<const int*>(smem + DC_STAGES * DC_STAGE_BYTES + 8 * (2 * DC_STAGES + 1) + 4);
+    u0 += decode_work<NT, true, true, WEIGH>(p, maps, pages, smem, base, w, kvh, members, 0, u0, item);
     ++item;
   }
+  return left_to_weigh(smem);
+}
+template <int NT>
+QB_DEVICE void decode_whole_weigh(const DecodeMaps& maps, const DecodeP& p, uint8_t* smem, uint32_t base) {
+  barriers_back(smem, base);
+  decode_barriers(maps, smem, base);
+  decode_whole_pass<NT, true>(maps, p, smem, base);
+}
+
+template <int NT>
+__global__ void __launch_bounds__(DC_THREADS, 3)
+decode_whole_fp8_kernel(const __grid_constant__ DecodeMaps maps, const __grid_constant__ DecodeP p) {
+  extern __shared__ uint8_t smem_raw[];
+  qb_pdl_trigger();
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  decode_barriers(maps, smem, base);
+  qb_pdl_wait();
+  if (decode_whole_pass<NT, false>(maps, p, smem, base)) decode_whole_weigh<NT>(maps, p, smem, base);
 }
 
 // Joins the splits of a (sequence, head): a warp each, weights 2^(lse - largest lse).  Only the splits

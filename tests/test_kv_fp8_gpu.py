@@ -713,6 +713,66 @@ def test_prefill_value_blocks_of_zeros_take_their_probability(cuda):
         check_prefill_values(cuda, q, cache, table, kv, msg)
 
 
+def check_decode_values(dev, q, cache, table, kv, msg=""):
+    """A sequence's last token: plain and grouped (512 keys shared), in one split and in several."""
+    n = kv[0][0].shape[0]
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    args = on(dev, q[-1:], *cache, table)
+    outs = [ops.paged_decode_attention_fp8(*args, i32(n - 1), 0.1, **kw)
+            for kw in ({}, {"split_tokens": 128, "max_splits": 6}, {"split_tokens": 64, "max_splits": 11})]
+    for plan in ((32, 512, 1, 192, 1), (1, 192, 3, 64, 3)):  # a CTA for all keys, and splits
+        members = torch.full((32, 8), -1, dtype=torch.int32, device=dev)
+        members[3, 0] = 0
+        shared = torch.zeros(32, dtype=torch.int32, device=dev)
+        shared[3] = 512
+        outs.append(ops.paged_decode_attention_grouped_fp8(*args, i32(n - 1), 0.1, members, shared, i32(512), plan))
+    assert ops._grouped_whole(4, 2, 32, 512, 1, 192, 1)
+    for h in range(4):
+        ref = attend(q[-1:, h], [kv[h]], 0.1)
+        for i, out in enumerate(outs):
+            check_attention(out[:, h], *ref, f"{msg} call {i} head {h}")
+    ops.check_device_errors()
+
+
+@pytest.mark.parametrize("lead,bits,small,other", VALUE_SCALES)
+def test_decode_weighs_value_scales_with_the_probabilities(cuda, lead, bits, small, other):
+    check_decode_values(cuda, *value_scale_case(lead, bits, small, other))
+
+
+def test_decode_value_blocks_of_zeros_take_their_probability(cuda):
+    for q, cache, table, kv, msg in zero_block_cases():
+        check_decode_values(cuda, q, cache, table, kv, msg)
+
+
+@pytest.mark.parametrize("plan", [(10, 192, 1, 192, 1), (10, 64, 3, 64, 3)])
+def test_grouped_value_scales_far_apart_in_some_groups(cuda, plan):
+    """CTAs that take several groups one after another, some of them with value scales far apart: those follow the
+    formula, the others keep their bits."""
+    g = gen(725)
+    groups = many_groups(g, 40, 150, 140)
+    q, k, v, ks, vs, parts, args, grp = grouped_inputs(g, 16, 8, groups, cuda)
+    assert ops._grouped_whole(16, 8, *plan) == (plan[1] == 192)
+    before = ops.paged_decode_attention_grouped_fp8(*args, 0.1, *grp, plan)
+    far, row = set(), 0
+    for i, (_, own) in enumerate(groups):
+        if i in (1, 5, 11, 12, 38):
+            far |= {parts[row + j][0] for j in range(len(own))}
+            for _, head, _, pages, _, _ in parts[row:row + len(own)]:
+                for page in {*head, *pages}:
+                    vs[page] = torch.exp2(torch.randint(-40, 40, vs[page].shape, generator=g).float())
+        row += len(own)
+    args[4] = vs.to(cuda)
+    out = ops.paged_decode_attention_grouped_fp8(*args, 0.1, *grp, plan)
+    near = [i for i in range(q.shape[0]) if i not in far]
+    assert torch.equal(out[near], before[near])
+    k64, v64 = values(k, ks), values(v, vs)
+    for r, head, s, pages, a, b in parts:
+        for h in (0, 7, 15) if r in far else ():
+            kv = [torch.cat([rows_of(c, head, 0, s, h // 2), rows_of(c, pages, a, b, h // 2)]) for c in (k64, v64)]
+            check_attention(out[r, h:h + 1], *attend(q[r, h:h + 1], [kv], 0.1), f"row {r} head {h}")
+    ops.check_device_errors()
+
+
 # ------------------------------------------------------------------------------------------ store
 def scale_for(top):
     if top == 0:
