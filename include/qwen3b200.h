@@ -257,8 +257,10 @@ size_t qb_paged_decode_grouped_fp8_workspace_bytes(int batch, int hq, int n_slot
 /* Causal attention of the query rows cu_seqlens_q over the first cu_seqlens_k keys of each sequence in
  * that cache; arguments as the paged form of qb_attn_varlen_fwd.  q and out rows q_stride / o_stride
  * elements apart (multiples of 8).  hq / hkv <= 16.  Rows in no sequence are left as they were.
- * tile_info has to hold every 64-row tile of a sequence; without it tiles_per_seq * 64 >= every Lq (rows
- * beyond are left as they were and set QB_DEVERR_SHAPE).  With n_splits > 1 the keys are split over
+ * tile_info holds the 64-row tiles (sequence, first row) to compute, all of a sequence's as a rule: rows are
+ * taken in units of 64, 128 or 256 (as many as 256 / (hq / hkv) allows), and those of a unit whose first tile is not
+ * listed are left as they were.  Without it tiles_per_seq * 64 >= every Lq (rows beyond are left as they were
+ * and set QB_DEVERR_SHAPE).  With n_splits > 1 the keys are split over
  * CTAs, split_keys (a multiple of 128) each, and joined by a second kernel; split_keys * n_splits >=
  * every Lk (keys beyond are left out and set QB_DEVERR_SHAPE); workspace:
  * qb_attn_paged_prefill_fp8_workspace_bytes(total_q, hq, n_splits), any contents. */

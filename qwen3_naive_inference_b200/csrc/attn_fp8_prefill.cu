@@ -86,7 +86,8 @@ struct PrefillP {
   const int32_t* cu_q;
   const int32_t* cu_k;
   int batch;
-  const int32_t* tiles;  // nullable [n, 2]: (sequence, first row of a 64-row tile)
+  const int32_t* tiles;  // nullable [n_tiles, 2]: (sequence, first row of a 64-row tile)
+  int n_tiles;
   int tiles_per_seq;     // without tiles: of `unit` rows
   int hq, hkv, pos_per_cta, unit;  // unit = max(64, pos_per_cta): rows a grid tile stands for
   float scale_log2;
@@ -635,7 +636,9 @@ prefill_fp8_kernel(PrefillP p) {
 }
 
 // Joins the key splits of a (row, head): a warp each, weights 2^(lse - largest lse), over the splits that
-// hold keys of the row.
+// hold keys of the row.  Rows of no tile have no partial outputs and are left as they are; the tiles of a call
+// that is split are few (fewer than the GPU has SMs, in what prefill_split_plan_fp8 splits), so a warp looks
+// through them.
 __global__ void __launch_bounds__(128)
 prefill_fp8_join_kernel(PrefillP p) {
   qb_pdl_trigger();
@@ -651,7 +654,15 @@ prefill_fp8_join_kernel(PrefillP p) {
     else hi = mid;
   }
   const int lq = p.cu_q[lo + 1] - p.cu_q[lo], lk = p.cu_k[lo + 1] - p.cu_k[lo], i = (int)row - p.cu_q[lo];
-  if (i < 0 || i >= lq || lk < lq || p.cu_q[lo + 1] > p.total_q || p.table_keys == 0) return;
+  if (p.cu_q[lo] < 0 || i < 0 || i >= lq || lk < lq || p.cu_q[lo + 1] > p.total_q || p.table_keys == 0) return;
+  bool tiled = i < (int64_t)p.tiles_per_seq * p.unit;
+  if (p.tiles) {
+    const int start = i & ~(p.unit - 1);  // of the grid tile that the row belongs to (unit is 64, 128 or 256)
+    tiled = false;
+    for (int k = lane; k < p.n_tiles; k += 32) tiled |= p.tiles[2 * k] == lo && p.tiles[2 * k + 1] == start;
+    tiled = __any_sync(0xffffffffu, tiled);
+  }
+  if (!tiled) return;
   const int n = min(p.n_splits, min(lk - lq + i, p.table_keys - 1) / p.split_keys + 1);
   const float* ws = p.ws + (row * p.hq + head) * p.n_splits * PF_WS_ROW;
   float m = -INFINITY;
@@ -701,7 +712,7 @@ extern "C" int qb_attn_paged_prefill_fp8(const void* q, int64_t q_stride, const 
   p.q = (const bf16*)q; p.q_stride = q_stride; p.k = (const uint8_t*)k_cache; p.v = (const uint8_t*)v_cache;
   p.ks = k_scale; p.vs = v_scale; p.num_blocks = num_blocks; p.bt = block_tables; p.bt_stride = bt_stride;
   p.bt_width = bt_width; p.table_keys = (int)std::min<int64_t>((int64_t)bt_width * KV8_PAGE, INT32_MAX);
-  p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k; p.batch = batch; p.tiles = tile_info;
+  p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k; p.batch = batch; p.tiles = tile_info; p.n_tiles = n_tiles;
   p.hq = hq; p.hkv = hkv;
   p.pos_per_cta = 16;
   while (p.pos_per_cta * 2 * (hq / hkv) <= 2 * PF_ROWS) p.pos_per_cta *= 2;

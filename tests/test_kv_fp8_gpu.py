@@ -773,6 +773,52 @@ def test_grouped_value_scales_far_apart_in_some_groups(cuda, plan):
     ops.check_device_errors()
 
 
+# ------------------------------------------------------------------------------------------ rows and elements
+@pytest.mark.parametrize("listed", [False, True])
+@pytest.mark.parametrize("hq,hkv", [(4, 2), (8, 8), (32, 2), (40, 8)])
+def test_prefill_rows_without_a_tile_are_left(cuda, hq, hkv, listed):
+    """Queries beyond max_seqlen_q, or of no listed tile, are left as they were where the keys are split too,
+    whatever the workspace held; the others are right."""
+    g = gen(730 + hq)
+    seqs = [(2000, 300), (2500, 10), (1700, 200)] if hkv == 2 else [(3000, 300 if hq == 8 else 130)]
+    lens, nq = [p + n for p, n in seqs], [n for _, n in seqs]
+    nb = sum(-(-n // PAGE) for n in lens)
+    k, v, ks, vs = random_cache(g, nb, hkv)
+    table = paged(g, lens, nb, width=16)
+    cu_q, cu_k = ([0] + np.cumsum(x).tolist() for x in (nq, lens))
+    q = torch.randn(cu_q[-1], hq, D, generator=g).to(BF)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    unit = max(64, 16 << max(i for i in range(5) if (16 << i) * (hq // hkv) <= 256))  # rows of a CTA's tile, or 64
+    if listed:  # all but the second tile of each sequence
+        tiles = torch.from_numpy(ops.build_tiles(nq)).view(-1, 2)
+        tiles = tiles[(tiles[:, 1] < unit) | (tiles[:, 1] >= 2 * unit)].contiguous().to(cuda)
+        left = lambda i: unit <= i < 2 * unit  # noqa: E731
+    else:
+        tiles = None
+        left = lambda i: i >= unit  # noqa: E731
+    max_q = max(nq) if listed else unit
+    assert ops.prefill_split_plan_fp8(len(seqs), cu_q[-1], max_q, 16 * PAGE, hq, hkv)[1] > 1
+    junk = [torch.full((1 << 24,), math.nan, device=cuda) for _ in range(2)]  # what a workspace may find
+    del junk
+    out = torch.full((cu_q[-1], hq, D), 2.0, dtype=BF, device=cuda)
+    ops.attention_paged_prefill_fp8(*on(cuda, q, k, v, ks, vs), i32(cu_q), i32(cu_k), max_q, table.to(cuda), 0.1, tiles=tiles,
+                                    out=out)
+    if listed or max(nq) <= unit:
+        ops.check_device_errors()
+    else:
+        with pytest.raises(ops.NativeError, match="inconsistent"):
+            ops.check_device_errors()
+    k64, v64 = values(k, ks), values(v, vs)
+    for b, (past, n) in enumerate(seqs):
+        rest = torch.tensor([left(i) for i in range(n)])
+        rows = out[cu_q[b]:cu_q[b + 1]].cpu()
+        assert bool((rows[rest] == 2.0).all()), f"sequence {b}"
+        for h in (0, hq - 1):
+            kv = [rows_of(c, table[b], 0, lens[b], h // (hq // hkv)) for c in (k64, v64)]
+            ref, mag, most = attend(q[cu_q[b]:cu_q[b + 1], h], [kv], 0.1, past)
+            check_attention(rows[~rest, h], ref[~rest], mag[~rest], most, f"sequence {b} head {h}")
+
+
 # ------------------------------------------------------------------------------------------ store
 def scale_for(top):
     if top == 0:
