@@ -596,7 +596,8 @@ class Qwen3ForCausalLM(nn.Module):
         if config.tie_word_embeddings:
             # separate Parameter sharing storage, as the reference (qwen3_naive.py:830-831)
             self.lm_head.weight.data = self.model.embed_tokens.weight.data
-        self._num_blocks = 0
+        self._num_blocks = 0  # pages of the pool; 0: as many as fit, found out when the pool is made
+        self._auto_blocks = None  # (pages, 8-bit?) so found: the other format's pages have another size
         self._graphs = {}
         self._has_cuda_graphs = False
         self.use_cuda_graphs = True  # decode steps replay captured graphs (False: eager launches)
@@ -645,6 +646,14 @@ class Qwen3ForCausalLM(nn.Module):
         available = int(total * gpu_memory_utilization - used - peak_act)
         return max(available // self._block_bytes(), 1)
 
+    def _drop_kv_cache(self):
+        """Lets go of the pool and of the graphs that were captured on it."""
+        for layer in self.model.layers:
+            at = layer.self_attn
+            at.k_cache = at.v_cache = at.k_scale = at.v_scale = None
+        self._graphs.clear()
+        self._has_cuda_graphs = False
+
     def allocate_global_kv_cache(self):
         """K and V caches [layers, num_blocks, 256, kv_heads, head_dim] bf16; each layer gets a view.  With
         ``kv_cache_dtype = "fp8"``: codes [layers, num_blocks, kv_heads, 256, head_dim] e4m3 and scales
@@ -653,8 +662,12 @@ class Qwen3ForCausalLM(nn.Module):
         fp8 = self._kv_fp8()
         if fp8 and a0.head_dim != 128:
             raise ValueError(f"an 8-bit K/V cache needs heads of 128 elements, not {a0.head_dim}")
+        if self._auto_blocks == (self._num_blocks, not fp8):
+            self._drop_kv_cache()  # the old pool's memory counts as free
+            self._num_blocks = 0
         if not self._num_blocks:
             self._num_blocks = self._compute_num_blocks()
+            self._auto_blocks = (self._num_blocks, fp8)
         if fp8:
             shape = (self._num_blocks, a0.num_kv_heads, self.BLOCK_SIZE, a0.head_dim)
         else:
@@ -663,11 +676,7 @@ class Qwen3ForCausalLM(nn.Module):
             return
         dev = self.lm_head.weight.device
         L = len(self.model.layers)
-        for layer in self.model.layers:  # drop old views before allocating the new pool
-            at = layer.self_attn
-            at.k_cache = at.v_cache = at.k_scale = at.v_scale = None
-        self._graphs.clear()
-        self._has_cuda_graphs = False
+        self._drop_kv_cache()
         if fp8:
             k, v, ks, vs = ops.kv_cache_fp8(L * self._num_blocks, a0.num_kv_heads, dev)
             ks, vs = (s.view(L, self._num_blocks, *s.shape[1:]) for s in (ks, vs))

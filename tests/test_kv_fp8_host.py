@@ -103,3 +103,39 @@ def test_plans_cover_the_context(batch, hkv, ctx):
 def test_prefill_plan_covers_the_keys(batch, total_q, max_q, hq, hkv, max_k):
     split, n = ops.prefill_split_plan_fp8(batch, total_q, max_q, max_k, hq, hkv)
     assert (split, n) == (0, 1) or (split % 128 == 0 and n > 1 and (n - 1) * split < max_k <= n * split)
+
+
+def test_automatic_page_count_follows_the_cache_format(monkeypatch):
+    """A pool sized to what memory holds is sized anew when the format changes (its pages take another number of
+    bytes), after the old pool has been let go; a count that the user set stays."""
+    from qwen3_naive_inference_b200.qwen3_naive import Qwen3Config, Qwen3ForCausalLM
+    model = Qwen3ForCausalLM(Qwen3Config(hidden_size=64, num_attention_heads=2, num_key_value_heads=1, head_dim=128,
+                                         intermediate_size=64, num_hidden_layers=2, vocab_size=32, max_position_embeddings=512))
+    at = model.model.layers[1].self_attn
+    budget, asked = 20 * 2 * 2 * 256 * 128 * 2, []
+
+    def count():
+        assert at.k_cache is None and at.v_scale is None and not model._has_cuda_graphs
+        asked.append(model.kv_cache_dtype)
+        return budget // model._block_bytes()
+
+    monkeypatch.setattr(model, "_compute_num_blocks", count)
+
+    def pool():
+        model.allocate_global_kv_cache()
+        t = [c for c in (at.k_cache, at.v_cache, at.k_scale, at.v_scale) if c is not None]
+        assert all(c.shape[0] == model._num_blocks for c in t)
+        return 2 * sum(c.numel() * c.element_size() for c in t)
+
+    for dtype, pages in (("bf16", 20), ("fp8", 39), ("bf16", 20), ("fp8", 39)):
+        model.kv_cache_dtype = dtype
+        model._has_cuda_graphs = at.k_cache is not None
+        assert pool() <= budget and model._num_blocks == pages
+        kept = at.k_cache
+        assert pool() <= budget and at.k_cache is kept  # nothing changed: the pool stays
+    assert asked == ["bf16", "fp8", "bf16", "fp8"]
+    model._num_blocks = 7  # the user's
+    for dtype in ("bf16", "fp8", "bf16"):
+        model.kv_cache_dtype = dtype
+        pool()
+        assert model._num_blocks == 7 and asked[4:] == []
