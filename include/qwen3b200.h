@@ -211,7 +211,10 @@ size_t qb_paged_decode_grouped_workspace_bytes(int batch, int hq, int D, int n_s
  * kept).  A block's scale is the smallest power of two, at least 2^-126, under which every finite value
  * appended since its first row lies within 448.  A call that writes the first row of a block begins it
  * anew; otherwise a larger value raises the scale and the rows already there are rounded again.  What is
- * not finite is stored as NaN.  The tokens of a call may be in any order. */
+ * not finite is stored as NaN.  The tokens of a call may be in any order.
+ *
+ * The attentions: scales are not negative.  A NaN code of a key makes the rows that attend it NaN, one of a value that
+ * element of those rows, in every form alike. */
 int qb_qk_norm_rope_store_fp8(const void* qkv, int64_t T, int64_t ld_in, int hq, int hkv, int D,
                               const int64_t* positions, const float* cos_sin, int64_t max_pos,
                               const void* q_norm_w, const void* k_norm_w, float eps, void* q_out,

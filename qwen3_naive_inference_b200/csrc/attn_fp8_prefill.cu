@@ -26,7 +26,8 @@
 // still hold probability: it gives P = 0 and its sum is taken from 2^(x - lref).
 // Keys behind a row's last one take a score of -inf; their V must not count either, so codes past the
 // sequence are zeroed and, in tiles that some row sees in part, NaN codes of V are zeroed too and their
-// keys noted: a row that does attend such a key becomes NaN.
+// keys noted: in a row that does attend such a key its NaN elements become NaN at the end (the codes are read once
+// more), as the product makes them in tiles that every row sees.
 // Few rows over many keys: the keys are split over CTAs, which write normalised partial outputs and the
 // rows' log-sums for a second kernel to join.
 //
@@ -60,8 +61,9 @@ constexpr int PF_Q = 0, PF_K = 2 * PF_Q_TILE, PF_V = PF_K + PF_STAGES * PF_KV_TI
 constexpr int PF_META = PF_V + PF_STAGES * PF_KV_TILE;
 constexpr int PF_SLOTS = 8, PF_SLOT = 4;           // tiles whose scales are held, words of one
 constexpr int PF_BARS = 4 * PF_STAGES + 20;
-// barriers; TMEM slot, abort flag; row factors; per slot the tile's scales and NaN keys
-constexpr int PF_SMEM = PF_META + PF_BARS * 8 + 8 + 2 * PF_ROWS * 4 + PF_SLOTS * PF_SLOT * 4 + 1024 /*align*/;
+// barriers; TMEM slot, abort flag; row factors; per slot the tile's scales and NaN keys; what the end needs
+constexpr int PF_KEPT = PF_META + PF_BARS * 8 + 8 + 2 * PF_ROWS * 4 + PF_SLOTS * PF_SLOT * 4, PF_KEPT_BYTES = 64;
+constexpr int PF_SMEM = PF_KEPT + PF_KEPT_BYTES + 1024 /*align*/;
 constexpr uint32_t PF_COL_S = 0, PF_COL_O = 256;   // S: + 128 * query tile + 64 * buffer; O: + 128 * query tile
 constexpr float PF_HEAD = 7.f, PF_SLACK = 15.f;    // ref = largest - 7; moves when one is above ref + 15
 constexpr float PF_APART = -100.f;                 // log2 of a share of O below which P is taken as zero
@@ -118,6 +120,20 @@ QB_DEVICE uint32_t operand_chunk(int r, int c, int half) {
   return (uint32_t)((c >> 3) * half + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
+// What a CTA works on.
+struct PrefillWork {
+  int b, q0, lq, shift, kvh;  // sequence, first query position, queries, Lk - Lq
+  int64_t row0;               // row of the sequence's first query
+  int rows, begin, end;       // query rows; keys [begin, end)
+  int n[2];                   // key tiles of query tiles A and B
+};
+// What the end of a CTA needs of it, so that nobody holds it in registers until then.
+struct PrefillKept {
+  PrefillWork work;
+  int nan;  // has a converter taken out a NaN value?
+};
+static_assert(sizeof(PrefillKept) <= PF_KEPT_BYTES && PF_KEPT % alignof(PrefillKept) == 0, "layout");
+
 struct PrefillSmem {
   uint32_t base;
   uint8_t* ptr;
@@ -148,14 +164,7 @@ struct PrefillSmem {
   // Eight slots: a slot is written for tile j + 8 when S of j + 4 is done, so the softmax is past j + 2.
   QB_DEVICE float* scales(int j) const { return row_fac() + 2 * PF_ROWS + j % PF_SLOTS * PF_SLOT; }
   QB_DEVICE uint32_t* nan_keys(int j) const { return reinterpret_cast<uint32_t*>(scales(j) + 2); }
-};
-
-// What a CTA works on.
-struct PrefillWork {
-  int b, q0, lq, shift, kvh;  // sequence, first query position, queries, Lk - Lq
-  int64_t row0;               // row of the sequence's first query
-  int rows, begin, end;       // query rows; keys [begin, end)
-  int n[2];                   // key tiles of query tiles A and B
+  QB_DEVICE PrefillKept* kept() const { return reinterpret_cast<PrefillKept*>(ptr + PF_KEPT); }
 };
 
 // Sixteen codes as halves into chunks 2c and 2c + 1 of row r.
@@ -236,6 +245,7 @@ QB_DEVICE void prefill_convert(const PrefillP& p, const PrefillSmem& sm, const P
           c.v[i].w &= ~((bad[3] >> 7) * 0xffu);
           const int key = row0 + 16 * i;
           atomicOr(&sm.nan_keys(j)[key >> 5], 1u << (key & 31));
+          sm.kept()->nan = 1;
         }
       }
     }
@@ -498,15 +508,7 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
   tc_fence_after();
   // 2^(ref - lref) / l in two factors: value scales reach both ends of the exponent range
   const float units = ref == -INFINITY ? 0.f : ref - lref, half = rintf(0.5f * units), back = exp2f(half);
-  float inv = l == 0.f ? 0.f : exp2f(units - half) / l;
-  // NaN values that the converters took out of the tiles some row sees in part (every V has been read)
-  for (int j = max(0, w.shift + w.q0 + 1 - w.begin) / PF_KEYS; j < n; ++j)
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int m = last - (w.begin + j * PF_KEYS + 32 * k) + 1;  // keys of the word that the row sees
-      const uint32_t mine = m >= 32 ? 0xffffffffu : (m <= 0 ? 0u : (1u << m) - 1u);
-      if (sm.nan_keys(j)[k] & mine) inv = __int_as_float(0x7fffffff);
-    }
+  const float inv = l == 0.f ? 0.f : exp2f(units - half) / l;
   const int64_t row = w.row0 + pos;
   const int head = w.kvh * group + R % group;
   bf16* out = p.out + row * p.o_stride + head * KV8_D;
@@ -535,6 +537,31 @@ QB_DEVICE void prefill_softmax(const PrefillP& p, const PrefillSmem& sm, const P
     }
   }
   if (live && p.n_splits > 1) ws[KV8_D] = l == 0.f ? -INFINITY : lref + log2f(l);
+}
+
+// NaN values that the converters took out of the tiles some row sees in part, into the elements of the rows that do
+// attend them, after the rows have been written.  A thread per row and half of its elements.
+QB_DEVICE void prefill_put_nan(const PrefillP& p, const PrefillSmem& sm, int split) {
+  const PrefillWork w = sm.kept()->work;
+  const int group = p.hq / p.hkv, R = threadIdx.x & 255, e0 = (threadIdx.x >> 8) * 64, n = w.n[R / PF_ROWS];
+  if (R >= w.rows) return;
+  const int64_t row = w.row0 + w.q0 + R / group;
+  const int head = w.kvh * group + R % group, last = min(w.shift + w.q0 + R / group, w.end - 1);
+  for (int j = max(0, w.shift + w.q0 + 1 - w.begin) / PF_KEYS; j < n; ++j)
+    for (int k = 0; k < 2; ++k) {
+      const int m = last - (w.begin + j * PF_KEYS + 32 * k) + 1;  // keys of the word that the row sees
+      const uint32_t seen = m >= 32 ? 0xffffffffu : (m <= 0 ? 0u : (1u << m) - 1u);
+      for (uint32_t keys = sm.nan_keys(j)[k] & seen; keys != 0; keys &= keys - 1) {
+        const int key = w.begin + j * PF_KEYS + 32 * k + __ffs(keys) - 1;
+        const int page = p.bt[(int64_t)w.b * p.bt_stride + key / KV8_PAGE];  // in the pool, or there would be no NaN
+        const uint8_t* codes = p.v + (((int64_t)page * p.hkv + w.kvh) * KV8_PAGE + key % KV8_PAGE) * KV8_D;
+        for (int e = e0; e < e0 + 64; ++e) {
+          if ((codes[e] & 0x7f) != 0x7f) continue;
+          if (p.n_splits > 1) p.ws[((row * p.hq + head) * p.n_splits + split) * PF_WS_ROW + e] = __int_as_float(0x7fffffff);
+          else p.out[row * p.o_stride + head * KV8_D + e] = f2bf(__int_as_float(0x7fffffff));
+        }
+      }
+    }
 }
 
 __global__ void __launch_bounds__(PF_THREADS, 1)
@@ -607,6 +634,8 @@ prefill_fp8_kernel(PrefillP p) {
     *sm.abort_flag() = 0;
     // tiles that some row sees in part are the last five at most: their slots' NaN keys are written once
     for (int j = 0; j < PF_SLOTS; ++j) sm.nan_keys(j)[0] = sm.nan_keys(j)[1] = 0;
+    sm.kept()->work = w;
+    sm.kept()->nan = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 12) {
@@ -633,6 +662,7 @@ prefill_fp8_kernel(PrefillP p) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   }
+  if (__builtin_expect(sm.kept()->nan, 0)) prefill_put_nan(p, sm, split);
 }
 
 // Joins the key splits of a (row, head): a warp each, weights 2^(lse - largest lse), over the splits that

@@ -819,6 +819,53 @@ def test_prefill_rows_without_a_tile_are_left(cuda, hq, hkv, listed):
             check_attention(rows[~rest, h], ref[~rest], mag[~rest], most, f"sequence {b} head {h}")
 
 
+def check_with_nan(out, q, k, v, scale, past=None, msg=""):
+    """Element d of a row is NaN exactly where a key that the row attends has NaN in element d of its value."""
+    at = ~torch.isfinite(v)
+    ref, mag, most = attend(q, [[k, torch.where(at, 0.0, v)]], scale, past)
+    sees = torch.ones(q.shape[0], k.shape[0], dtype=torch.bool)
+    if past is not None:
+        sees = torch.arange(k.shape[0]) <= past + torch.arange(q.shape[0])[:, None]
+    want = (sees.double() @ at.double()) > 0
+    out = out.cpu()
+    assert torch.equal(out.isnan(), want), f"{msg} NaN in {int(out.isnan().sum())} elements, not {int(want.sum())}"
+    check_attention(torch.where(want, torch.zeros_like(out), out), torch.where(want, 0.0, ref), mag, most, msg)
+
+
+@pytest.mark.parametrize("hq,hkv", [(4, 2), (8, 8), (32, 2), (5, 1)])
+@pytest.mark.parametrize("past", [0, 90, 1500])
+def test_nan_values_reach_their_element_of_the_rows_that_attend_them(cuda, hq, hkv, past):
+    """Whatever the tile that holds them -- one that every row sees, or one that some rows see in part --
+    and in decode as in prefill, in one split and in several."""
+    g = gen(740 + hq + past)
+    n = 300
+    nb = -(-(past + n) // PAGE)
+    k, v, ks, vs = random_cache(g, nb, hkv)
+    table = paged(g, [past + n], nb)
+    for _ in range(14):
+        key, h = int(torch.randint(0, past + n, (1,), generator=g)), int(torch.randint(0, hkv, (1,), generator=g))
+        e = torch.randint(0, D, (2,), generator=g)
+        v.view(torch.uint8)[int(table[0, key // PAGE]), h, key % PAGE, e] = torch.tensor([0x7F, 0xFF], dtype=torch.uint8)
+    q = torch.randn(n, hq, D, generator=g).to(BF)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    args = on(cuda, q, k, v, ks, vs)
+    k64, v64 = values(k, ks), values(v, vs)
+    wide = torch.full((1, 64), -1, dtype=torch.int32)
+    wide[:, :nb] = table
+    outs = [ops.attention_paged_prefill_fp8(*args, i32(0, n), i32(0, past + n), n, t.to(cuda), 0.1) for t in (table, wide)]
+    at = [0, 63, 64, 150, n - 1]
+    dec = [ops.paged_decode_attention_fp8(args[0][at], *args[1:], table.to(cuda).expand(len(at), -1), i32(*[past + i for i in at]),
+                                          0.1, **kw) for kw in ({}, {"split_tokens": 128, "max_splits": 15})]
+    for h in range(hq):
+        kv = [rows_of(c, table[0], 0, past + n, h // (hq // hkv)) for c in (k64, v64)]
+        for out in outs:
+            check_with_nan(out[:, h], q[:, h], *kv, 0.1, past, f"prefill head {h}")
+        for out in dec:
+            for r, i in enumerate(at):
+                check_with_nan(out[r:r + 1, h], q[i:i + 1, h], *[c[:past + i + 1] for c in kv], 0.1, None, f"decode {i} head {h}")
+    ops.check_device_errors()
+
+
 # ------------------------------------------------------------------------------------------ store
 def scale_for(top):
     if top == 0:
