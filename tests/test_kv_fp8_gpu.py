@@ -866,6 +866,31 @@ def test_nan_values_reach_their_element_of_the_rows_that_attend_them(cuda, hq, h
     ops.check_device_errors()
 
 
+def test_infinite_queries_give_nan(cuda):
+    """A head whose query holds an infinity: some score is +inf, the softmax has no value, all of the head's
+    outputs are NaN; the other heads and rows are as before.  One split and several."""
+    g = gen(750)
+    k, v, ks, vs = random_cache(g, 3, 2)
+    table = torch.tensor([[1, 0, 2]], dtype=torch.int32)
+    q = torch.randn(3, 4, D, generator=g).to(BF)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    args = on(cuda, k, v, ks, vs)
+    wide = torch.cat([table, torch.full((1, 29), -1, dtype=torch.int32)], 1).to(cuda)
+    calls = [lambda x: ops.paged_decode_attention_fp8(x, *args, table.to(cuda).expand(3, -1), i32(600, 99, 700), 0.1),
+             lambda x: ops.paged_decode_attention_fp8(x, *args, table.to(cuda).expand(3, -1), i32(600, 99, 700), 0.1,
+                                                      split_tokens=64, max_splits=12),
+             lambda x: ops.attention_paged_prefill_fp8(x, *args, i32(0, 3), i32(0, 700), 3, table.to(cuda), 0.1),
+             lambda x: ops.attention_paged_prefill_fp8(x, *args, i32(0, 3), i32(0, 700), 3, wide, 0.1)]
+    for value in (math.inf, -math.inf):
+        bad = q.clone()
+        bad[1, 3, 0] = value
+        for i, call in enumerate(calls):
+            a, b = call(q.to(cuda)), call(bad.to(cuda))
+            assert bool(b[1, 3].isnan().all()), f"call {i}"
+            assert torch.equal(a[[0, 2]], b[[0, 2]]) and torch.equal(a[1, :3], b[1, :3]), f"call {i}"
+    ops.check_device_errors()
+
+
 # ------------------------------------------------------------------------------------------ store
 def scale_for(top):
     if top == 0:
