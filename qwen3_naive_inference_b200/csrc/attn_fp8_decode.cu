@@ -19,13 +19,13 @@
 //   O^T += vs V^T P^T   the 128 head elements are the M rows (8 tiles), the warp's 16 keys the K dimension,
 //                  so a tile's product is one mma per 16 elements: vs, one number a tile, joins with the
 //                  fp32 accumulator.
-// Where a CTA's tiles have scales more than 2^8 apart, a probability that is nothing beside the largest may still
+// Where a CTA's tiles have scales more than 16 times its first one's, or less than a 16th, a probability that is nothing beside the largest may still
 // make the output (and near the ends of the exponent range vs P V leaves it).  The producer, which has the scales in
 // hand, sees it; the CTA then writes nothing and takes a second pass, which weighs before it rounds:
 // P = 2^(x + log2 vs - oref), where oref follows the largest x + log2 vs as ref does x, O counts in units of 2^oref,
 // and the sum takes sum(P) 2^(oref - log2 vs - ref).  That form for all CTAs cost 10% (512 sequences of up to 1024
 // keys 98 -> 109 us), a choice between the two inside the loop 3%; the second pass costs calls that do not take it
-// 0.2% (plain) and 2% (64 groups 83.0 -> 84.6, five small groups 12.2 -> 12.5).
+// nothing (plain) to 1.4% (16 groups of 8, 40 over 8 heads 38.7 -> 39.3; 64 groups, 16 over 8 heads 82.8 -> 83.2).
 // The order of head elements and keys inside a product is free, so every operand comes straight from
 // 16-byte shared-memory reads (conflict-free under the TMA swizzle) without a transpose but for the
 // byte pairs of V (prmt) and P (movmatrix).
@@ -44,6 +44,8 @@
 // Fewer warps a CTA and more CTAs an SM (two warps, four to six CTAs: 110 to 120 us for the 512 sequences), three
 // stages and four CTAs (111), CTAs that live on and take sequence after sequence (127) or equal shares of all
 // keys (133) were slower.
+#include <float.h>
+
 #include "attn_fp8.cuh"
 
 namespace {
@@ -60,9 +62,10 @@ constexpr int DC_LEFT = DC_MOST + 4;  // set where a work's scales were far apar
 constexpr int DC_SMEM = DC_STAGES * DC_STAGE_BYTES + DC_META + 1024 /*align*/;
 static_assert(DC_WARPS * 16 * DC_O_ROW * 4 <= DC_STAGES * DC_STAGE_BYTES, "the join reuses the stages");
 constexpr float DC_HEAD = 7.f, DC_SLACK = 15.f;    // ref = max - 7; moves when a score is above ref + 15
-// Largest ratio of a CTA's scales, and the range of their largest, without weighing before rounding: a P that is lost
-// (2^-32 of the largest) is then at most 2^-24 of the output's largest share, and |O| below 2^15 * 448 * 8192 vs.
-constexpr float DC_NEAR = 256.f, DC_VS_LEAST = 0x1p-100f, DC_VS_MOST = 0x1p60f;
+// How far a CTA's scales may be from its first tile's, and the range of that, without weighing before rounding: a P
+// that is lost (2^-32 of the largest) is then at most 2^-24 of the output's largest share, and |O| below
+// 2^15 * 448 * 8192 * 16 vs.
+constexpr float DC_NEAR = 16.f, DC_VS_LEAST = 0x1p-100f, DC_VS_MOST = 0x1p60f;
 // Weighed, a tile whose scale is less than 2^-50 of the largest (a block of zeros under the smallest scale, say) may
 // hold probability although its P, as small as 2^-126, does not: its sum is taken from 2^(x - ref).  Within 2^50
 // a P below 2^-100 has x - ref below -42: with x', vs' of the key that set oref, oref is at most x' + log2 vs' - 7,
@@ -285,7 +288,7 @@ QB_DEVICE int decode_work(const DecodeP& p, const DecodeMaps& maps, const int (&
   float* vs_of = ks_of + DC_MAX_TILES;
   float* join = vs_of + DC_MAX_TILES;  // [warp][16] ref, [warp][16] l
   float* oref = join + 2 * DC_WARPS * 16;   // [warp][16], where P is weighed
-  float* most_of = oref + DC_WARPS * 16;    // the largest scale where P is weighed, else 0
+  float* most_of = oref + DC_WARPS * 16;    // where P is weighed (by then) the largest scale, else 0
   int* left_of = reinterpret_cast<int*>(most_of + 1);
 
   if (warp == DC_WARPS) {
@@ -384,22 +387,28 @@ QB_DEVICE int decode_work(const DecodeP& p, const DecodeMaps& maps, const int (&
         vs_of[lane + 32 * j] = vs[j];
       }
     __syncwarp();
-    auto look = [&] {  // are the scales far apart?  (They are not negative: their bits order as they do.)
-      uint32_t least = ~0u, most = 0;
+    // Are the scales far apart?  Both passes ask the same way.
+    auto look = [&] {
+      const float v0 = __shfl_sync(0xffffffffu, vs[0], 0), up = v0 * DC_NEAR, down = v0 / DC_NEAR;
+      bool far = v0 < DC_VS_LEAST || v0 > DC_VS_MOST;
 #pragma unroll
-      for (int j = 0; j < DC_LANE_TILES; ++j)
-        if (lane + 32 * j < n) {  // (a tile without a page counts as a scale of zero)
-          least = min(least, __float_as_uint(vs[j]));
-          most = max(most, __float_as_uint(vs[j]));
-        }
-      const float lo = __uint_as_float(__reduce_min_sync(0xffffffffu, least)), hi = __uint_as_float(__reduce_max_sync(0xffffffffu, most));
-      const bool apart = hi > 0.f && (hi > DC_NEAR * lo || hi < DC_VS_LEAST || hi > DC_VS_MOST);
-      if (lane == 0) *most_of = apart ? hi : 0.f;
-      if (lane == 0 && apart) *left_of = 1;
+      for (int j = 0; j < DC_LANE_TILES; ++j) far |= lane + 32 * j < n && (vs[j] > up || vs[j] < down);
+      return __any_sync(0xffffffffu, far) && n > 0;
     };
-    if (WEIGH) look();
+    if (WEIGH) {
+      float most = FLT_MIN;  // (scales may all be zero)
+#pragma unroll
+      for (int j = 0; j < DC_LANE_TILES; ++j) most = fmaxf(most, vs[j]);
+      most = warp_max(most);
+      const bool far = look();
+      if (lane == 0) *most_of = far ? most : 0.f;
+    }
     if (lane == 0) mbar_arrive(ready);
-    if (!WEIGH) look();  // off the way to the first tile
+    if (!WEIGH) {  // off the way to the first tile
+      const bool far = look();
+      if (lane == 0) *most_of = far ? 1.f : 0.f;
+      if (lane == 0 && far) *left_of = 1;
+    }
     if (lane == 0) {
       issue_to(n);
       // never leave with a copy in flight into this CTA's shared memory

@@ -744,6 +744,27 @@ def test_decode_value_blocks_of_zeros_take_their_probability(cuda):
         check_decode_values(cuda, q, cache, table, kv, msg)
 
 
+def test_a_zeroed_cache_gives_zeros(cuda):
+    """Scales of zero everywhere, as a cache is made: every form writes zeros."""
+    k, v, ks, vs = ops.kv_cache_fp8(3, 2, cuda)
+    q = torch.randn(20, 4, D, generator=gen(726)).to(BF).to(cuda)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    table, out = i32(2, 0, 1).view(1, 3), torch.full((1, 4, D), 3.0, dtype=BF, device=cuda)
+    members, shared = i32(0, *[-1] * 255).view(32, 8), i32(512, *[0] * 31)
+    calls = [lambda kw=kw: ops.paged_decode_attention_fp8(q[:1], k, v, ks, vs, table, i32(699), 0.1, out=out, **kw)
+             for kw in ({}, {"split_tokens": 128, "max_splits": 6})]
+    calls += [lambda plan=plan: ops.paged_decode_attention_grouped_fp8(q[:1], k, v, ks, vs, table, i32(699), 0.1, members,
+                                                                       shared, i32(512), plan, out=out)
+              for plan in ((32, 512, 1, 192, 1), (1, 192, 3, 64, 3))]
+    for i, call in enumerate(calls):
+        out.fill_(3.0)
+        assert not bool(call().any()), f"call {i}"
+    for t in (table, torch.cat([table, i32(*[-1] * 21).view(1, 21)], 1)):
+        assert not bool(ops.attention_paged_prefill_fp8(q, k, v, ks, vs, i32(0, 20), i32(0, 700), 20, t, 0.1,
+                                                        out=torch.full_like(q, 3.0)).any())
+    ops.check_device_errors()
+
+
 @pytest.mark.parametrize("plan", [(10, 192, 1, 192, 1), (10, 64, 3, 64, 3)])
 def test_grouped_value_scales_far_apart_in_some_groups(cuda, plan):
     """CTAs that take several groups one after another, some of them with value scales far apart: those follow the
