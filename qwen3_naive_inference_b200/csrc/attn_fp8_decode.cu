@@ -33,11 +33,15 @@
 // NaN codes of a recycled page included).  Pages outside the pool are reported and their tile skipped.
 //
 // Measured on a B200 (16 query and 8 kv heads, 128 elements; a plain copy reaches 6.52 TB/s):
-//   512 sequences of 64 to 1024 keys      97.3 us, 556 MB: 5.7 TB/s
+//   512 sequences of 64 to 1024 keys      98 us, 556 MB: 5.7 TB/s (one state again and again; 101 to 107, by box, where
+//                                         the caches change from call to call: 5.2 to 5.5)
 //   16 sequences of 2048 to 32768 keys      88 us, 458 MB: 5.2 TB/s (ragged lengths: CTAs end at different times);
 //                                         as many bytes in equal lengths: 6.5 TB/s and more
-//   one sequence of 700 keys              8.4 us: the chain of lookups (length, page, scale), copy and join
-//   64 groups of 8, 64 to 512 shared and 170 to 512 own keys   82 us, 404 MB: 4.9 TB/s
+//   one sequence of 700 keys              8.6 us: the chain of lookups (length, page, scale), copy and join
+//   64 groups of 8, 64 to 512 shared and 170 to 512 own keys   83 us, 404 MB: 4.9 TB/s (84 to 86 where the caches change)
+//   16 groups of 8, 87 to 700 shared and 100 to 300 own keys   40 over 8 heads 40 us, 70 MB; 32 over 4 heads 26 us, 35 MB:
+//                                         a quarter and a fifth of HBM; with five heads and more a kv head a CTA takes one
+//                                         member, so each streams the shared keys for itself, from L2 if not from HBM
 // What a CTA needs before its first and after its last tile is as long as two to four tiles, and three CTAs of an
 // SM hide it only in part: 4096 CTAs of one key each take 21 us.  Longer work a CTA (decode_whole_fp8_kernel) pays
 // where members share it, not for plain sequences of these lengths (512 of up to 750 keys: 86 us against 80).

@@ -32,11 +32,11 @@
 // rows' log-sums for a second kernel to join.
 //
 // Measured on a B200 (16 query and 8 kv heads):
-//   2048 queries over 32768 keys        584 us, 533 GFLOP: 912 TFLOP/s (a plain matrix product: 1662)
-//   2048 over 8192                      154 us: 780 TFLOP/s
-//   8 fresh prompts of 256 to 512       35.5 us; 11 short sequences 18.2 us: a CTA's start, first tile and end,
+//   2048 queries over 32768 keys        562 to 572 us by box, 533 GFLOP: 940 TFLOP/s (a plain matrix product: 1662)
+//   2048 over 8192                      150 us: 800 TFLOP/s
+//   8 fresh prompts of 256 to 512       35.5 us; 11 short sequences 18.6 us: a CTA's start, first tile and end,
 //                                       8 us of every call
-// Of the long case: tensor pipe and exponential unit are busy 44 and 45% of the time each, issue slots 44%.  No
+// Of 2048 over 8192: tensor pipe and exponential unit are busy 46 and 47% of the time each, issue slots 47%.  No
 // single one holds it up: without the exponentials it took 10% less, with an eighth of the MMAs 5%.  What a softmax
 // warp does to a tile -- load, maximum, exponentials, store, each waiting for the one before -- is the period, about
 // 2200 cycles, of which the exponential unit needs 1024 for its two warps.  Turns at that unit, eight converter warps,

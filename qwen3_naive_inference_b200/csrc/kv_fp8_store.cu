@@ -19,8 +19,8 @@
 // not, and as many heads share a scan as leave enough CTAs.
 //
 // Bound by HBM: 2 bytes read and 2 (q) or 1 (codes) written an element.  Measured on a B200 (16 query and 8 kv
-// heads): one token 2.5 us; 512 tokens in 512 blocks 6.0 us (the rows and scales of a step are 8 MB: latency);
-// 37 chunks, 10361 tokens, 45.6 us for 154 MB, 3.4 TB/s: a block's CTA loads, meets at a barrier for the scale and
+// heads): one token 2.8 us; 512 tokens in 512 blocks 6.3 us (the rows and scales of a step are 8 MB: latency);
+// 37 chunks, 10361 tokens, 45.4 us for 154 MB, 3.4 TB/s: a block's CTA loads, meets at a barrier for the scale and
 // then stores, and two CTAs an SM overlap only in part.
 #include <float.h>
 

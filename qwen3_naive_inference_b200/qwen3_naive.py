@@ -811,7 +811,8 @@ class Qwen3ForCausalLM(nn.Module):
         return ("split", split_tokens, max_splits, ws)
 
     def _grouped_plan(self, bs, max_shared, max_own):
-        """(plan, workspace) of the grouped decode attention for ``bs`` sequences."""
+        """(plan, workspace) of the grouped decode attention for ``bs`` sequences (8-bit cache: in groups of eight;
+        more and smaller groups are walked several to a CTA)."""
         a = self.model.layers[0].self_attn
         dev = self.lm_head.weight.device
         if self._kv_fp8():
