@@ -19,13 +19,13 @@
 //   O^T += vs V^T P^T   the 128 head elements are the M rows (8 tiles), the warp's 16 keys the K dimension,
 //                  so a tile's product is one mma per 16 elements: vs, one number a tile, joins with the
 //                  fp32 accumulator.
-// Where a CTA's tiles have scales more than 16 times its first one's, or less than a 16th, a probability that is nothing beside the largest may still
-// make the output (and near the ends of the exponent range vs P V leaves it).  The producer, which has the scales in
-// hand, sees it; the CTA then writes nothing and takes a second pass, which weighs before it rounds:
-// P = 2^(x + log2 vs - oref), where oref follows the largest x + log2 vs as ref does x, O counts in units of 2^oref,
-// and the sum takes sum(P) 2^(oref - log2 vs - ref).  That form for all CTAs cost 10% (512 sequences of up to 1024
-// keys 98 -> 109 us), a choice between the two inside the loop 3%; the second pass costs calls that do not take it
-// nothing (plain) to 1.4% (16 groups of 8, 40 over 8 heads 38.7 -> 39.3; 64 groups, 16 over 8 heads 82.8 -> 83.2).
+// Where a CTA's tiles have scales over 16 times its first one's, or under a 16th, a probability that is nothing beside
+// the largest may still make the output (and near the ends of the exponent range vs P V leaves it).  The producer,
+// which has the scales in hand, sees it; the CTA then writes nothing and takes a second pass, which weighs before it
+// rounds: P = 2^(x + log2 vs - oref), where oref follows the largest x + log2 vs as ref does x, O counts in units of
+// 2^oref, and the sum takes sum(P) 2^(oref - log2 vs - ref).  That form for all CTAs cost 10% (512 sequences of up to
+// 1024 keys 98 -> 109 us), a choice between the two inside the loop 3%; the second pass costs calls that do not take
+// it nothing (plain) to 2% (16 groups of 8, 32 over 4 heads 25.6 -> 26.1; 64 groups, 16 over 8 heads 82.9 -> 83.4).
 // The order of head elements and keys inside a product is free, so every operand comes straight from
 // 16-byte shared-memory reads (conflict-free under the TMA swizzle) without a transpose but for the
 // byte pairs of V (prmt) and P (movmatrix).
@@ -275,7 +275,7 @@ QB_DEVICE float4 join_weighed(const float* so, const float* orefs, float m, floa
 // Nothing is written of work whose scales are far apart (for WEIGH: are not), which `*most_of` says.  Returns the tiles.
 template <int NT, bool SHARED, bool WHOLE, bool WEIGH>
 QB_DEVICE int decode_work(const DecodeP& p, const DecodeMaps& maps, const int (&pages)[DC_LANE_TILES], uint8_t* smem,
-                           uint32_t base, const Work& w, int kvh, const int32_t* members, int b, int u0, int item) {
+                          uint32_t base, const Work& w, int kvh, const int32_t* members, int b, int u0, int item) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   int n = (w.end - w.begin + KV8_BLOCK - 1) / KV8_BLOCK;
   const int group = p.hq / p.hkv;
@@ -291,8 +291,8 @@ QB_DEVICE int decode_work(const DecodeP& p, const DecodeMaps& maps, const int (&
   float* ks_of = reinterpret_cast<float*>(part_of + DC_MAX_TILES);
   float* vs_of = ks_of + DC_MAX_TILES;
   float* join = vs_of + DC_MAX_TILES;  // [warp][16] ref, [warp][16] l
-  float* oref = join + 2 * DC_WARPS * 16;   // [warp][16], where P is weighed
-  float* most_of = oref + DC_WARPS * 16;    // where P is weighed (by then) the largest scale, else 0
+  float* oref = join + 2 * DC_WARPS * 16;  // [warp][16], WEIGH
+  float* most_of = oref + DC_WARPS * 16;   // 0, or not (WEIGH: the largest scale) where the scales are far apart
   int* left_of = reinterpret_cast<int*>(most_of + 1);
 
   if (warp == DC_WARPS) {
